@@ -313,6 +313,30 @@ int cuda_dispatch_rope_kv_page_write(CUDADeviceRef contextRef, int elementDType,
                                      double lowFreqFactor, double highFreqFactor, uint32_t originalContext, uint64_t completionToken,
                                      CUDAStatus* status);
 
+/* ---- paged KV in 4 bits (no counterpart in the reference) ----
+   A vector x of one (token, KV head) is held as 16 levels between its extremes:
+     least = round(min x), step = round((max x - min x) / 15), code = clamp(rint((x - least) / step), 0, 15), value = least + step * code,
+   round = to elementDType (f16 / bf16).  A vector with a NaN or an infinity reads back as NaN.
+     codes  [pageCount, kvHeads, pageSize, headDim / 2] bytes: byte j = element 2j (low four bits) and 2j + 1 (high)
+     params [pageCount, kvHeads, pageSize, 2] elementDType: (step, least)
+   headDim is 64 or 128; pools are 16-byte aligned; any page size. */
+/* NEW: cuda_dispatch_rope_kv_page_write for these pools: RoPE(k) at positions[row] in float32 (not rounded to elementDType in between),
+   then K and V quantised and written in place.  ropeMode: 0 interleaved, 1 half, 2 = K already rotated (positionsRef may be NULL).
+   Rows whose page, offset or position (>= maxPositions) is out of range are skipped and raise the context's error flag.  Two rows
+   aimed at the same (page, offset) within one call race: the slot then holds neither. */
+int cuda_dispatch_rope_kv_page_write_q4(CUDADeviceRef contextRef, int elementDType, CUDABufferRef kRef, CUDABufferRef vRef,
+                                        CUDABufferRef positionsRef, CUDABufferRef pageIDsRef, CUDABufferRef offsetsRef,
+                                        CUDABufferRef kCodesRef, CUDABufferRef kParamsRef, CUDABufferRef vCodesRef,
+                                        CUDABufferRef vParamsRef, uint32_t rows, uint32_t kvHeads, uint32_t headDim, uint32_t pageCount,
+                                        uint32_t pageSize, uint32_t maxPositions, uint32_t ropeMode, double baseFreq, uint32_t scaling,
+                                        double scalingFactor, double lowFreqFactor, double highFreqFactor, uint32_t originalContext,
+                                        uint64_t completionToken, CUDAStatus* status);
+/* NEW: cuda_dispatch_kv_page_gather from one such pool: output [outRows, kvHeads * headDim] elementDType; row r comes from page
+   pageTable[r / pageSize], slot r % pageSize.  Rows of a page out of range are skipped and raise the error flag. */
+int cuda_dispatch_kv_page_gather_q4(CUDADeviceRef contextRef, int elementDType, CUDABufferRef codesRef, CUDABufferRef paramsRef,
+                                    CUDABufferRef pageTableRef, CUDABufferRef outputRef, uint32_t pageCount, uint32_t pageSize,
+                                    uint32_t kvHeads, uint32_t headDim, uint32_t outRows, uint64_t completionToken, CUDAStatus* status);
+
 /* ---- attention ---- */
 /* device/cuda/attention/multihead.h:10-27 (device.Attention.MultiHeadAttention, device/interface.go:98-103).
    Layout q/out [seqQ, numHeads*headDim], k/v [seqK, kvHeads*headDim]; causal mask is bottom-right
@@ -374,6 +398,29 @@ int cuda_dispatch_paged_decode_attention_noalloc(CUDADeviceRef contextRef, int e
                                                  CUDABufferRef outRef, CUDABufferRef errorFlagRef, uint32_t batch, uint32_t maxPagesPerSeq,
                                                  uint32_t pageCount, uint32_t pageSize, uint32_t numHeads, uint32_t kvHeads,
                                                  uint32_t headDim, uint64_t completionToken, CUDAStatus* status);
+
+/* NEW: paged decode attention over the cache in 4 bits, arguments as cuda_dispatch_paged_decode_attention with (codes, params) in the
+   place of the pages.  Any number of query heads per KV head, headDim 64 or 128, any page size.  ctxLens[i] == 0 leaves row i of out
+   untouched; a bad page id or an over-long or negative context is handled as there (never dereferenced, flag 1, the row is not valid). */
+int cuda_dispatch_paged_decode_attention_q4(CUDADeviceRef contextRef, int elementDType, CUDABufferRef queryRef, CUDABufferRef kCodesRef,
+                                            CUDABufferRef kParamsRef, CUDABufferRef vCodesRef, CUDABufferRef vParamsRef,
+                                            CUDABufferRef pageTableRef, CUDABufferRef ctxLensRef, CUDABufferRef outRef,
+                                            CUDABufferRef errorFlagRef, uint32_t batch, uint32_t maxPagesPerSeq, uint32_t pageCount,
+                                            uint32_t pageSize, uint32_t numHeads, uint32_t kvHeads, uint32_t headDim,
+                                            uint64_t completionToken, CUDAStatus* status);
+/* NEW: attention over whole prompts of different lengths, packed one behind the other: q/out [totalTokens, numHeads*headDim], k/v
+   [totalTokens, kvHeads*headDim]; sequence i holds rows seqStarts[i] .. seqStarts[i+1]-1 (device int32 [batch + 1], non-decreasing).
+   Per sequence as cuda_dispatch_rope_attention_prefill: positions startPosition .. restart with every sequence, causal or not,
+   ropeMode 2 = inputs already rotated.  float32, f16, bf16; headDim <= 256.  Rows of no sequence are left as they were.  A pair of starts
+   that is no range of the packed rows, or is longer than maxSeqLen, is skipped and raises the error flag (1); where the starts are
+   not non-decreasing the other rows of the call are not valid either.  out may not be one of the inputs. */
+int cuda_dispatch_rope_packed_attention_prefill(CUDADeviceRef contextRef, int elementDType, CUDABufferRef queryRef, CUDABufferRef keyRef,
+                                                CUDABufferRef valueRef, CUDABufferRef seqStartsRef, CUDABufferRef outRef, uint32_t batch,
+                                                uint32_t totalTokens, uint32_t maxSeqLen, uint32_t numHeads, uint32_t kvHeads,
+                                                uint32_t headDim, uint32_t causal, uint32_t ropeMode, double baseFreq,
+                                                int64_t startPosition, uint32_t scaling, double scalingFactor, double lowFreqFactor,
+                                                double highFreqFactor, uint32_t originalContext, uint64_t completionToken,
+                                                CUDAStatus* status);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop

@@ -77,6 +77,10 @@ SIGNATURES = {
     "cuda_dispatch_kv_page_gather": (cint, [vp, cint, vp, vp, vp, u32, u32, u32, u32, u64, u64, SP]),
     "cuda_dispatch_rope_kv_page_write": (cint, [vp, cint, cint, vp, vp, vp, vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, u32, u32, dbl, u32, u32,
                                                 dbl, dbl, dbl, u32, u64, SP]),
+    "cuda_dispatch_rope_kv_page_write_q4": (cint, [vp, cint] + [vp] * 9 + [u32] * 7 + [dbl, u32, dbl, dbl, dbl, u32, u64, SP]),
+    "cuda_dispatch_kv_page_gather_q4": (cint, [vp, cint, vp, vp, vp, vp, u32, u32, u32, u32, u32, u64, SP]),
+    "cuda_dispatch_paged_decode_attention_q4": (cint, [vp, cint] + [vp] * 9 + [u32] * 7 + [u64, SP]),
+    "cuda_dispatch_rope_packed_attention_prefill": (cint, [vp, cint] + [vp] * 5 + [u32] * 8 + [dbl, i64, u32, dbl, dbl, dbl, u32, u64, SP]),
     "cuda_dispatch_multi_head_attention": (cint, [vp, cint, cint, vp, vp, vp, vp, u32, u32, u32, u32, u32, u32, u32, u64, SP]),
     "cuda_dispatch_flash_attention": (cint, [vp, cint, vp, vp, vp, vp, u32, u32, u32, u32, u64, SP]),
     "cuda_dispatch_flash_attention_causal": (cint, [vp, cint, vp, vp, vp, vp, u32, u32, u32, u32, u32, u64, SP]),

@@ -26,9 +26,12 @@ SOURCES = [
     "softmax.cu",
     "rope.cu",
     "pages.cu",
+    "kv4.cu",
     "attention_exact.cu",
     "decode_attention.cu",
+    "decode_q4.cu",
     "prefill_attention.cu",
+    "packed_prefill.cu",
     "attention.cu",
 ]
 

@@ -24,6 +24,25 @@ struct Buffer {
     int device;
 };
 
+// One cached cos/sin table.  `pinned`: a captured launch reads it, so it is neither overwritten nor freed before the context closes.
+struct RopeTable {
+    float* data;
+    size_t bytes;
+    double key[10];
+    int valid, pinned;
+    unsigned long long used;
+    RopeTable* next;
+};
+
+// Scratch handed to the launches captured under one capture id; it lives until the context closes.
+struct GraphScratch {
+    unsigned long long id;
+    char* base;
+    size_t bytes;
+    int* counters;
+    GraphScratch* next;
+};
+
 struct Context {
     int device;
     int ccMajor;
@@ -44,11 +63,11 @@ struct Context {
     // arrival counters of the split-KV decode kernels: zeroed once here, every launch returns them to zero
     int* decodeCounters;
     size_t decodeCounterBytes;
-    // cos/sin table of the last RoPE configuration (positions x headDim/2, cos then sin), reused while the config repeats
-    float* ropeTable;
-    size_t ropeTableBytes;
-    double ropeKey[10];
-    int ropeKeyValid;
+    // cos/sin tables of the last RoPE configurations (positions x headDim/2, cos then sin), reused while a config repeats
+    struct RopeTable* ropeTables;
+    unsigned long long ropeClock;
+    // scratch of captured calls: one list entry per graph (see call_scratch)
+    struct GraphScratch* graphScratch;
     cudaEvent_t streamSwitchEvent;  // orders work of a newly adopted stream after what the previous stream still has queued
 };
 
@@ -60,6 +79,18 @@ void* dev_ptr(CUDABufferRef ref);
 int check_buffer(CUDAStatus* status, CUDABufferRef ref, const char* name, size_t needBytes);
 int check_launch(Context* ctx, CUDAStatus* status, const char* what);
 void* ensure_workspace(Context* ctx, size_t bytes, CUDAStatus* status);
+// capture state of the context's stream; *id (may be null) names the capture
+bool stream_capturing(Context* ctx, unsigned long long* id);
+
+// Scratch of one call.  Eager calls share the context's grow-only workspace and its arrival counters: the context's launches are
+// stream-ordered, also across a change of stream.  A captured call gets scratch that belongs to its graph alone, so that a workspace
+// that grows later cannot pull it away from under a replay and two graphs can be replayed at the same time.
+struct Scratch {
+    char* base;         // 256-byte aligned
+    int* counters;      // counterBytes of arrival counters, zero on entry and again after every launch
+    bool clearCounters; // not known to be zero: clear them on the stream first
+};
+int call_scratch(Context* ctx, size_t bytes, size_t counterBytes, Scratch* out, CUDAStatus* status);
 
 inline size_t dtype_size(int dt) {
     switch (dt) {

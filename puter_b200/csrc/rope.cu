@@ -434,35 +434,64 @@ int build_rope_table(Context* ctx, float* table, size_t seqLen, int headDim, dou
     return check_launch(ctx, status, "rope table");
 }
 
-// Returns the cos/sin table for this configuration from the context's cache, rebuilding it only when the configuration
-// (or the number of positions) changed.  A decoder applies the same RoPE to q and k of every layer, so the float64
-// angle evaluation runs once per configuration instead of once per call.
+// Returns the cos/sin table for this configuration from the context's cache, building it only for a configuration (or a
+// number of positions) that is not among the last few.  A decoder applies the same RoPE to q and k of every layer, so the
+// float64 angle evaluation runs once per configuration instead of once per call; several tables are kept because a layer may
+// alternate between two (prefill over its own length, cache writes over the whole range of positions).
+// A captured launch keeps the pointer: its table is pinned, and a table that is missing during a capture is refused, since
+// building it there would only record the work.
+static constexpr int kRopeTables = 4;  // unpinned tables kept
+
 const float* cached_rope_table(Context* ctx, size_t seqLen, int headDim, double base, long long startPos, int scaling, double factor,
                                double low, double high, int origCtx, CUDAStatus* status) {
     const double key[10] = {(double)seqLen, (double)headDim, base, (double)startPos, (double)scaling, scaling ? factor : 0.0,
                             scaling ? low : 0.0, scaling ? high : 0.0, scaling ? (double)origCtx : 0.0, 0.0};
     const size_t need = seqLen * (size_t)(headDim / 2) * 2 * sizeof(float);
-    if (ctx->ropeKeyValid && memcmp(key, ctx->ropeKey, sizeof(key)) == 0 && ctx->ropeTable && ctx->ropeTableBytes >= need)
-        return ctx->ropeTable;
-    ctx->ropeKeyValid = 0;
-    if (ctx->ropeTableBytes < need) {
-        if (ctx->ropeTable) {
-            cudaStreamSynchronize(ctx->stream);  // earlier launches may still read the old table
-            cudaFree(ctx->ropeTable);
-            ctx->ropeTable = nullptr;
-            ctx->ropeTableBytes = 0;
+    const bool capturing = stream_capturing(ctx, nullptr);
+    RopeTable* oldest = nullptr;
+    int unpinned = 0;
+    for (RopeTable* t = ctx->ropeTables; t; t = t->next) {
+        if (t->valid && memcmp(key, t->key, sizeof(key)) == 0) {
+            t->used = ++ctx->ropeClock;
+            if (capturing) t->pinned = 1;
+            return t->data;
         }
-        if (cudaMalloc((void**)&ctx->ropeTable, need) != cudaSuccess) {
+        if (!t->pinned) {
+            unpinned++;
+            if (!oldest || t->used < oldest->used) oldest = t;
+        }
+    }
+    if (capturing) {
+        fail(status, -2, "rope: no cos / sin table for this configuration yet: make one call with it before the capture");
+        return nullptr;
+    }
+    RopeTable* t = unpinned >= kRopeTables ? oldest : nullptr;
+    if (!t) {
+        t = new RopeTable();
+        t->next = ctx->ropeTables;
+        ctx->ropeTables = t;
+    }
+    t->valid = 0;
+    if (t->bytes < need) {
+        if (t->data) {
+            cudaStreamSynchronize(ctx->stream);  // earlier launches may still read the old table
+            cudaFree(t->data);
+            t->data = nullptr;
+            t->bytes = 0;
+        }
+        if (cudaMalloc((void**)&t->data, need) != cudaSuccess) {
             cudaGetLastError();
+            t->data = nullptr;
             fail(status, -7, "rope: table allocation of %zu bytes failed", need);
             return nullptr;
         }
-        ctx->ropeTableBytes = need;
+        t->bytes = need;
     }
-    if (build_rope_table(ctx, ctx->ropeTable, seqLen, headDim, base, startPos, scaling, factor, low, high, origCtx, status) != 0) return nullptr;
-    memcpy(ctx->ropeKey, key, sizeof(key));
-    ctx->ropeKeyValid = 1;
-    return ctx->ropeTable;
+    if (build_rope_table(ctx, t->data, seqLen, headDim, base, startPos, scaling, factor, low, high, origCtx, status) != 0) return nullptr;
+    memcpy(t->key, key, sizeof(key));
+    t->valid = 1;
+    t->used = ++ctx->ropeClock;
+    return t->data;
 }
 
 }  // namespace puter

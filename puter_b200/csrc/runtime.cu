@@ -71,6 +71,56 @@ void* ensure_workspace(Context* ctx, size_t bytes, CUDAStatus* status) {
     return ctx->workspace;
 }
 
+bool stream_capturing(Context* ctx, unsigned long long* id) {
+    cudaStreamCaptureStatus state = cudaStreamCaptureStatusNone;
+    unsigned long long name = 0;
+    if (cudaStreamGetCaptureInfo(ctx->stream, &state, &name) != cudaSuccess) {
+        cudaGetLastError();  // the legacy stream while another stream is being captured: this call is not part of that capture
+        return false;
+    }
+    if (id) *id = name;
+    return state == cudaStreamCaptureStatusActive;
+}
+
+int call_scratch(Context* ctx, size_t bytes, size_t counterBytes, Scratch* out, CUDAStatus* status) {
+    const bool own = counterBytes <= ctx->decodeCounterBytes;  // the kept, always-zero counters hold this call's
+    const size_t body = (bytes + 255) & ~(size_t)255;
+    const size_t need = body + (own ? 0 : counterBytes) + 512;
+    unsigned long long id = 0;
+    if (!stream_capturing(ctx, &id)) {
+        char* ws = (char*)ensure_workspace(ctx, need, status);
+        if (!ws) return status ? status->code : -7;
+        out->base = ws;
+        out->counters = own ? ctx->decodeCounters : (int*)(ws + body);
+        out->clearCounters = !own;
+        return 0;
+    }
+    GraphScratch* g = ctx->graphScratch;
+    while (g && (g->id != id || g->bytes < need)) g = g->next;
+    if (!g) {
+        // allocating is not part of the captured work: done in relaxed mode, cleared on a stream of the context's own
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        void* p = nullptr;
+        const size_t total = ctx->decodeCounterBytes + need;
+        cudaError_t err = cudaMalloc(&p, total);
+        if (err == cudaSuccess) err = cudaMemsetAsync(p, 0, ctx->decodeCounterBytes, ctx->uploadStream);
+        if (err == cudaSuccess) err = cudaStreamSynchronize(ctx->uploadStream);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (err != cudaSuccess) {
+            cudaGetLastError();
+            if (p) cudaFree(p);
+            return fail(status, -7, "cuda: scratch of %zu bytes for a captured call failed: %s", total, cudaGetErrorString(err));
+        }
+        g = new GraphScratch{id, (char*)p + ctx->decodeCounterBytes, need, (int*)p, ctx->graphScratch};
+        ctx->graphScratch = g;
+    }
+    out->base = g->base;
+    out->counters = own ? g->counters : (int*)(g->base + body);
+    out->clearCounters = !own;
+    return 0;
+}
+
 static std::mutex g_mu;
 static Context* g_default = nullptr;
 
@@ -152,7 +202,18 @@ void cuda_close_device(CUDADeviceRef device) {
         if (ctx->pinned[i]) cudaFreeHost(ctx->pinned[i]);
     if (ctx->errorFlag) cudaFree(ctx->errorFlag);
     if (ctx->decodeCounters) cudaFree(ctx->decodeCounters);
-    if (ctx->ropeTable) cudaFree(ctx->ropeTable);
+    for (RopeTable* t = ctx->ropeTables; t;) {
+        RopeTable* next = t->next;
+        cudaFree(t->data);
+        delete t;
+        t = next;
+    }
+    for (GraphScratch* g = ctx->graphScratch; g;) {
+        GraphScratch* next = g->next;
+        cudaFree(g->counters);
+        delete g;
+        g = next;
+    }
     for (int i = 0; i < 4; i++)
         if (ctx->stageEvents[i]) cudaEventDestroy(ctx->stageEvents[i]);
     if (ctx->streamSwitchEvent) cudaEventDestroy(ctx->streamSwitchEvent);
@@ -296,9 +357,13 @@ int cuda_context_set_stream(CUDADeviceRef device, void* cudaStream, CUDAStatus* 
         // the context's scratch (workspace, RoPE table, decode counters) may still be read by kernels queued on the old stream:
         // whatever the new stream launches is ordered after them
         cudaSetDevice(ctx->device);
-        if (cudaEventRecord(ctx->streamSwitchEvent, ctx->stream) == cudaSuccess) cudaStreamWaitEvent(next, ctx->streamSwitchEvent, 0);
-        cudaGetLastError();
+        // (a stream under capture runs nothing now, and an event may not tie it to work outside its capture)
+        const bool from = stream_capturing(ctx, nullptr);
+        cudaStream_t last = ctx->stream;
         ctx->stream = next;
+        if (!from && !stream_capturing(ctx, nullptr) && cudaEventRecord(ctx->streamSwitchEvent, last) == cudaSuccess)
+            cudaStreamWaitEvent(next, ctx->streamSwitchEvent, 0);
+        cudaGetLastError();
     }
     return ok(status);
 }

@@ -407,6 +407,24 @@ class Device:
                               pageSize, maxPositions, float(rope.BaseFreq), int(rope.Mode), int(rope.Scaling), float(rope.ScalingFactor),
                               float(rope.LowFreqFactor), float(rope.HighFreqFactor), int(rope.OriginalContext), 0))
 
+    # ---- Shape: paged KV in 4 bits ----------------------------------------------------------------------
+    def RoPEKVPageWriteQ4(self, rope: RoPEConfig | None, k, v, positions, pageIDs, offsets, kCodes, kParams, vCodes, vParams, rows, kvHeads,
+                          headDim, pageCount, pageSize, maxPositions, format):
+        """KV-cache producer for the cache in 4 bits, one launch: RoPE(k) at positions[row] (float32, not rounded in between), then every
+        vector of K and of V quantised to 16 levels between its extremes and written in place.  rope=None: k is already rotated
+        (positions may be None).  Codes are [pageCount, kvHeads, pageSize, headDim / 2] bytes, params [pageCount, kvHeads, pageSize, 2]
+        of `format` = (step, least); an element is least + step * code."""
+        rc = rope or RoPEConfig()
+        mode = 2 if rope is None else int(rc.Mode)
+        self._call("cuda_dispatch_rope_kv_page_write_q4", [k, v, positions, pageIDs, offsets, kCodes, kParams, vCodes, vParams],
+                   lambda r: (format, *r, rows, kvHeads, headDim, pageCount, pageSize, maxPositions, mode, float(rc.BaseFreq), int(rc.Scaling),
+                              float(rc.ScalingFactor), float(rc.LowFreqFactor), float(rc.HighFreqFactor), int(rc.OriginalContext), 0))
+
+    def KVPageGatherQ4(self, codes, params, pageTable, output, pageCount, pageSize, kvHeads, headDim, outRows, format):
+        """KVPageGather from the cache in 4 bits: output [outRows, kvHeads * headDim] of `format`, rounded once."""
+        self._call("cuda_dispatch_kv_page_gather_q4", [codes, params, pageTable, output],
+                   lambda r: (format, *r, pageCount, pageSize, kvHeads, headDim, outRows, 0))
+
     # ---- Attention ------------------------------------------------------------------------------------
     def MultiHeadAttention(self, config: MultiHeadAttentionConfig, query, key, value, output, seqQ, seqK, format):
         if config.ALiBiSlope != 0:
@@ -432,6 +450,31 @@ class Device:
                    lambda r: (format, r[0], r[1], r[2], r[3], batch, seqLen, attn.NumHeads, kv, attn.HeadDim, int(attn.Causal), mode,
                               float(rc.BaseFreq), int(rc.StartPosition), int(rc.Scaling), float(rc.ScalingFactor),
                               float(rc.LowFreqFactor), float(rc.HighFreqFactor), int(rc.OriginalContext), 0))
+
+    def RoPEPackedAttentionPrefill(self, rope: RoPEConfig | None, attn: MultiHeadAttentionConfig, query, key, value, seqStarts, output, batch,
+                                   totalTokens, maxSeqLen, format):
+        """Prompts of different lengths in one call: rows seqStarts[i] .. seqStarts[i + 1] - 1 (int32 on the device, batch + 1 entries) are
+        sequence i; per sequence RoPE(q), RoPE(k) at positions that restart with it, then MultiHeadAttention.  No sequence is longer
+        than maxSeqLen.  rope=None: inputs already rotated.  Rows of no sequence are left as they were."""
+        if attn.ALiBiSlope != 0 or attn.WindowSize != 0:
+            raise DeviceError(-6, "packed prefill attention: no ALiBi and no sliding window")
+        kv = attn.KVHeadCount if attn.KVHeadCount > 0 else attn.NumHeads
+        rc = rope or RoPEConfig()
+        mode = 2 if rope is None else int(rc.Mode)
+        self._call("cuda_dispatch_rope_packed_attention_prefill", [query, key, value, seqStarts, output],
+                   lambda r: (format, *r, batch, totalTokens, maxSeqLen, attn.NumHeads, kv, attn.HeadDim, int(attn.Causal), mode,
+                              float(rc.BaseFreq), int(rc.StartPosition), int(rc.Scaling), float(rc.ScalingFactor),
+                              float(rc.LowFreqFactor), float(rc.HighFreqFactor), int(rc.OriginalContext), 0))
+
+    def PagedDecodeAttentionQ4(self, attn: MultiHeadAttentionConfig, query, kCodes, kParams, vCodes, vParams, pageTable, ctxLens, output,
+                               batch, maxPagesPerSeq, pageCount, pageSize, format, errorFlag=None):
+        """PagedDecodeAttention over the cache in 4 bits that RoPEKVPageWriteQ4 fills."""
+        if attn.ALiBiSlope != 0 or attn.WindowSize != 0:
+            raise DeviceError(-6, "paged decode attention (4 bits): no ALiBi and no sliding window")
+        kv = attn.KVHeadCount if attn.KVHeadCount > 0 else attn.NumHeads
+        self._call("cuda_dispatch_paged_decode_attention_q4",
+                   [query, kCodes, kParams, vCodes, vParams, pageTable, ctxLens, output, errorFlag],
+                   lambda r: (format, *r, batch, maxPagesPerSeq, pageCount, pageSize, attn.NumHeads, kv, attn.HeadDim, 0))
 
     def PagedDecodeAttention(self, attn: MultiHeadAttentionConfig, query, kPages, vPages, pageTable, ctxLens, output, batch,
                              maxPagesPerSeq, pageCount, pageSize, format, kvFormat=None, kScale=None, vScale=None, errorFlag=None):
