@@ -308,7 +308,13 @@ def test_decode_flags(d):
             ctx[0] = 10 ** 6 if change == "long" else -5
         got = decode(d, (q, kc, kp, vc, vp, table, ctx), kv, dim, page, group, 2)
         assert d.take_error() == 1
-        assert torch.equal(got[1], want[1])
+        if "page" in change:
+            assert torch.equal(got[1], want[1])
+        else:  # another length of sequence 0 divides the work at other tokens of sequence 1: other sums, the same tolerance
+            ctx[0] = 0
+            got[0] = 7
+            check_decode(got, (q, kc, kp, vc, vp, table, ctx), kv, dim, page, group, 2)
+            ctx[0] = 10 ** 6 if change == "long" else -5
         decode(d, (q, kc, kp, vc, vp, table, ctx), kv, dim, page, group, 2, flag=flag)
         assert int(flag) == 1 and d.take_error() == 0
         flag.zero_()
