@@ -9,23 +9,36 @@
 // limits the kernel is therefore the number of instructions per element, and its layout follows from that:
 //   * The tokens are the rows of mma.sync m16n8k16 and the query heads of a KV head's group its columns (S^T = K Q^T, O^T = V^T P^T), as
 //     in the 16-bit kernel; a matrix unit at a few tens of per cent of its rate and no reduction over lanes per score.
-//   * A code becomes an f16 operand with ONE instruction per two elements and no arithmetic: the four bits, masked in place, ARE
-//     the subnormal f16 n * 2^-24 (bits 0-3) or 16 n * 2^-24 (bits 4-7), exact.  The factors are powers of two and are put back
-//     into the scores and the output.  Bits 4-7 go to products and accumulators of their own.
+//   * A code becomes an f16 operand with one logic instruction per two elements and no arithmetic: bits masked in place ARE a subnormal
+//     f16, exact: the low four bits of a byte are n_even * 2^-24, the high four 16 n_odd * 2^-24, the whole byte their sum F (the high
+//     byte of a half comes down with a byte permute that clears the rest).  The factors are powers of two and are put back into
+//     the query fragments and the output.  Logic instructions run at half rate and are what binds (160 of a step's ~230), so V takes F
+//     where it does not need the mask: the odd dimension is (F - even) / 16, taken from the accumulators at the end.  (K cannot: the
+//     query fragment of the even element would be q_even - q_odd / 16, which f16 rounds; measured beyond the tolerance of f16 queries
+//     with peaked scores.)
 //   * K: a lane's 16-byte (D = 128) piece of a token holds its A fragments for all of the contraction, since the order of the contraction
 //     is free: the query fragments are loaded in the order in which the masks deliver the elements.  V: two byte permutes pair the
 //     words of two tokens, then the same masks.
-//   * Queries enter as f16, scaled by a power of two per (sequence, head) so that a bf16 query of any size fits; the weights
-//     p_t * step_t enter as f16 (half a step of 2^-11, an eighth of what the 16-bit output keeps), relative to a running power of two above
-//     the largest step, which joins the running maximum of the softmax in rescaling the accumulator.
+//   * Up to four query heads per KV head (QUAD): the scores are integer products.  As bytes the codes need no conversion at all: F is the word
+//     as it lies in memory and L one mask per word (16 logic instructions per step and lane where the f16 form needs 80), and
+//     the four unused columns take the lower bytes of the queries' integers, so that a lane has whole scores of one head.  The integers
+//     hold a query to 2^-16 of its largest element.  More heads take the f16 form: queries as f16, scaled by a power of two per
+//     (sequence, head) so that a bf16 query of any size fits.
+//   * The weights p_t * step_t enter as f16 (half a step of 2^-11, an eighth of what the 16-bit output keeps), relative to a running power of
+//     two about the largest step, which joins the running maximum of the softmax in rescaling the accumulator.
 // Sums, maxima and accumulators are float32.
 //
 // Work: the tiles of 16 tokens of all (KV head, sequence) pairs in one list, cut into equal contiguous ranges, one per CTA, and each
-// CTA's range into equal ranges, one per warp.  A warp owns its pipeline (cp.async into its own stages, copies running ahead across
-// sequence boundaries; page entries one step further ahead), so there is no block-wide barrier before the end.  A pair that lies inside a
-// warp's range is written by the warp.  Otherwise the warps of a CTA put their partial (maximum, sum, accumulator) together, and
-// the CTA that arrives last at a pair joins those of all CTAs, in their order: the same bits whoever is last.
+// CTA's range into equal ranges, one per warp.  A warp owns its pipeline (stages of 32 tokens, copies running ahead across sequence
+// boundaries, page entries one step further ahead), so there is no block-wide barrier before the end.  Where pages hold whole tiles the
+// copies are bulk copies, four per tile (codes and params of K and V), each issued by a lane of its own: ~20 instructions per step where
+// 16-byte copies with a page lookup per token take ~90.  A pair that lies inside a warp's range is written by the warp.  Otherwise the warps
+// of a CTA put their partials (maximum, sum, accumulator) together, and the CTAs that share a pair join theirs together: each waits, bounded,
+// for the pair's counter and takes its share of the output's 32-dimension slices (a cooperative launch makes all CTAs resident; where it
+// is refused the CTA that arrives last joins everything).  Fixed order either way: the same bits from call to call.  One CTA joining 38
+// others' parts of 16 heads took 18 us, all of them together 3.
 #include <math.h>
+#include <stdlib.h>
 
 #include "common.cuh"
 
@@ -34,8 +47,8 @@ namespace puter {
 namespace q4d {
 
 constexpr int kTile = 16;             // tokens per tile
-constexpr int kStep = 32;             // tokens per step of a warp
-constexpr int kPrefixSmem = 2048;     // sequences whose tile prefix sums fit shared memory
+constexpr int kPrefixSmem = 1024;     // sequences whose tile prefix sums fit shared memory
+constexpr int kStageBytes = 209 * 1024;  // of shared memory for the copies in flight: three steps of 16 warps or of 8 with twice the tokens
 constexpr int kWarpTiles = 2;         // tiles that a warp gets at least before another CTA takes part
 
 struct Params {
@@ -46,9 +59,10 @@ struct Params {
     uint16_t* out;
     int* errorFlag;
     const int* tileStart;  // [batch + 1] exclusive prefix of tiles, or nullptr: scanned in shared memory
-    float* acc;            // partial accumulators [slots, heads of a block, D]: two slots per warp, then two per CTA
+    float* acc;            // partial accumulators [slots, heads of a block, D]: one slot per warp, then two per CTA
     float2* ml;            // (maximum in the log2 domain, sum) [slots, heads of a block]
-    int* counters;         // arrivals per (unit, sequence): zero on entry and on exit
+    int* counters;         // arrivals (and departures) per (unit, sequence): zero on entry and on exit
+    int together;          // all CTAs run at the same time (cooperative launch): the owners of a pair join it together
     int batch, maxPages, pageCount, pageSize, pageShift, numHeads, kvHeads, group;
     int blocks, units;     // head blocks per KV head, KV heads * blocks
     float scaleLog2;
@@ -60,6 +74,21 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, uint32_t b
 }
 __device__ __forceinline__ void copy4(uint32_t dst, const void* src, uint32_t bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// one bulk copy, counted by the mbarrier `bar`; addresses and size are multiples of 16 bytes
+__device__ __forceinline__ void bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar, uint64_t pol) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(bar), "l"(pol) : "memory");
+}
+// false when the copies that `bar` counts have not landed after about a second
+__device__ __forceinline__ bool landed(uint32_t bar, uint32_t parity) {
+    for (int i = 0; i < (1 << 22); i++) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+                     : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+        if (done) return true;
+    }
+    return false;
 }
 __device__ __forceinline__ void lds128(uint32_t a, uint32_t* r) {
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
@@ -73,9 +102,32 @@ __device__ __forceinline__ uint32_t lds32(uint32_t a) {
     return r;
 }
 __device__ __forceinline__ void mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the same onto zero
+__device__ __forceinline__ void mma0(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// codes as bytes (0 .. 255) times signed query bytes, exact sums
+__device__ __forceinline__ void imma(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void imma0(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+}
+// lowest signed byte of v; v is left with the rest: v = rest * 256 + byte
+__device__ __forceinline__ uint32_t limb(int& v) {
+    const int b = (int)(int8_t)v;
+    v = (v - b) >> 8;
+    return (uint32_t)b & 255u;
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
     uint32_t d;
@@ -100,16 +152,14 @@ __device__ __forceinline__ int seq_ctx(const Params& p, int b) {
     return (int)ctx;
 }
 
-// exclusive prefix sum of tiles per sequence: out[0 .. batch].  Every thread of the block calls it.
-__device__ void block_prefix(const Params& p, int* out) {
+// exclusive prefix sum of tiles per sequence: out[0 .. batch]; lens (may be null): the cut contexts.  Every thread of the block calls it.
+__device__ void block_prefix(const Params& p, int* out, int* lens) {
     __shared__ int sums[32];
-    __shared__ int carry;
-    if (threadIdx.x == 0) carry = 0;
-    __syncthreads();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int carry = 0;
     for (int base = 0; base < p.batch; base += blockDim.x) {
-        const int b = base + threadIdx.x;
-        const int tiles = b < p.batch ? (int)(((long long)seq_ctx(p, b) + kTile - 1) / kTile) : 0;
+        const int b = base + threadIdx.x, ctx = b < p.batch ? seq_ctx(p, b) : 0;
+        const int tiles = (int)(((long long)ctx + kTile - 1) / kTile);
         int incl = tiles;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -118,93 +168,79 @@ __device__ void block_prefix(const Params& p, int* out) {
         }
         if (lane == 31) sums[warp] = incl;
         __syncthreads();
+        const int used = (min(p.batch - base, (int)blockDim.x) + 31) / 32;
         int before = carry;
-        for (int w = 0; w < warp; w++) before += sums[w];
-        if (b < p.batch) out[b] = before + incl - tiles;
-        __syncthreads();
-        if (threadIdx.x == blockDim.x - 1) carry = before + incl;
-        __syncthreads();
+        for (int w = 0; w < used; w++) {
+            if (w < warp) before += sums[w];
+            carry += sums[w];
+        }
+        if (b < p.batch) {
+            out[b] = before + incl - tiles;
+            if (lens) lens[b] = ctx;
+        }
+        if (base + (int)blockDim.x < p.batch) __syncthreads();  // the sums have been read
     }
     if (threadIdx.x == 0) out[p.batch] = carry;
     __syncthreads();
 }
-__global__ void __launch_bounds__(1024) prefix_kernel(Params p, int* out) { block_prefix(p, out); }
+__global__ void __launch_bounds__(1024) prefix_kernel(Params p, int* out) { block_prefix(p, out, nullptr); }
 
-// the part that holds tile g when `total` tiles are cut into `parts` ranges [i * total / parts, (i + 1) * total / parts)
-__device__ __forceinline__ int part_of(long long g, long long total, long long parts) { return (int)(((g + 1) * parts - 1) / total); }
-
-// NT: blocks of eight query heads that a warp serves with one pass over the codes
-template <int DT, int D, int NT>
-struct Shape {
-    static constexpr int WARPS = NT == 1 ? 16 : 8;  // 8: the accumulators of 16 heads need more than 128 registers a thread
-    static constexpr int ROW = D / 2;               // bytes of a token's codes
-    static constexpr int STAGE = 2 * kStep * ROW + 2 * kStep * 4;
-    static constexpr int STAGES = (NT == 1 ? 3 : 6) * (D == 128 ? 1 : 2);
-    static constexpr int SMEM = WARPS * STAGES * STAGE;
-    static constexpr int HEADS = 8 * NT;
+// a / b for b > 0; 64-bit divisions take a hundred instructions and are hardly ever needed
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    return ((unsigned long long)(a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
+// `total` tiles cut into `parts` ranges: the first `more` of them have one tile more than `each`
+struct Split {
+    long long each, more;
+    __device__ __forceinline__ Split(long long total, int parts) : each(quotient(total, parts)), more(total - each * parts) {}
+    __device__ __forceinline__ long long begin(int i) const { return i * each + (i < more ? i : more); }
+    __device__ __forceinline__ int holding(long long g) const {
+        const long long edge = more * (each + 1);
+        return (int)(g < edge ? quotient(g, each + 1) : more + quotient(g - edge, each));
+    }
 };
 
-// Columns (head, four dimensions) of a block of heads, dealt to the threads of the CTA: joins the partials that `slot_of` names for
-// i in [0, n), in order, and hands on (maximum, sum, four sums).  The loads of eight partials are issued together.
-template <int D, typename SlotOf, typename Put>
-__device__ __forceinline__ void join(const Params& p, int heads, int stride, int n, SlotOf slot_of, Put put) {
-    for (int col = threadIdx.x; col < heads * (D / 4); col += blockDim.x) {
-        const int h = col / (D / 4), d = (col % (D / 4)) * 4;
-        float M = -INFINITY, den = 0.f;
-        float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i0 = 0; i0 < n; i0 += 8) {
-            float2 ml[8];
-            float4 a[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const long long slot = i0 + i < n ? slot_of(i0 + i) : -1;
-                if (slot >= 0) {
-                    ml[i] = __ldcg(p.ml + slot * stride + h);
-                    a[i] = __ldcg((const float4*)(p.acc + (slot * stride + h) * D + d));
-                } else {
-                    ml[i] = make_float2(-INFINITY, 0.f);
-                    a[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                }
-            }
-            float Mn = M;
-#pragma unroll
-            for (int i = 0; i < 8; i++) Mn = fmaxf(Mn, ml[i].x);
-            const float old = M == -INFINITY ? 0.f : exp2f(M - Mn);
-            den *= old;
-            num.x *= old; num.y *= old; num.z *= old; num.w *= old;
-            M = Mn;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                // (a part without a finite score has sum 0, or NaN, which stays NaN)
-                const float w = ml[i].x == -INFINITY ? (ml[i].y == 0.f ? 0.f : ml[i].y) : exp2f(ml[i].x - M);
-                den += ml[i].y * w;
-                num.x += a[i].x * w; num.y += a[i].y * w; num.z += a[i].z * w; num.w += a[i].w * w;
-            }
-        }
-        put(h, d, M, den, num);
-    }
-}
+// NT: blocks of eight query heads that a warp serves with one pass over the codes, 0: a block of four with integer scores (QUAD);
+// MT: tiles per step
+template <int D_, int NT_, int WARPS_, int MT_>
+struct Shape {
+    static constexpr int D = D_, NT = NT_ ? NT_ : 1, WARPS = WARPS_, MT = MT_;
+    static constexpr bool QUAD = NT_ == 0;
+    static constexpr int STEP = 16 * MT;            // tokens per step of a warp
+    static constexpr int ROW = D / 2;               // bytes of a token's codes
+    static constexpr int STAGE = 2 * STEP * ROW + 2 * STEP * 4;
+    static constexpr int STAGES = kStageBytes / (WARPS * STAGE);
+    static constexpr int SMEM = WARPS * STAGES * STAGE;
+    static constexpr int HEADS = QUAD ? 4 : 8 * NT;
+};
 
-template <int DT>
-__device__ __forceinline__ void store4(uint16_t* dst, float den, float4 num) {
-    *(uint2*)dst = make_uint2(pack16_arith<DT>(num.x / den, num.y / den), pack16_arith<DT>(num.z / den, num.w / den));
-}
+// weight of a part under the maximum M of all (a part without a finite score has sum 0, or NaN, which stays NaN)
+__device__ __forceinline__ float weight(float2 ml, float M) { return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : exp2f(ml.x - M); }
 
-template <int DT, int D, int NT>
-__global__ void __launch_bounds__(Shape<DT, D, NT>::WARPS * 32, 1) decode_kernel(Params p) {
-    using S = Shape<DT, D, NT>;
+// PAGED: pages hold whole tiles (page size a multiple of 16): bulk copies.  Otherwise 16-byte copies with a page lookup per token.
+template <int DT, typename S, bool PAGED>
+__global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
+    constexpr int D = S::D, NT = S::NT, MT = S::MT, kStep = S::STEP;
     constexpr int WK = D / 32;   // words of a token's K codes in a lane
     constexpr int WV = D / 64;   // words of a token's V codes in a lane
     constexpr int ROW = S::ROW;
+    constexpr bool QUAD = S::QUAD;
+    constexpr int J = QUAD ? 1 : 2;  // heads of a lane: t, or 8nt + 2t and 8nt + 2t + 1
+    constexpr int kPart = S::HEADS * D * 4 + S::HEADS * 8;  // a partial in shared memory: accumulators, then (maximum, sum)
+    static_assert(kPart <= S::STAGES * S::STAGE, "a warp's partial takes the place of its stages");
     extern __shared__ __align__(128) unsigned char smemRaw[];
-    __shared__ int sStart[kPrefixSmem + 1];
-    __shared__ int sSeg[2 * S::WARPS];
-    __shared__ int sLast[2];
+    __shared__ int sStart[kPrefixSmem + 1], sCtx[kPrefixSmem];
+    __shared__ int sSeg[32];       // entry 2w + i: the pair of warp w's partial i (0: it began before the warp's range, 1: it goes on behind it)
+    __shared__ int sNear[S::WARPS];  // which of the two lies in shared memory
+    __shared__ int sB[32], sUnit[32], sWhere[32];  // of an entry: sequence, unit; pair inside the CTA's range (2) or begun before it (0) or going on behind it (1)
+    __shared__ int sShared[2], sFirst[2], sOwners[2], sGo[2];  // pairs shared with other CTAs: entry, first owner, owners, whether to join
+    __shared__ __align__(8) uint64_t sBar[S::WARPS * S::STAGES];
     const int* ts = p.tileStart;
     if (!ts) {
-        block_prefix(p, sStart);
+        block_prefix(p, sStart, sCtx);
         ts = sStart;
     }
+    auto ctx_of = [&](int b) { return p.tileStart ? seq_ctx(p, b) : sCtx[b]; };
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const long long T = ts[p.batch], total = T * p.units;
     if (total == 0) return;
@@ -212,19 +248,28 @@ __global__ void __launch_bounds__(Shape<DT, D, NT>::WARPS * 32, 1) decode_kernel
     const long long most = (total + S::WARPS * kWarpTiles - 1) / (S::WARPS * kWarpTiles);
     const int parts = most < (long long)gridDim.x ? (int)most : (int)gridDim.x;
     if ((int)blockIdx.x >= parts) return;
-    const long long clo = blockIdx.x * total / parts, chi = (blockIdx.x + 1) * total / parts;
+    const Split split(total, parts);
+    const long long clo = split.begin(blockIdx.x), chi = split.begin(blockIdx.x + 1);
     const long long lo = clo + warp * (chi - clo) / S::WARPS, hi = clo + (warp + 1) * (chi - clo) / S::WARPS;
-    if (lane < 2) sSeg[2 * warp + lane] = -1;
-    __syncwarp();
+    if (threadIdx.x < 32) sSeg[threadIdx.x] = -1;
+    if (threadIdx.x < S::WARPS) sNear[threadIdx.x] = -1;
+    if (threadIdx.x < 2) sShared[threadIdx.x] = -1;
+    const uint32_t bars = smem_u32(sBar) + warp * S::STAGES * 8;
+    if (PAGED && lane == 0) {
+        for (int i = 0; i < S::STAGES; i++) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bars + 8 * i) : "memory");
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
 
-    const uint32_t base = smem_u32(smemRaw) + warp * (S::STAGES * S::STAGE);
+    unsigned char* const mine = smemRaw + warp * (S::STAGES * S::STAGE);
+    const uint32_t base = smem_u32(mine);
     uint64_t pol;
     asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(pol));
 
     if (lo < hi) {
         // ---- the copies' own place in the range, ahead of the computation's ----
         long long iNext = lo;     // first tile behind the segment that is being copied
-        int iUnit = (int)(lo / T), ib = 0, iTok = 0, iEnd = 0, iStage = 0;
+        int iUnit = (int)quotient(lo, T), ib = 0, iTok = 0, iEnd = 0, iStage = 0;
         {
             const int r = (int)(lo - iUnit * T);
             int a = 0, z = p.batch;
@@ -236,71 +281,105 @@ __global__ void __launch_bounds__(Shape<DT, D, NT>::WARPS * 32, 1) decode_kernel
             ib = a;
         }
         int cUnit = iUnit, cb = ib;
-        int entryPage = 0;        // page of this lane's token of the step to be copied next
-        uint32_t inPage = 0;      // and its place in that page
+        constexpr int PL = PAGED ? 1 : MT / 2;  // look-ups of a lane
+        int entryPage[PL] = {};       // page of this lane's tile (not PAGED: tokens lane + 32 i) of the step to be copied next
+        uint32_t inPage[PL] = {};     // and its place in that page, plus the KV head's place in a page
+        uint32_t headOff = (uint32_t)(iUnit / p.blocks) * (uint32_t)p.pageSize;
+        const uint32_t pageSlots = (uint32_t)p.kvHeads * (uint32_t)p.pageSize;
+        const int32_t* iTable = p.table;
+        // PAGED: lanes 0 .. 4 MT - 1 issue one copy each: tile lane / 4 of the step, pool lane % 4
+        const int part = lane & 3, tileOf = (lane >> 2) % MT;
+        const unsigned char* const pool = part == 0 ? p.kCodes : part == 1 ? p.vCodes : (const unsigned char*)(part == 2 ? p.kParams : p.vParams);
+        const uint32_t perSlot = part < 2 ? ROW : 4;
+        const uint32_t dstOff = (part < 2 ? part * kStep * ROW : 2 * kStep * ROW + (part - 2) * kStep * 4) + tileOf * kTile * perSlot;
         // Moves to the next step and starts fetching its page entries.
         auto look_ahead = [&]() {
             if (iTok >= iEnd) {
                 if (iNext >= hi) return;
                 long long r = iNext - (long long)iUnit * T;
-                if (r >= T) { iUnit++; ib = 0; r -= T; }
+                if (r >= T) {
+                    iUnit++;
+                    ib = 0;
+                    r -= T;
+                    headOff = (uint32_t)(iUnit / p.blocks) * (uint32_t)p.pageSize;
+                }
                 while (ts[ib + 1] <= r) ib++;
                 const long long s0 = ts[ib], s1 = ts[ib + 1], stop = hi - (long long)iUnit * T, e = s1 < stop ? s1 : stop;
-                const int ctx = seq_ctx(p, ib);
+                const int ctx = ctx_of(ib);
                 const long long end = (e - s0) * kTile;
+                iTable = p.table + (size_t)ib * p.maxPages;
                 iTok = (int)((r - s0) * kTile);
                 iEnd = (int)(end < ctx ? end : ctx);
                 iNext = (long long)iUnit * T + e;
             }
-            const int tok = iTok + lane;
-            const int entry = p.pageShift >= 0 ? tok >> p.pageShift : tok / p.pageSize;
-            inPage = (uint32_t)(tok - entry * p.pageSize);
-            entryPage = tok < iEnd ? __ldg(p.table + (size_t)ib * p.maxPages + entry) : 0;
+#pragma unroll
+            for (int i = 0; i < PL; i++) {
+                const int tok = PAGED ? iTok + tileOf * kTile : iTok + lane + 32 * i;
+                const int entry = p.pageShift >= 0 ? tok >> p.pageShift : tok / p.pageSize;
+                inPage[i] = (uint32_t)(tok - entry * p.pageSize) + headOff;
+                entryPage[i] = tok < iEnd ? __ldg(iTable + entry) : 0;
+            }
         };
-        // Copies the step that look_ahead found (tokens past its end are zero-filled: step and least 0, codes 0) and looks for the next.
+        // Copies the step that look_ahead found and looks for the next.  PAGED copies whole tiles (a tile lies in one page), so tokens
+        // behind the sequence come along and are masked; otherwise they are zero-filled.
         auto issue = [&]() {
             if (iTok < iEnd) {
-                const bool live = iTok + lane < iEnd;
-                int page = entryPage;
-                if (page < 0 || page >= p.pageCount) {
-                    atomicExch(p.errorFlag, 1);
-                    page = 0;  // never dereferenced
-                }
-                const uint32_t kvh = (uint32_t)iUnit / (uint32_t)p.blocks;
-                const uint32_t slot = live ? ((uint32_t)page * (uint32_t)p.kvHeads + kvh) * (uint32_t)p.pageSize + inPage : 0u;
-                const uint32_t st = base + iStage * S::STAGE;
-                copy4(st + 2 * kStep * ROW + lane * 4, p.kParams + slot, live ? 4 : 0);
-                copy4(st + 2 * kStep * ROW + kStep * 4 + lane * 4, p.vParams + slot, live ? 4 : 0);
-                constexpr int PER = ROW / 16;  // 16-byte pieces of a token
+                uint32_t slot[PL];
 #pragma unroll
-                for (int i = 0; i < PER; i++) {
-                    const int token = (lane + 32 * i) / PER, piece = (lane + 32 * i) % PER;
-                    const uint32_t src = __shfl_sync(0xffffffffu, slot, token);
-                    const uint32_t bytes = iTok + token < iEnd ? 16u : 0u;
-                    // pieces 2, 3 before 0, 1 in every second pair of tokens: four tokens' 32-byte halves then lie in different banks
-                    const uint32_t dst = st + token * ROW + ((piece ^ (PER == 4 ? (token & 2) : 0)) * 16);
-                    copy16(dst, p.kCodes + (size_t)src * ROW + piece * 16, bytes, pol);
-                    copy16(dst + kStep * ROW, p.vCodes + (size_t)src * ROW + piece * 16, bytes, pol);
+                for (int i = 0; i < PL; i++) {
+                    if ((uint32_t)entryPage[i] >= (uint32_t)p.pageCount) {
+                        atomicExch(p.errorFlag, 1);
+                        entryPage[i] = 0;  // never dereferenced
+                    }
+                    slot[i] = (uint32_t)entryPage[i] * pageSlots + inPage[i];
+                }
+                const uint32_t st = base + iStage * S::STAGE;
+                if (PAGED) {
+                    const uint32_t bar = bars + 8 * iStage;
+                    const int tiles = min((iEnd - iTok + kTile - 1) / kTile, MT);
+                    if (lane == 0)
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(tiles * (2 * kTile * ROW + 2 * kTile * 4)) : "memory");
+                    __syncwarp();
+                    if (lane < 4 * tiles) bulk(st + dstOff, pool + (size_t)slot[0] * perSlot, kTile * perSlot, bar, pol);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < PL; i++) {
+                        const bool live = iTok + lane + 32 * i < iEnd;
+                        if (!live) slot[i] = 0;
+                        copy4(st + 2 * kStep * ROW + (lane + 32 * i) * 4, p.kParams + slot[i], live ? 4 : 0);
+                        copy4(st + 2 * kStep * ROW + kStep * 4 + (lane + 32 * i) * 4, p.vParams + slot[i], live ? 4 : 0);
+                    }
+                    constexpr int PER = ROW / 16;  // 16-byte pieces of a token
+#pragma unroll
+                    for (int i = 0; i < PER * PL; i++) {
+                        const int token = (lane + 32 * i) / PER, piece = (lane + 32 * i) % PER;
+                        const uint32_t src = __shfl_sync(0xffffffffu, slot[i / PER], token & 31);
+                        const uint32_t bytes = iTok + token < iEnd ? 16u : 0u;
+                        const uint32_t dst = st + (lane + 32 * i) * 16;
+                        copy16(dst, p.kCodes + (size_t)src * ROW + piece * 16, bytes, pol);
+                        copy16(dst + kStep * ROW, p.vCodes + (size_t)src * ROW + piece * 16, bytes, pol);
+                    }
                 }
                 iTok += kStep;
                 look_ahead();
             }
             if (++iStage == S::STAGES) iStage = 0;
-            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (!PAGED) asm volatile("cp.async.commit_group;" ::: "memory");
         };
         look_ahead();
 #pragma unroll
         for (int s = 0; s < S::STAGES - 1; s++) issue();
 
-        // rows of a tile: row r is token rowTok(r); pairs of rows differ in the lowest bit and even rows cover all four classes mod 4, so that
-        // neither the K nor the V loads meet in a bank
+        // rows of a tile: row r is token rowTok(r): neighbouring rows differ in the lowest bit of their token, so the K loads of eight lanes
+        // cover all banks, and even rows' tokens lie in both halves of 128 bytes (the V loads of D = 128 take two turns all the same)
         auto rowTok = [](int r) { return r < 4 ? r : r ^ 1; };
-        const int tokG = rowTok(g), tokA = rowTok(2 * t), tokB = rowTok(2 * t + 1);
-        const uint32_t kOff = ROW == 64 ? tokG * 64 + ((t ^ (tokG & 2)) * 16) : tokG * 32 + t * 8;
-        auto v_off = [&](int token) { return ROW == 64 ? token * 64 + ((((uint32_t)g >> 1) ^ (token & 2)) * 16) + (g & 1) * 8 : token * 32 + g * 4; };
-        const uint32_t vOffA = v_off(tokA), vOffB = v_off(tokB);
+        const int tokG = rowTok(g);
+        const uint32_t kOff = tokG * ROW + t * (ROW / 4);
+        const uint32_t vOffA = rowTok(2 * t) * ROW + g * (ROW / 8), vOffB = rowTok(2 * t + 1) * ROW + g * (ROW / 8);
 
         int stage = 0;
+        uint32_t parity = 0;  // of the stages' barriers
+        bool okay = true;
         long long cur = lo;
         while (cur < hi) {
             long long r = cur - (long long)cUnit * T;
@@ -308,16 +387,60 @@ __global__ void __launch_bounds__(Shape<DT, D, NT>::WARPS * 32, 1) decode_kernel
             while (ts[cb + 1] <= r) cb++;
             const int b = cb;
             const long long s0 = ts[b], s1 = ts[b + 1], stop = hi - (long long)cUnit * T, e = s1 < stop ? s1 : stop;
-            const int ctx = seq_ctx(p, b);
+            const int ctx = ctx_of(b);
             const int tok0 = (int)((r - s0) * kTile);
             const long long endTok = (e - s0) * kTile;
             const int tokEnd = (int)(endTok < ctx ? endTok : ctx);
             const int kvh = cUnit / p.blocks, block = cUnit % p.blocks;
             const int head0 = kvh * p.group + block * S::HEADS, heads = min(p.group - block * S::HEADS, S::HEADS);
 
-            // ---- queries: f16 fragments in the order of the masks, scaled by 2^-qe; sums for the least terms ----
-            uint32_t qb[WK][NT][4];  // [word][block of heads][dims (0,4), (2,6), (1,5), (3,7)]
-            float qScale[NT][2], qSum[NT][2];
+            // ---- queries, and their sums for the least terms.
+            // QUAD: integers Q = q 32600 / max |q| (an error of 2^-16 of the largest element), in signed bytes.  With L and F as above,
+            // 16 q . n = sum (16 Q_even - Q_odd) L + Q_odd F: three and two bytes.  Column 2h takes the middle byte of head h and column 2h + 1 the
+            // lowest, so a lane finds both in its two accumulators; the top byte has products of its own.
+            // Otherwise: f16 fragments in the order of the masks, scaled by 2^-qe (and by 1/16 where the codes come 16-fold). ----
+            uint32_t qb[WK][NT][4];  // f16: [word][block of heads][dims (0,4), (2,6), (1,5), (3,7)]; QUAD: [word][0][bytes for L, top for L, for F]
+            float qScale[NT][J], qSum[NT][J];
+            if (QUAD) {
+                float x[WK][8], big = 0.f, sum = 0.f;
+                const int h = g >> 1;
+                const uint16_t* row = p.q + ((size_t)b * p.numHeads + head0 + (h < heads ? h : 0)) * D + t * (D / 4);
+#pragma unroll
+                for (int w = 0; w < WK; w++) {
+                    const uint4 raw = __ldg((const uint4*)(row + 8 * w));
+                    unpack16_arith<DT>(raw.x, x[w][0], x[w][1]);
+                    unpack16_arith<DT>(raw.y, x[w][2], x[w][3]);
+                    unpack16_arith<DT>(raw.z, x[w][4], x[w][5]);
+                    unpack16_arith<DT>(raw.w, x[w][6], x[w][7]);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        if (h >= heads) x[w][i] = 0.f;
+                        big = fmaxf(big, fabsf(x[w][i]));
+                        sum += x[w][i];
+                    }
+                }
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                big = fminf(fmaxf(big, 1e-30f), 1e36f);
+                const float toInt = 32600.f / big;
+#pragma unroll
+                for (int w = 0; w < WK; w++) {
+                    qb[w][0][0] = qb[w][0][1] = qb[w][0][2] = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int even = __float2int_rn(x[w][2 * i] * toInt);
+                        int odd = __float2int_rn(x[w][2 * i + 1] * toInt), mix = 16 * even - odd;
+                        const uint32_t m0 = limb(mix), m1 = limb(mix), o0 = limb(odd);
+                        qb[w][0][0] |= ((g & 1) ? m0 : m1) << (8 * i);
+                        qb[w][0][1] |= ((g & 1) ? 0u : (uint32_t)mix & 255u) << (8 * i);
+                        qb[w][0][2] |= ((g & 1) ? o0 : (uint32_t)odd & 255u) << (8 * i);
+                    }
+                }
+                qScale[0][0] = __shfl_sync(0xffffffffu, big * (p.scaleLog2 / (16.f * 32600.f * 4096.f)), 8 * t);
+                qSum[0][0] = __shfl_sync(0xffffffffu, sum * p.scaleLog2, 8 * t);
+            } else {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 float x[WK][8], big = 0.f, sum = 0.f;
@@ -341,28 +464,36 @@ __global__ void __launch_bounds__(Shape<DT, D, NT>::WARPS * 32, 1) decode_kernel
                 big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                // the largest element to [2^14, 2^15): elements down to 2^-21 of it keep all bits of bf16
+                // the largest element to [2^14, 2^15): elements down to 2^-17 of it keep all bits of bf16, with the 1/16 too
                 const int qe = big > 0.f ? min(max((int)(__float_as_uint(big) >> 23) - 141, -112), 112) : 0;
-                const float down = pow2(-qe);
+                const float down = pow2(-qe), odd = down * 0.0625f;
 #pragma unroll
                 for (int w = 0; w < WK; w++) {
-                    qb[w][nt][0] = pack16_arith<DT_F16>(x[w][0] * down, x[w][4] * down);
-                    qb[w][nt][1] = pack16_arith<DT_F16>(x[w][2] * down, x[w][6] * down);
-                    qb[w][nt][2] = pack16_arith<DT_F16>(x[w][1] * down, x[w][5] * down);
-                    qb[w][nt][3] = pack16_arith<DT_F16>(x[w][3] * down, x[w][7] * down);
+                    float lo[4], hi[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        hi[i] = x[w][2 * i + 1] * odd;
+                        lo[i] = x[w][2 * i] * down;
+                    }
+                    qb[w][nt][0] = pack16_arith<DT_F16>(lo[0], lo[2]);
+                    qb[w][nt][1] = pack16_arith<DT_F16>(lo[1], lo[3]);
+                    qb[w][nt][2] = pack16_arith<DT_F16>(hi[0], hi[2]);
+                    qb[w][nt][3] = pack16_arith<DT_F16>(hi[1], hi[3]);
                 }
-                const float up = pow2(qe) * p.scaleLog2, scaled = sum * p.scaleLog2;
+                // (2^24 puts the subnormals' unit back: 2^136 at most in the two factors of a score together)
+                const float up = pow2(qe) * p.scaleLog2 * 4096.f, scaled = sum * p.scaleLog2;
 #pragma unroll
                 for (int j = 0; j < 2; j++) {  // this lane's score columns: heads 2t, 2t + 1
-                    qScale[nt][j] = __shfl_sync(0xffffffffu, up, (2 * t + j) * 4);
-                    qSum[nt][j] = __shfl_sync(0xffffffffu, scaled, (2 * t + j) * 4);
+                    qScale[nt][j % J] = __shfl_sync(0xffffffffu, up, (2 * t + j) * 4);
+                    qSum[nt][j % J] = __shfl_sync(0xffffffffu, scaled, (2 * t + j) * 4);
                 }
             }
+            }
 
-            // O^T in units of 2^-24 2^ve (odd dimensions: 16 times that): word w, pair i: [0], [1] = dim base + 8w + 2i of heads 2t, 2t + 1,
-            // [2], [3] = the dim behind it; base = g * D / 8
+            // O^T in units of 2^-24 2^ve: word w, pair i: [0], [1] = dim base + 8w + 2i of heads 2t, 2t + 1; [2], [3] = that dim plus 16
+            // times the one behind it; base = g * D / 8.  QUAD: [0], [2] of head t ([1], [3] stay zero)
             float o[WV][4][NT][4];
-            float m[NT][2], l[NT][2], z[NT][2];
+            float m[NT][J], l[NT][J], z[NT][J];
 #pragma unroll
             for (int w = 0; w < WV; w++)
 #pragma unroll
@@ -372,114 +503,222 @@ __global__ void __launch_bounds__(Shape<DT, D, NT>::WARPS * 32, 1) decode_kernel
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int j = 0; j < 2; j++) { m[nt][j] = -INFINITY; l[nt][j] = 0.f; z[nt][j] = 0.f; }
-            int ve = -110;  // exponent of the power of two that the weights are relative to
+                for (int j = 0; j < J; j++) { m[nt][j] = -INFINITY; l[nt][j] = 0.f; z[nt][j] = 0.f; }
+            // the weights are relative to m (per head) and to 2^ve: references that move only when the exponentials of a lane add up to more
+            // than kMost or its steps to more than 2 MT 2^ve, so most steps neither reduce a maximum over the lanes nor touch the accumulators.  A
+            // weight is then at most kMost 2 MT = 8192: inside f16, and float32 sums do not mind.
+            int ve = -110;
+            float veUp = pow2(-110), veInv = pow2(110);
+            float from[NT][J];  // the reference in use: m, or 0 while there is none (nothing but scores of -inf)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) from[nt][0] = from[nt][J - 1] = 0.f;
+            constexpr float kMost = 1024.f;
+            float limit = -INFINITY;  // -inf until every head of this lane has a reference
 
             for (int tk = tok0; tk < tokEnd; tk += kStep) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2) : "memory");
+                if (PAGED) {
+                    okay = okay && __all_sync(0xffffffffu, landed(bars + 8 * stage, parity));
+                    if (!okay) {  // the range is gone through all the same, so that every arrival is counted; its rows are NaN
+                        atomicExch(p.errorFlag, 3);
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) l[nt][0] = l[nt][J - 1] = NAN;
+                        break;
+                    }
+                } else {
+                    asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2) : "memory");
+                }
                 __syncwarp();
                 issue();
                 const uint32_t st = base + stage * S::STAGE;
-                if (++stage == S::STAGES) stage = 0;
+                if (++stage == S::STAGES) {
+                    stage = 0;
+                    parity ^= 1;
+                }
                 // ---- scores ----
-                float se[2][NT][4], so[2][NT][4];
+                float se[MT][NT][4];
+                {
+                    uint32_t rows[MT][2][4];
 #pragma unroll
-                for (int mt = 0; mt < 2; mt++) {
+                    for (int mt = 0; mt < MT; mt++) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
+                        for (int i = 0; i < 2; i++) {
+                            const uint32_t at = st + (mt * 16 + i * 8) * ROW + kOff;
+                            if (WK == 4) lds128(at, rows[mt][i]);
+                            else lds64(at, rows[mt][i]);
+                        }
+                    }
+                    // (tiles innermost: the products of a tile wait for one another)
+                    if (QUAD) {
+                        int mid[MT][4], top[MT][4];  // 256 and 1 times a sum; 65536 times a sum
 #pragma unroll
-                        for (int i = 0; i < 4; i++) se[mt][nt][i] = so[mt][nt][i] = 0.f;
-                    uint32_t lowRow[4], highRow[4];
-                    const uint32_t at = st + mt * 16 * ROW + kOff;
-                    if (WK == 4) { lds128(at, lowRow); lds128(at + 8 * ROW, highRow); }
-                    else { lds64(at, lowRow); lds64(at + 8 * ROW, highRow); }
+                        for (int w = 0; w < WK; w += 2) {
+#pragma unroll
+                            for (int mt = 0; mt < MT; mt++) {
+                                const uint32_t* x = rows[mt][0] + w;
+                                const uint32_t* y = rows[mt][1] + w;
+                                const uint32_t x0 = x[0] & 0x0F0F0F0Fu, y0 = y[0] & 0x0F0F0F0Fu, x1 = x[1] & 0x0F0F0F0Fu, y1 = y[1] & 0x0F0F0F0Fu;
+                                if (w == 0) {
+                                    imma0(mid[mt], x0, y0, x1, y1, qb[w][0][0], qb[w + 1][0][0]);
+                                    imma0(top[mt], x0, y0, x1, y1, qb[w][0][1], qb[w + 1][0][1]);
+                                } else {
+                                    imma(mid[mt], x0, y0, x1, y1, qb[w][0][0], qb[w + 1][0][0]);
+                                    imma(top[mt], x0, y0, x1, y1, qb[w][0][1], qb[w + 1][0][1]);
+                                }
+                                imma(mid[mt], x[0], y[0], x[1], y[1], qb[w][0][2], qb[w + 1][0][2]);
+                            }
+                        }
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++) {  // at most 16 * 32600 * 15 * 128 < 2^30
+                            se[mt][0][0] = (float)(top[mt][0] * 65536 + mid[mt][0] * 256 + mid[mt][1]);
+                            se[mt][0][2] = (float)(top[mt][2] * 65536 + mid[mt][2] * 256 + mid[mt][3]);
+                        }
+                    } else
 #pragma unroll
                     for (int w = 0; w < WK; w++) {
-                        const uint32_t x = lowRow[w], y = highRow[w], x8 = x >> 8, y8 = y >> 8;
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            mma(se[mt][nt], x & 0x000F000Fu, y & 0x000F000Fu, x8 & 0x000F000Fu, y8 & 0x000F000Fu, qb[w][nt][0], qb[w][nt][1]);
-                            mma(so[mt][nt], x & 0x00F000F0u, y & 0x00F000F0u, x8 & 0x00F000F0u, y8 & 0x00F000F0u, qb[w][nt][2], qb[w][nt][3]);
+                        for (int mt = 0; mt < MT; mt++) {
+                            const uint32_t x = rows[mt][0][w], y = rows[mt][1][w];
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) {
+                                if (w == 0) mma0(se[mt][nt], x & 0x000F000Fu, y & 0x000F000Fu, (x >> 8) & 0x000F000Fu, (y >> 8) & 0x000F000Fu, qb[w][nt][0], qb[w][nt][1]);
+                                else mma(se[mt][nt], x & 0x000F000Fu, y & 0x000F000Fu, (x >> 8) & 0x000F000Fu, (y >> 8) & 0x000F000Fu, qb[w][nt][0], qb[w][nt][1]);
+                            }
+                        }
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++) {
+                            const uint32_t x = rows[mt][0][w], y = rows[mt][1][w];
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++)
+                                mma(se[mt][nt], x & 0x00F000F0u, y & 0x00F000F0u, (x >> 8) & 0x00F000F0u, (y >> 8) & 0x00F000F0u, qb[w][nt][2], qb[w][nt][3]);
                         }
                     }
                 }
                 // ---- parameters of this lane's rows: token 8i + tokG ----
-                float ks[4], kl[4], vs[4], vl[4];
-                uint32_t top = 0;
+                const bool tail = tk + kStep > tokEnd;
+                const uint32_t params = st + 2 * kStep * ROW;
+                if (PAGED && tail) {  // whatever lies behind the sequence: step and least 0
+                    for (int i = lane; i < kStep; i += 32) {
+                        if (tk + i < tokEnd) continue;
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(params + i * 4), "r"(0) : "memory");
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(params + kStep * 4 + i * 4), "r"(0) : "memory");
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before a later copy into this stage
+                    }
+                    __syncwarp();
+                }
+                float ks[2 * MT], kl[2 * MT], vs[2 * MT], vl[2 * MT], vSum = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint32_t at = st + 2 * kStep * ROW + (8 * i + tokG) * 4;
+                for (int i = 0; i < 2 * MT; i++) {
+                    const uint32_t at = params + (8 * i + tokG) * 4;
                     unpack16_arith<DT>(lds32(at), ks[i], kl[i]);
                     unpack16_arith<DT>(lds32(at + kStep * 4), vs[i], vl[i]);
-                    ks[i] *= 16777216.f;
-                    top = max(top, __float_as_uint(vs[i]) & 0x7FFFFFFFu);
+                    ks[i] *= 4096.f;
+                    vSum += vs[i];
                 }
-                top = __reduce_max_sync(0xffffffffu, top);
-                const int need = min(max((int)((top + 0x7FFFFFu) >> 23) - 127, -110), 110);
-                float grow = 1.f;
-                if (need > ve) {  // uniform over the warp
-                    grow = ve - need < -126 ? 0.f : pow2(ve - need);
-                    ve = need;
-                }
-                const float veInv = pow2(-ve);
-                // ---- online softmax in the log2 domain ----
-                const bool tail = tk + kStep > tokEnd;
-                bool rescale = grow != 1.f;
-                float alpha[NT][2];
+                // ---- scores in the log2 domain, relative to the reference, and their exponentials ----
+                float x[NT][J][2 * MT], e[NT][J][2 * MT], eSum[NT][J], most = 0.f;
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        float x[4];
+                    for (int j = 0; j < J; j++) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float dot = fmaf(so[i >> 1][nt][2 * (i & 1) + j], 0.0625f, se[i >> 1][nt][2 * (i & 1) + j]);
-                            x[i] = fmaf(dot * ks[i], qScale[nt][j], kl[i] * qSum[nt][j]);
-                            if (tail && tk + 8 * i + tokG >= tokEnd) x[i] = -INFINITY;
-                        }
-                        float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                        const float mNew = fmaxf(m[nt][j], mx);
-                        const float from = mNew == -INFINITY ? 0.f : mNew;
-                        const float a = ex2(m[nt][j] - from);
-                        float sum = 0.f, least = 0.f;
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float w = ex2(x[i] - from);
-                            sum += w;
-                            least = fmaf(w, vl[i], least);
-                            se[i >> 1][nt][2 * (i & 1) + j] = w * (vs[i] * veInv);
-                        }
-                        l[nt][j] = fmaf(l[nt][j], a, sum);
-                        z[nt][j] = fmaf(z[nt][j], a, least);
-                        m[nt][j] = mNew;
-                        alpha[nt][j] = a * grow;
-                        rescale |= a != 1.f;
+                        for (int i = 0; i < 2 * MT; i++)
+                            x[nt][j][i] = fmaf(se[i >> 1][nt][2 * (i & 1) + j] * ks[i], qScale[nt][j], fmaf(kl[i], qSum[nt][j], -from[nt][j]));
                     }
                 }
-                if (__any_sync(0xffffffffu, rescale)) {
+                if (tail) {
+                    __syncwarp();  // (keeps this a branch: as selects it would cost every step)
 #pragma unroll
-                    for (int w = 0; w < WV; w++)
+                    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
+                        for (int i = 0; i < 2 * MT; i++)
+                            if (tk + 8 * i + tokG >= tokEnd) x[nt][0][i] = x[nt][J - 1][i] = -INFINITY;
+                }
+                auto exponentials = [&]() {
 #pragma unroll
-                            for (int nt = 0; nt < NT; nt++) {
-                                o[w][i][nt][0] *= alpha[nt][0];
-                                o[w][i][nt][1] *= alpha[nt][1];
-                                o[w][i][nt][2] *= alpha[nt][0];
-                                o[w][i][nt][3] *= alpha[nt][1];
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int j = 0; j < J; j++) {
+                            eSum[nt][j] = 0.f;
+#pragma unroll
+                            for (int i = 0; i < 2 * MT; i++) {
+                                e[nt][j][i] = ex2(x[nt][j][i]);
+                                eSum[nt][j] += e[nt][j][i];
                             }
+                        }
+                };
+                exponentials();
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) most += J == 2 ? eSum[nt][0] + eSum[nt][J - 1] : eSum[nt][0];
+                // (sums in the place of maxima: they run on another pipe than the logic instructions and cover the maxima)
+                if (__any_sync(0xffffffffu, most > limit || vSum > 2 * MT * veUp)) {
+                    float vTop = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 2 * MT; i++) vTop = fmaxf(vTop, vs[i]);
+                    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(vTop));
+                    const int need = max(ve, min((int)((top + 0x7FFFFFu) >> 23) - 127, 110));
+                    const float grow = ve - need < -126 ? 0.f : pow2(ve - need);
+                    ve = need;
+                    veUp = pow2(ve);
+                    veInv = pow2(-ve);
+                    limit = kMost;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        float alpha[J];
+#pragma unroll
+                        for (int j = 0; j < J; j++) {
+                            float mx = x[nt][j][0];
+#pragma unroll
+                            for (int i = 1; i < 2 * MT; i++) mx = fmaxf(mx, x[nt][j][i]);
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                            const float mNew = fmaxf(m[nt][j], mx + from[nt][j]);
+                            const float a = mNew == -INFINITY ? 1.f : ex2(m[nt][j] - mNew), next = mNew == -INFINITY ? 0.f : mNew;
+                            if (mNew == -INFINITY) limit = -INFINITY;  // still no reference: the next score makes one
+#pragma unroll
+                            for (int i = 0; i < 2 * MT; i++) x[nt][j][i] += from[nt][j] - next;
+                            l[nt][j] *= a;
+                            z[nt][j] *= a;
+                            m[nt][j] = mNew;
+                            from[nt][j] = next;
+                            alpha[j] = a * grow;
+                        }
+#pragma unroll
+                        for (int w = 0; w < WV; w++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                o[w][i][nt][0] *= alpha[0];
+                                o[w][i][nt][2] *= alpha[0];
+                                if (!QUAD) {
+                                    o[w][i][nt][1] *= alpha[J - 1];
+                                    o[w][i][nt][3] *= alpha[J - 1];
+                                }
+                            }
+                    }
+                    exponentials();
+                }
+#pragma unroll
+                for (int i = 0; i < 2 * MT; i++) vs[i] *= veInv;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                    for (int j = 0; j < J; j++) {
+                        l[nt][j] += eSum[nt][j];
+#pragma unroll
+                        for (int i = 0; i < 2 * MT; i++) {
+                            z[nt][j] = fmaf(e[nt][j][i], vl[i], z[nt][j]);
+                            se[i >> 1][nt][2 * (i & 1) + j] = e[nt][j][i] * vs[i];
+                        }
+                    }
                 }
                 // ---- O^T += V^T P^T ----
 #pragma unroll
-                for (int mt = 0; mt < 2; mt++) {
+                for (int mt = 0; mt < MT; mt++) {
                     uint32_t pb[NT][2];
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        pb[nt][0] = transpose8(pack16_arith<DT_F16>(se[mt][nt][0], se[mt][nt][1]));
-                        pb[nt][1] = transpose8(pack16_arith<DT_F16>(se[mt][nt][2], se[mt][nt][3]));
+                        pb[nt][0] = transpose8(pack16_arith<DT_F16>(se[mt][nt][0], QUAD ? 0.f : se[mt][nt][1]));
+                        pb[nt][1] = transpose8(pack16_arith<DT_F16>(se[mt][nt][2], QUAD ? 0.f : se[mt][nt][3]));
                     }
                     const uint32_t at = st + kStep * ROW + mt * 16 * ROW;
                     uint32_t va[2], vb[2], vc[2], vd[2];  // tokens of rows 2t, 2t + 1, 2t + 8, 2t + 9
@@ -493,41 +732,46 @@ __global__ void __launch_bounds__(Shape<DT, D, NT>::WARPS * 32, 1) decode_kernel
 #pragma unroll
                         for (int half = 0; half < 2; half++) {
                             const uint32_t x = __byte_perm(va[w], vb[w], half ? 0x7632 : 0x5410), y = __byte_perm(vc[w], vd[w], half ? 0x7632 : 0x5410);
-                            const uint32_t x8 = x >> 8, y8 = y >> 8;
+                            const uint32_t x8 = __byte_perm(x, 0, 0x4341), y8 = __byte_perm(y, 0, 0x4341);
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) {
-                                mma(o[w][2 * half][nt], x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u, pb[nt][0], pb[nt][1]);
-                                mma(o[w][2 * half + 1][nt], x8 & 0x000F000Fu, x8 & 0x00F000F0u, y8 & 0x000F000Fu, y8 & 0x00F000F0u, pb[nt][0], pb[nt][1]);
+                                mma(o[w][2 * half][nt], x & 0x000F000Fu, x & 0x00FF00FFu, y & 0x000F000Fu, y & 0x00FF00FFu, pb[nt][0], pb[nt][1]);
+                                mma(o[w][2 * half + 1][nt], x8 & 0x000F000Fu, x8, y8 & 0x000F000Fu, y8, pb[nt][0], pb[nt][1]);
                             }
                         }
                     }
                 }
             }
 
-            // ---- end of this warp's part of the pair: the rows themselves, or a partial ----
+            // ---- end of this warp's part of the pair: the rows themselves, or a partial.  The last partial of a warp goes where its stages
+            // were (every copy has landed and been read), an earlier one to the scratch. ----
             const bool begun = r > s0, whole = !begun && e == s1;
             const int which = begun ? 0 : 1;
-            const long long slot = 2ll * (blockIdx.x * S::WARPS + warp) + which;
+            cur = (long long)cUnit * T + e;
+            const bool near = cur >= hi;
+            const long long slot = blockIdx.x * S::WARPS + warp;
+            float* const acc = near ? (float*)mine : p.acc + slot * S::HEADS * D;
+            float2* const ml = near ? (float2*)(mine + S::HEADS * D * 4) : p.ml + slot * S::HEADS;
+            if (!whole) __syncwarp();  // every lane has read the stages
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
+                for (int j = 0; j < J; j++) {
                     float sum = l[nt][j], least = z[nt][j];
 #pragma unroll
                     for (int off = 4; off < 32; off <<= 1) {
                         sum += __shfl_xor_sync(0xffffffffu, sum, off);
                         least += __shfl_xor_sync(0xffffffffu, least, off);
                     }
-                    const int h = nt * 8 + 2 * t + j;
+                    const int h = QUAD ? t : nt * 8 + 2 * t + j;
                     if (h >= heads) continue;
-                    const float unit = pow2(ve);
                     float x[8 * WV];
 #pragma unroll
                     for (int w = 0; w < WV; w++)
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            x[8 * w + 2 * i] = fmaf(o[w][i][nt][j] * 16777216.f, unit, least);
-                            x[8 * w + 2 * i + 1] = fmaf(o[w][i][nt][2 + j] * 1048576.f, unit, least);
+                            x[8 * w + 2 * i] = fmaf(o[w][i][nt][j] * 16777216.f, veUp, least);
+                            x[8 * w + 2 * i + 1] = fmaf((o[w][i][nt][2 + j] - o[w][i][nt][j]) * 1048576.f, veUp, least);
                         }
                     if (whole) {
                         uint16_t* dst = p.out + ((size_t)b * p.numHeads + head0 + h) * D + g * (D / 8);
@@ -541,86 +785,211 @@ __global__ void __launch_bounds__(Shape<DT, D, NT>::WARPS * 32, 1) decode_kernel
                             *(uint4*)(dst + 8 * w) = v;
                         }
                     } else {
-                        float* dst = p.acc + (slot * S::HEADS + h) * D + g * (D / 8);
+                        float* dst = acc + h * D + g * (D / 8);
 #pragma unroll
                         for (int i = 0; i < 2 * WV; i++) *(float4*)(dst + 4 * i) = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-                        if (g == 0) p.ml[slot * S::HEADS + h] = make_float2(m[nt][j], sum);
+                        if (g == 0) ml[h] = make_float2(m[nt][j], sum);
                     }
                 }
             }
-            if (!whole && lane == 0) sSeg[2 * warp + which] = cUnit * p.batch + b;
-            cur = (long long)cUnit * T + e;
+            if (!whole && lane == 0) {
+                const int at = 2 * warp + which;
+                const long long gs = (long long)cUnit * T + s0, ge = (long long)cUnit * T + s1;
+                sSeg[at] = cUnit * p.batch + b;
+                sB[at] = b;
+                sUnit[at] = cUnit;
+                sWhere[at] = gs >= clo && ge <= chi ? 2 : gs < clo ? 0 : 1;
+                if (near) sNear[warp] = which;
+            }
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (!PAGED) asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
 
-    // ---- pairs that several warps of this CTA share: joined here; written, or left as the CTA's partial ----
+    // ---- pairs that several warps of this CTA share: joined here, a warp per (pair, head), D / 32 dimensions a lane; written, or left as
+    // the CTA's partial in the scratch.  (From here on every instruction runs once per launch and comes cold from the instruction
+    // cache: short code before fast code.) ----
     __syncthreads();
-    const long long ctaSlots = 2ll * gridDim.x * S::WARPS;  // behind the warps' slots
-    int shared[2] = {-1, -1};  // pairs that this CTA shares with its neighbours: began before its range / goes on behind it
-    for (int e0 = 0; e0 < 2 * S::WARPS;) {
-        const int seg = sSeg[e0];
-        if (seg < 0) { e0++; continue; }
-        int e1 = e0 + 1;
-        while (e1 < 2 * S::WARPS && (sSeg[e1] < 0 || sSeg[e1] == seg)) e1++;
-        const int unit = seg / p.batch, b = seg % p.batch, block = unit % p.blocks;
-        const int head0 = (unit / p.blocks) * p.group + block * S::HEADS, heads = min(p.group - block * S::HEADS, S::HEADS);
-        const long long gs = (long long)unit * T + ts[b], ge = (long long)unit * T + ts[b + 1];
-        const bool mine = gs >= clo && ge <= chi;
-        const int which = gs < clo ? 0 : 1;
-        const long long slot = ctaSlots + 2ll * blockIdx.x + which;
-        if (!mine) shared[which] = seg;
-        auto slot_of = [&](int i) -> long long { return sSeg[e0 + i] < 0 ? -1ll : 2ll * blockIdx.x * S::WARPS + e0 + i; };
-        join<D>(p, heads, S::HEADS, e1 - e0, slot_of, [&](int h, int d, float M, float den, float4 num) {
-            if (mine) {
-                store4<DT>(p.out + ((size_t)b * p.numHeads + head0 + h) * D + d, den, num);
-            } else {
-                *(float4*)(p.acc + (slot * S::HEADS + h) * D + d) = num;
-                if (d == 0) p.ml[slot * S::HEADS + h] = make_float2(M, den);
+    const long long ctaSlots = (long long)gridDim.x * S::WARPS;  // behind the warps' slots, two per CTA
+    constexpr int E = D / 32;
+    {
+        const int seg = sSeg[lane];
+        const uint32_t have = __ballot_sync(0xffffffffu, seg >= 0);
+        const uint32_t below = have & ((1u << lane) - 1);
+        const int before = __shfl_sync(0xffffffffu, seg, below ? 31 - __clz(below) : lane);
+        const uint32_t starts = __ballot_sync(0xffffffffu, seg >= 0 && (!below || before != seg));
+        if (warp == 0 && (starts >> lane & 1) && sWhere[lane] < 2) sShared[sWhere[lane]] = lane;
+        for (int item = warp; item < __popc(starts) * S::HEADS; item += S::WARPS) {
+            const int h = item % S::HEADS;
+            uint32_t left = starts;
+            for (int i = item / S::HEADS; i > 0; i--) left &= left - 1;
+            const int e0 = __ffs(left) - 1;
+            left &= left - 1;
+            const uint32_t members = have & (left ? (1u << (__ffs(left) - 1)) - 1 : 0xffffffffu) & ~((1u << e0) - 1);
+            const int unit = sUnit[e0], where = sWhere[e0];
+            const int kvh = unit / p.blocks, block = unit - kvh * p.blocks, head = block * S::HEADS + h;
+            if (head >= p.group) continue;
+            // (a warp has at most one entry in a pair: entry e is of warp e / 2; lane i looks at warp w0 + i)
+            const int w0 = e0 >> 1, n = ((31 - __clz(members)) >> 1) - w0 + 1, w = w0 + lane;
+            const uint32_t bits = lane < n ? (members >> (2 * w)) & 3 : 0;
+            float2 ml = make_float2(-INFINITY, 0.f);
+            const float* at = p.acc;  // (where there is no partial: not read)
+            if (bits) {
+                const unsigned char* own = smemRaw + w * (S::STAGES * S::STAGE);
+                const long long far = (long long)blockIdx.x * S::WARPS + w;
+                const bool near = sNear[w] == (bits & 1 ? 0 : 1);
+                ml = near ? ((const float2*)(own + S::HEADS * D * 4))[h] : p.ml[far * S::HEADS + h];
+                at = (near ? (const float*)own : p.acc + far * (S::HEADS * D)) + h * D;
             }
-        });
-        e0 = e1;
-    }
-    if (shared[0] < 0 && shared[1] < 0) return;  // uniform over the CTA
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x < 2) {
-        const int seg = threadIdx.x == 0 ? shared[0] : shared[1];
-        int last = 0;
-        if (seg >= 0) {
-            const int unit = seg / p.batch, b = seg % p.batch;
-            const long long gs = (long long)unit * T + ts[b], ge = (long long)unit * T + ts[b + 1];
-            const int owners = part_of(ge - 1, total, parts) - part_of(gs, total, parts) + 1;
-            last = atomicAdd(p.counters + seg, 1) == owners - 1;
-            if (last) p.counters[seg] = 0;  // nobody else comes in this launch
+            float M = ml.x;
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+            const float k = weight(ml, M);
+            float den = ml.y * k, num[E] = {};
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) den += __shfl_xor_sync(0xffffffffu, den, off);
+#pragma unroll 2
+            for (int i = 0; i < n; i++) {
+                const float wt = __shfl_sync(0xffffffffu, k, i);
+                const float* from = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)at, i);
+                if (!((members >> (2 * (w0 + i))) & 3)) continue;  // uniform
+#pragma unroll
+                for (int d = 0; d < E; d++) num[d] = fmaf(from[lane + 32 * d], wt, num[d]);
+            }
+            const long long slot = (ctaSlots + 2ll * blockIdx.x + where) * S::HEADS + h;
+            if (where == 2) {
+                uint16_t* dst = p.out + ((size_t)sB[e0] * p.numHeads + kvh * p.group + head) * D + lane;
+#pragma unroll
+                for (int d = 0; d < E; d++) Storage<DT>::store(dst, 32 * d, num[d] / den);
+            } else {
+#pragma unroll
+                for (int d = 0; d < E; d++) p.acc[slot * D + lane + 32 * d] = num[d];
+                if (lane == 0) p.ml[slot] = make_float2(M, den);
+            }
         }
-        sLast[threadIdx.x] = last;
-        __threadfence();
     }
     __syncthreads();
+    if (sShared[0] < 0 && sShared[1] < 0) return;  // uniform over the CTA
+    // ---- pairs that several CTAs share ----
+    if (threadIdx.x < 2) {
+        const int e = sShared[threadIdx.x];
+        int go = 0;
+        if (e >= 0) {
+            const long long at = (long long)sUnit[e] * T;
+            const int first = split.holding(at + ts[sB[e]]), owners = split.holding(at + ts[sB[e] + 1] - 1) - first + 1;
+            int* const counter = p.counters + sSeg[e];
+            sFirst[threadIdx.x] = first;
+            sOwners[threadIdx.x] = owners;
+            __threadfence();  // the CTA's partial (ordered before this thread by the barrier) before its arrival
+            const int came = atomicAdd(counter, 1);
+            if (p.together) {
+                go = 1;
+                int seen;
+                for (unsigned spins = 0;; spins++) {
+                    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(seen) : "l"(counter) : "memory");
+                    if (seen >= owners) break;
+                    if (spins > (1u << 21)) {  // about a second: an owner never arrived
+                        atomicExch(p.errorFlag, 4);
+                        go = 0;
+                        break;
+                    }
+                    __nanosleep(40);
+                }
+            } else {
+                go = came == owners - 1;
+                if (go) *counter = 0;  // nobody else comes in this launch
+            }
+            __threadfence();
+        }
+        sGo[threadIdx.x] = go;
+    }
+    __syncthreads();
+    float* const sums = (float*)smemRaw;  // [warp][32] sums, then maximum and sum of weights
     for (int s = 0; s < 2; s++) {
-        if (!sLast[s]) continue;
-        const int seg = shared[s], unit = seg / p.batch, b = seg % p.batch, block = unit % p.blocks;
-        const int head0 = (unit / p.blocks) * p.group + block * S::HEADS, heads = min(p.group - block * S::HEADS, S::HEADS);
-        const long long gs = (long long)unit * T + ts[b], ge = (long long)unit * T + ts[b + 1];
-        const int c0 = part_of(gs, total, parts), c1 = part_of(ge - 1, total, parts);
-        auto slot_of = [&](int i) -> long long { return ctaSlots + 2ll * (c0 + i) + (gs < (c0 + i) * total / parts ? 0 : 1); };
-        join<D>(p, heads, S::HEADS, c1 - c0 + 1, slot_of, [&](int h, int d, float M, float den, float4 num) {
-            store4<DT>(p.out + ((size_t)b * p.numHeads + head0 + h) * D + d, den, num);
-        });
+        if (!sGo[s]) continue;
+        const int e = sShared[s], n = sOwners[s], unit = sUnit[e], kvh = unit / p.blocks, block = unit - kvh * p.blocks;
+        const int heads = min(p.group - block * S::HEADS, S::HEADS);
+        // this CTA's slices (of 32 dimensions): rank, rank + of, ...; a warp per slice, or several that take every `ways`-th owner each
+        const int rank = p.together ? blockIdx.x - sFirst[s] : 0, of = p.together ? n : 1;
+        const int mine = rank < heads * E ? (heads * E - rank + of - 1) / of : 0, cols = min(mine, S::WARPS), ways = cols ? S::WARPS / cols : 1;
+        // slot of owner i: the pair begins inside the first one's range and before the others'
+        const long long slot0 = ctaSlots + 2ll * sFirst[s];
+        for (int c0 = 0; c0 < mine; c0 += cols) {
+            const int way = warp / cols, c = c0 + warp - way * cols, slice = rank + c * of, h = slice / E;
+            const bool on = way < ways && c < mine;
+            float M = -INFINITY, den = 0.f, num = 0.f;
+            if (on) {
+                for (int i0 = way; i0 < n; i0 += 8 * ways) {
+                    float2 ml[8];
+                    float a[8], Mn = M;
+#pragma unroll
+                    for (int u = 0; u < 8; u++) {
+                        const int i = i0 + u * ways;
+                        const long long row = (slot0 + 2 * i + (i == 0 ? 1 : 0)) * S::HEADS + h;
+                        ml[u] = make_float2(-INFINITY, 0.f);
+                        a[u] = 0.f;
+                        if (i < n) {
+                            ml[u] = __ldcg(p.ml + row);
+                            a[u] = __ldcg(p.acc + row * D + (slice % E) * 32 + lane);
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < 8; u++) Mn = fmaxf(Mn, ml[u].x);
+                    const float old = weight(make_float2(M, den), Mn);
+                    den *= old;
+                    num *= old;
+                    M = Mn;
+#pragma unroll
+                    for (int u = 0; u < 8; u++) {
+                        const float w = weight(ml[u], M);
+                        den = fmaf(ml[u].y, w, den);
+                        num = fmaf(a[u], w, num);
+                    }
+                }
+            }
+            if (ways > 1) {
+                float* const mineAt = sums + warp * 34;
+                __syncthreads();
+                mineAt[lane] = num;
+                if (lane == 0) {
+                    mineAt[32] = M;
+                    mineAt[33] = den;
+                }
+                __syncthreads();
+                if (on && way == 0) {
+                    float all = M;
+                    for (int w = 1; w < ways; w++) all = fmaxf(all, mineAt[w * cols * 34 + 32]);
+                    float total = 0.f, sum = 0.f;
+                    for (int w = 0; w < ways; w++) {
+                        const float* other = mineAt + w * cols * 34;
+                        const float k = weight(make_float2(other[32], other[33]), all);
+                        total = fmaf(other[33], k, total);
+                        sum = fmaf(other[lane], k, sum);
+                    }
+                    den = total;
+                    num = sum;
+                }
+            }
+            if (on && way == 0)
+                Storage<DT>::store(p.out, ((size_t)sB[e] * p.numHeads + kvh * p.group + block * S::HEADS + h) * D + (slice % E) * 32 + lane, num / den);
+        }
+    }
+    if (!p.together) return;
+    __syncthreads();
+    if (threadIdx.x < 2 && sShared[threadIdx.x] >= 0) {  // the last owner to leave a pair returns its counter to zero
+        int* const counter = p.counters + sSeg[sShared[threadIdx.x]];
+        if (atomicAdd(counter, 1) == 2 * sOwners[threadIdx.x] - 1) *counter = 0;
     }
 }
 
-template <int DT, int D, int NT>
+template <int DT, typename S>
 static int launch(Context* ctx, Params& p, CUDAStatus* status) {
-    using S = Shape<DT, D, NT>;
     const char* what = "paged decode attention (4 bits)";
     const unsigned grid = (unsigned)ctx->smCount;
     p.blocks = (p.group + S::HEADS - 1) / S::HEADS;
     p.units = p.kvHeads * p.blocks;
     if ((long long)p.units * p.batch > 0x7FFFFFFFll) return fail(status, -2, "%s: batch times heads exceeds 31 bits", what);
-    const size_t slots = 2ull * grid * (S::WARPS + 1);
-    const size_t accBytes = slots * S::HEADS * D * 4, mlBytes = slots * S::HEADS * 8;
+    const size_t slots = (size_t)grid * (S::WARPS + 2);
+    const size_t accBytes = slots * S::HEADS * S::D * 4, mlBytes = slots * S::HEADS * 8;
     const size_t prefixBytes = p.batch > kPrefixSmem ? ((size_t)p.batch + 1) * 4 : 0;
     const size_t counterBytes = (size_t)p.units * p.batch * 4;
     Scratch ws;
@@ -638,8 +1007,17 @@ static int launch(Context* ctx, Params& p, CUDAStatus* status) {
         if (rc != 0) return rc;
         p.tileStart = prefix;
     }
-    cudaFuncSetAttribute(decode_kernel<DT, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-    decode_kernel<DT, D, NT><<<grid, S::WARPS * 32, S::SMEM, ctx->stream>>>(p);
+    // PUTER_DECODE_NO_COOPERATIVE (any value) forces the plain launch: the path a refused cooperative launch takes, reachable for tests
+    const bool cooperative = getenv("PUTER_DECODE_NO_COOPERATIVE") == nullptr;
+    const auto kernel = p.pageSize % kTile == 0 ? decode_kernel<DT, S, true> : decode_kernel<DT, S, false>;
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    p.together = 1;
+    void* args[] = {&p};
+    if (!cooperative || cudaLaunchCooperativeKernel((const void*)kernel, dim3(grid), dim3(S::WARPS * 32), args, S::SMEM, ctx->stream) != cudaSuccess) {
+        cudaGetLastError();
+        p.together = 0;
+        kernel<<<grid, S::WARPS * 32, S::SMEM, ctx->stream>>>(p);
+    }
     return check_launch(ctx, status, what);
 }
 
@@ -701,10 +1079,12 @@ extern "C" int cuda_dispatch_paged_decode_attention_q4(CUDADeviceRef contextRef,
     p.pageShift = -1;
     for (int s = 0; s < 31; s++)
         if (pageSize == (1u << s)) p.pageShift = s;
-    const int two = p.group > 8;
-#define DECODE(DT)                                                                                                                      \
-    (headDim == 128 ? (two ? q4d::launch<DT, 128, 2>(ctx, p, status) : q4d::launch<DT, 128, 1>(ctx, p, status))                      \
-                    : (two ? q4d::launch<DT, 64, 2>(ctx, p, status) : q4d::launch<DT, 64, 1>(ctx, p, status)))
-    return elementDType == DT_BF16 ? DECODE(DT_BF16) : DECODE(DT_F16);
+    // query heads per KV head: up to 4, up to 8, more (in blocks of 16)
+#define DECODE(DT, D)                                                                       \
+    (p.group <= 4   ? q4d::launch<DT, q4d::Shape<D, 0, 16, 2>>(ctx, p, status)               \
+     : p.group <= 8 ? q4d::launch<DT, q4d::Shape<D, 1, 8, 4>>(ctx, p, status)               \
+                    : q4d::launch<DT, q4d::Shape<D, 2, 8, 2>>(ctx, p, status))
+    if (headDim == 128) return elementDType == DT_BF16 ? DECODE(DT_BF16, 128) : DECODE(DT_F16, 128);
+    return elementDType == DT_BF16 ? DECODE(DT_BF16, 64) : DECODE(DT_F16, 64);
 #undef DECODE
 }
