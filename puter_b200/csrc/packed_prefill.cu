@@ -6,9 +6,24 @@
 // (device/cpu/attention/typed_compute.go:142-237): out_r = sum_{t <= r} p_t v_t, p = softmax(q_r . k_t / sqrt(D)).
 // Rows that belong to no sequence (before the first start, behind the last) are neither read into a result nor written.
 // A pair of starts that is not 0 <= start <= end <= totalTokens with at most maxSeqLen rows is skipped and raises the error flag.
+//
+// Two kernels.  rows_kernel is a warp per (row, head) for any type and head dimension.  pk::tiles_kernel is the tensor-core form (bf16 / f16,
+// head dimensions up to 128 that are multiples of 8), built like the prefill kernel for equal lengths: two tiles of 128 rows that take turns
+// on the tensor core, softmax in registers with one row a thread, P handed back through TMEM, K and V through a TMA ring.  What the
+// different lengths change:
+//   * A tile's 128 rows are PACK query heads of one KV head (PACK = the largest power of two in the group, 128 at most) times 128 / PACK
+//     positions: a group of 4 turns 33 tokens into 132 rows instead of 4 x 33 of 128, and short prompts are what packing is for.
+//     A TMA box of 64 dimensions x PACK heads x 128 / PACK rows brings such a tile in; long prompts cost the same either way.
+//   * The work list (sequence, block of 2 * 128 / PACK positions) is built on the device, longest key ranges first, by the first block of the
+//     launch that also rotates: the host never learns the lengths.
+//   * Keys behind the end of a sequence and keys that a row may not see are masked by position; their weights are exactly zero.  A value row
+//     that is not finite would still reach every row of the tile through 0 * NaN, so a warp looks through the value tiles that are not
+//     seen by all rows, clears what is not finite, and the rows that do see it add it back at the end.
+//   * The last rows of a sequence share their TMA box with the next sequence, so that box is written row by row.
 #include <math.h>
 
 #include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace puter {
 
@@ -110,6 +125,720 @@ __global__ void __launch_bounds__(256) rows_kernel(const void* __restrict__ q, c
     }
 }
 
+// ---------------------------------------------------------------------------------------------------------------------------------
+// the launch before the attention: block 0 builds the work list, the others rotate q and k
+// ---------------------------------------------------------------------------------------------------------------------------------
+struct Entry { int row0, len, pos, pad; };  // a block of `span` positions from pos on, of the sequence of `len` rows at row0
+
+struct Lists {
+    int* count;      // entries
+    Entry* entries;
+    int* above;      // [levels] scratch: sequences by number of blocks, then entries of higher levels
+    int* cursor;     // [levels] scratch
+    int span, levels, capacity;
+};
+
+// x[0 .. n) becomes its suffix sum (x[i] + x[i + 1] + ...), or the sum of what follows x[i] when `exclusive`.  The whole block calls it.
+__device__ void suffix_sum(int* x, int n, bool exclusive) {
+    __shared__ int sums[32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    int carry = 0;
+    for (int base = 0; base < n; base += blockDim.x) {
+        const int i = n - 1 - (base + (int)threadIdx.x);
+        const int v = i >= 0 ? x[i] : 0;
+        int incl = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 31) sums[warp] = incl;
+        __syncthreads();
+        int before = carry;
+        for (int w = 0; w < warps; w++) {
+            if (w < warp) before += sums[w];
+            carry += sums[w];
+        }
+        if (i >= 0) x[i] = before + incl - (exclusive ? v : 0);
+        __syncthreads();
+    }
+}
+
+// Entries by level (block number within the sequence: what decides its number of keys), highest first; within a level in any order.
+__device__ void build_list(const Seqs& s, const Lists& l) {
+    for (int i = threadIdx.x; i < l.levels; i += blockDim.x) l.above[i] = l.cursor[i] = 0;
+    __syncthreads();
+    for (int b = threadIdx.x; b < s.batch; b += blockDim.x) {
+        int s0, s1;
+        if (seq_rows(s, b, s0, s1)) atomicAdd(l.above + (s1 - s0 - 1) / l.span, 1);  // by its last block
+    }
+    __syncthreads();
+    suffix_sum(l.above, l.levels, false);  // entries per level: sequences with a block of that number
+    __shared__ int total;
+    if (threadIdx.x == 0) total = l.above[0];
+    __syncthreads();
+    suffix_sum(l.above, l.levels, true);   // entries of higher levels
+    if (threadIdx.x == 0) *l.count = min(total + l.above[0], l.capacity);  // (starts that go back can count rows twice)
+    const int lane = threadIdx.x & 31;
+    for (int b = threadIdx.x >> 5; b < s.batch; b += blockDim.x >> 5) {
+        int s0, s1;
+        if (!seq_rows(s, b, s0, s1)) continue;
+        const int blocks = (s1 - s0 + l.span - 1) / l.span;
+        for (int i = lane; i < blocks; i += 32) {
+            const int at = l.above[i] + atomicAdd(l.cursor + i, 1);
+            if (at < l.capacity) l.entries[at] = Entry{s0, s1 - s0, i * l.span, 0};
+        }
+    }
+}
+
+// Rotates [total, qHeads + kHeads, D] (two tensors, one row of both at a time, a warp per row) with 16-byte vectors.
+template <int DT>
+__global__ void __launch_bounds__(256) prologue_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, uint16_t* __restrict__ qOut,
+                                                       uint16_t* __restrict__ kOut, Seqs s, Lists l, const float* __restrict__ cosT,
+                                                       const float* __restrict__ sinT, int qHeads, int kHeads, int dim, int halfMode) {
+    if (blockIdx.x == 0) {
+        build_list(s, l);
+        return;
+    }
+    const int lane = threadIdx.x & 31, half = dim / 2, perHead = halfMode ? half / 8 : dim / 8;  // vectors, or pairs of vectors
+    const int items = (qHeads + kHeads) * perHead;
+    for (int row = (blockIdx.x - 1) * 8 + (threadIdx.x >> 5); row < s.total; row += (gridDim.x - 1) * 8) {
+        int s0, s1;
+        if (!seq_rows(s, seq_of(s, row), s0, s1) || row < s0 || row >= s1) continue;
+        const float* cr = cosT + (size_t)(row - s0) * half;
+        const float* sr = sinT + (size_t)(row - s0) * half;
+        for (int it = lane; it < items; it += 32) {
+            const int head = it / perHead, j = it - head * perHead;
+            const uint16_t* src = head < qHeads ? q + ((size_t)row * qHeads + head) * dim : k + ((size_t)row * kHeads + head - qHeads) * dim;
+            uint16_t* dst = head < qHeads ? qOut + ((size_t)row * qHeads + head) * dim : kOut + ((size_t)row * kHeads + head - qHeads) * dim;
+            if (halfMode) {
+                Vec16 a = ld_stream(src + 8 * j), b = ld_stream(src + half + 8 * j);
+                const float4 c0 = __ldg((const float4*)(cr + 8 * j)), c1 = __ldg((const float4*)(cr + 8 * j + 4));
+                const float4 n0 = __ldg((const float4*)(sr + 8 * j)), n1 = __ldg((const float4*)(sr + 8 * j + 4));
+                const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, sn[8] = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, n1.z, n1.w};
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    float e0, e1, o0, o1;
+                    unpack16_arith<DT>(a.w[w], e0, e1);
+                    unpack16_arith<DT>(b.w[w], o0, o1);
+                    a.w[w] = pack16_arith<DT>(sub(mul(e0, cs[2 * w]), mul(o0, sn[2 * w])), sub(mul(e1, cs[2 * w + 1]), mul(o1, sn[2 * w + 1])));
+                    b.w[w] = pack16_arith<DT>(add(mul(e0, sn[2 * w]), mul(o0, cs[2 * w])), add(mul(e1, sn[2 * w + 1]), mul(o1, cs[2 * w + 1])));
+                }
+                *(Vec16*)(dst + 8 * j) = a;
+                *(Vec16*)(dst + half + 8 * j) = b;
+            } else {
+                Vec16 a = ld_stream(src + 8 * j);
+                const float4 c = __ldg((const float4*)(cr + 4 * j)), n = __ldg((const float4*)(sr + 4 * j));
+                const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {n.x, n.y, n.z, n.w};
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    float e, o;
+                    unpack16_arith<DT>(a.w[w], e, o);
+                    a.w[w] = pack16_arith<DT>(sub(mul(e, cs[w]), mul(o, sn[w])), add(mul(e, sn[w]), mul(o, cs[w])));
+                }
+                *(Vec16*)(dst + 8 * j) = a;
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------
+// tensor-core kernel
+// ---------------------------------------------------------------------------------------------------------------------------------
+using namespace pf;
+
+constexpr int kThreads = 384;  // warps 0-3 / 4-7 softmax of tile 0 / 1, 8 MMA, 9 TMA loads, 10 output, 11 value tiles that not all rows see
+constexpr int kRows = 128;     // rows (head, position) of a tile
+constexpr int kKeys = 128;     // keys of a tile
+constexpr uint32_t kBlock = 128 * 128;  // bytes of 128 rows x 64 dimensions
+
+// NB: blocks of 64 dimensions
+template <int NB>
+struct Smem {
+    static constexpr int STAGES = NB == 2 ? 2 : 4;
+    static constexpr uint32_t TILE = NB * kBlock;
+    static constexpr uint32_t Q = 0, K = 2 * TILE, V = K + STAGES * TILE, STAGING = V + STAGES * TILE, BARS = STAGING + TILE, TOTAL = BARS + 512 + 1024;
+};
+
+struct TileParams {
+    CUtensorMap tmQ, tmK, tmV, tmO;
+    const Entry* entries;
+    const int* count;
+    const uint16_t* v;  // values, for the rows that see one that is not finite
+    uint16_t* out;
+    int* errorFlag;
+    int heads, kvHeads, dim, causal;
+    int packLog, headGroups;  // PACK = 1 << packLog heads per tile, heads / PACK tiles per block of positions
+    float scaleLog2;
+};
+
+// bounded wait for the count at `at`
+__device__ __forceinline__ bool turn_wait(uint32_t at, int need, volatile int* abortFlag) {
+    for (long long i = 0; i < kSpinLimit; i++) {
+        int now;
+        asm volatile("ld.acquire.cta.shared::cta.s32 %0, [%1];" : "=r"(now) : "r"(at) : "memory");
+        if (now >= need) return true;
+        if ((i & 1023) == 1023 && *abortFlag) return false;
+    }
+    return false;
+}
+
+template <int STAGES>
+struct Bar {
+    // VRAW: a value tile that not all rows see has landed (VFULL follows once it has been looked through)
+    enum : uint32_t { Q = 0, QREADY = 2, S = 4, P = 6, P2 = 8, O = 10, QFREE = 12, STAGED = 14, KFULL = 16, KEMPTY = KFULL + STAGES,
+                      VFULL = KEMPTY + STAGES, VEMPTY = VFULL + STAGES, VRAW = VEMPTY + STAGES, COUNT = VRAW + STAGES };
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int c0, int c1, int c2) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(dst), "l"(tm), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* tm, uint32_t src, int c0, int c1, int c2) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
+                 ::"l"(tm), "r"(src), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+
+// which halves of a word are not finite (their sign bits)
+template <bool BF16> __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    constexpr uint32_t E = BF16 ? 0x7F807F80u : 0x7C007C00u, ONE = BF16 ? 0x00800080u : 0x04000400u;
+    return ((w & E) + ONE) & 0x80008000u;
+}
+
+// Adds to 32 normalised outputs of a row what is not finite among the values it sees in keys [k0, k1): any weight leaves an infinity
+// or a NaN as it is.  Runs only where the value warp has met one.
+template <bool BF16>
+__device__ __noinline__ void add_not_finite(float* o, const uint16_t* v, size_t stride, int k0, int k1, int cols) {
+    for (int key = k0; key < k1; key++)
+        for (int i = 0; i < cols; i++) {
+            const uint32_t bits = v[(size_t)key * stride + i];
+            if (not_finite<BF16>(bits)) o[i] += widen16<BF16>(bits);
+        }
+}
+
+template <bool BF16, int NB>
+__global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constant__ TileParams p) {
+    using M = Smem<NB>;
+    using B = Bar<M::STAGES>;
+    constexpr uint32_t kColS = 0, kColO = 256;  // TMEM columns: S0 S1 (P over their first halves), O0 O1
+    extern __shared__ unsigned char smemRaw[];
+    unsigned char* smem = (unsigned char*)(((uintptr_t)smemRaw + 1023) & ~(uintptr_t)1023);  // swizzled boxes: 1024-byte aligned
+    const uint32_t sBase = smem_u32(smem);
+    auto bar = [&](uint32_t i) { return sBase + M::BARS + i * 8; };
+    __shared__ uint32_t tmemBaseShared;
+    __shared__ int abortShared;
+    __shared__ int turn;       // output tiles that have left the staging tile: item it's tile 0 is number 2 it, its tile 1 (or none) 2 it + 1
+    __shared__ int notFinite;  // set once a value that is not finite has been cleared anywhere in this CTA's work
+    volatile int* abortFlag = &abortShared;
+
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const int posTile = kRows >> p.packLog;  // positions of a tile
+    // A work item: one block of two tiles' positions of one sequence for PACK heads.  Dealt in serpentine order, heavy items first.
+    struct Item { int row0, len, pos, head, kvHead, nMax, nT0, nT1, firstPartial; };  // nT: key tiles of a tile; firstPartial: first key tile not seen by all rows
+    auto get_item = [&](int it, Item& w) -> bool {
+        asm volatile("" : "+r"(it));  // decoded anew by every role: kept values would cost the softmax threads registers
+        const int G = (int)gridDim.x;
+        const int idx = it * G + ((it & 1) ? G - 1 - (int)blockIdx.x : (int)blockIdx.x);
+        const int e = idx / p.headGroups;
+        if (e >= __ldg(p.count)) return false;
+        const int4 raw = __ldg((const int4*)(p.entries + e));
+        w.row0 = raw.x;
+        w.len = raw.y;
+        w.pos = raw.z;
+        w.head = (idx - e * p.headGroups) << p.packLog;
+        w.kvHead = w.head / (p.heads / p.kvHeads);
+        auto tiles_for = [&](int from) {
+            const int last = p.causal ? min(w.len, from + posTile) : w.len;
+            return from < w.len ? (last + kKeys - 1) / kKeys : 0;
+        };
+        w.nT0 = tiles_for(w.pos);
+        w.nT1 = tiles_for(w.pos + posTile);
+        w.nMax = max(w.nT0, w.nT1);
+        w.firstPartial = p.causal ? (w.pos + 1) / kKeys : w.len / kKeys;  // tile j is seen by all rows if its keys end at pos + 1 / at len or before
+        return true;
+    };
+
+    if (threadIdx.x == 0) {
+        abortShared = 0;
+        notFinite = 0;
+        turn = 0;
+        for (int t = 0; t < 2; t++) {
+            mbar_init(bar(B::Q + t), 1);
+            mbar_init(bar(B::QREADY + t), 128);
+            mbar_init(bar(B::S + t), 1);
+            mbar_init(bar(B::P + t), 128);
+            mbar_init(bar(B::P2 + t), 128);
+            mbar_init(bar(B::O + t), 1);
+            mbar_init(bar(B::QFREE + t), 1);
+            mbar_init(bar(B::STAGED + t), 128);
+        }
+        for (int s = 0; s < M::STAGES; s++) {
+            mbar_init(bar(B::KFULL + s), 1);
+            mbar_init(bar(B::KEMPTY + s), 1);
+            mbar_init(bar(B::VFULL + s), 1);
+            mbar_init(bar(B::VEMPTY + s), 1);
+            mbar_init(bar(B::VRAW + s), 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmemBaseShared)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, tmemBaseShared, 0);
+
+    // registers: 384 x 168 at launch; 256 x 200 + 128 x 96 afterwards
+    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    if (warp == 11) {
+        // ------------------------------------------------ value tiles that not all rows see ------------------------------------
+        uint32_t lc = 0;   // ring position of the item's first key tile
+        uint32_t raw = 0;  // per stage: parity of its VRAW phases
+        bool okay = true;
+        Item w = {};
+        for (int it = 0; okay && get_item(it, w); it++) {
+            for (int j = w.firstPartial; j < w.nMax && okay; j++) {
+                const uint32_t ring = lc + (uint32_t)j;
+                const int st = ring % M::STAGES;
+                okay = __all_sync(0xffffffffu, mbar_wait(bar(B::VRAW + st), (raw >> st) & 1, abortFlag));
+                if (!okay) break;
+                raw ^= 1u << st;
+                Vec16* tile = (Vec16*)(smem + M::V + st * M::TILE);
+                uint32_t found = 0;
+#pragma unroll 8
+                for (int i = lane; i < (int)(M::TILE / 16); i += 32) {
+                    const Vec16 x = tile[i];
+                    found |= not_finite<BF16>(x.w[0]) | not_finite<BF16>(x.w[1]) | not_finite<BF16>(x.w[2]) | not_finite<BF16>(x.w[3]);
+                }
+                if (__any_sync(0xffffffffu, found != 0)) {
+                    for (int i = lane; i < (int)(M::TILE / 16); i += 32) {
+                        Vec16 x = tile[i];
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            const uint32_t bad = not_finite<BF16>(x.w[c]);
+                            x.w[c] &= ~((bad >> 15) * 0xFFFFu);  // 0x8000 -> all ones of that half
+                        }
+                        tile[i] = x;
+                    }
+                    *(volatile int*)&notFinite = 1;
+                    __threadfence_block();
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(B::VFULL + st));
+            }
+            lc += (uint32_t)w.nMax;
+        }
+        if (!okay && lane == 0) *abortFlag = 1;
+    } else if (warp == 10) {
+        // ------------------------------------------------ output: tile 0, tile 1, next item ... ---------------------------------
+        uint32_t uc[2] = {};  // items each tile took part in so far
+        bool okay = true;
+        Item w = {};
+        for (int it = 0; okay && get_item(it, w); it++) {
+            for (int t = 0; t < 2; t++) {
+                if ((t == 0 ? w.nT0 : w.nT1) == 0) continue;
+                okay = __all_sync(0xffffffffu, mbar_wait(bar(B::STAGED + t), uc[t] & 1, abortFlag));  // every row staged
+                if (!okay) break;
+                uc[t]++;
+                const int pos = w.pos + t * posTile;
+                if (pos + posTile <= w.len) {
+                    if (lane == 0) {
+#pragma unroll
+                        for (int n = 0; n < NB; n++) tma_store_3d(&p.tmO, sBase + M::STAGING + n * kBlock, 64 * n, w.head, w.row0 + pos);
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // shared memory must outlive the read
+                    }
+                } else {
+                    // rows behind the sequence belong to the next one: the live rows one by one, 16-byte pieces across the lanes
+                    const int live = (w.len - pos) << p.packLog, perRow = p.dim / 8;
+                    for (int i = lane; i < live * perRow; i += 32) {
+                        const int row = i / perRow, c = i - row * perRow;
+                        const Vec16 x = *(const Vec16*)(smem + M::STAGING + (c >> 3) * kBlock + row * 128 + (((c & 7) ^ (row & 7)) * 16));
+                        const size_t at = ((size_t)(w.row0 + pos + (row >> p.packLog)) * p.heads + w.head + (row & ((1 << p.packLog) - 1))) * p.dim;
+                        *(Vec16*)(p.out + at + c * 8) = x;
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) asm volatile("st.release.cta.shared::cta.s32 [%0], %1;" ::"r"(smem_u32(&turn)), "r"(2 * it + (w.nT1 == 0 ? 2 : t + 1)) : "memory");
+            }
+        }
+        if (!okay && lane == 0) *abortFlag = 1;
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    } else if (warp == 9) {
+        // ------------------------------------------------ TMA loads --------------------------------------------------------------
+        if (lane == 0) {
+            uint32_t lc = 0;
+            uint32_t uc[2] = {};
+            bool okay = true;
+            Item w = {};
+            auto load_kv = [&](const CUtensorMap* tm, uint32_t at, uint32_t full, uint32_t empty, int j) {  // `full`, `empty`: barriers of stage 0
+                const uint32_t ring = lc + (uint32_t)j;
+                const int st = ring % M::STAGES;
+                if (ring >= M::STAGES && !mbar_wait(bar(empty + st), ((ring / M::STAGES) - 1) & 1, abortFlag)) return false;
+                mbar_expect_tx(bar(full + st), M::TILE);
+#pragma unroll
+                for (int n = 0; n < NB; n++) tma_load_3d(sBase + at + st * M::TILE + n * kBlock, tm, bar(full + st), 64 * n, w.kvHead, w.row0 + j * kKeys);
+                return true;
+            };
+            auto load_k = [&](int j) { return load_kv(&p.tmK, M::K, B::KFULL, B::KEMPTY, j); };
+            auto load_v = [&](int j) { return load_kv(&p.tmV, M::V, j >= w.firstPartial ? B::VRAW : B::VFULL, B::VEMPTY, j); };
+            auto load_q = [&](int t) {
+                if ((t == 0 ? w.nT0 : w.nT1) == 0) return true;
+                // the buffer is free once the last score product of the tile's previous item has run
+                if (uc[t] > 0 && !mbar_wait(bar(B::QFREE + t), (uc[t] - 1) & 1, abortFlag)) return false;
+                uc[t]++;
+                mbar_expect_tx(bar(B::Q + t), M::TILE);
+#pragma unroll
+                for (int n = 0; n < NB; n++)
+                    tma_load_3d(sBase + M::Q + t * M::TILE + n * kBlock, &p.tmQ, bar(B::Q + t), 64 * n, w.head, w.row0 + w.pos + t * posTile);
+                return true;
+            };
+            // one thread issues every load, in the order in which the buffers come free at the end of the item before
+            for (int it = 0; okay && get_item(it, w); it++) {
+                if (it == 0) okay = load_q(0) && load_k(0) && load_q(1) && load_v(0);
+                else okay = load_k(0) && load_q(0) && load_v(0) && load_q(1);
+                for (int j = 1; j < w.nMax && okay; j++) okay = load_k(j) && load_v(j);
+                lc += (uint32_t)w.nMax;
+            }
+            if (!okay) *abortFlag = 1;
+        }
+    } else if (warp == 8) {
+        // ------------------------------------------------ MMA issue: the turns of the equal-length kernel --------------------------
+        const bool leader = elect_one();
+        const uint32_t idescQK = make_idesc(BF16, false), idescPV = make_idesc(BF16, true, 64 * NB);
+        bool okay = true;
+        const uint64_t kmajorHi = make_desc(0, 16, 1024) >> 32, vHi = make_desc(0, kBlock, 1024) >> 32;
+        const uint32_t qLo = (uint32_t)make_desc(sBase + M::Q, 16, 1024), kLo = (uint32_t)make_desc(sBase + M::K, 16, 1024);
+        const uint32_t vLo = (uint32_t)make_desc(sBase + M::V, kBlock, 1024);
+        auto desc = [](uint64_t hi, uint32_t lo) { return (hi << 32) | (uint64_t)lo; };
+        uint32_t lc = 0;        // ring position of key tile 0 of the current item
+        uint32_t sc[2] = {}, uc[2] = {};  // key-tile steps / items each tile has run so far (parities of its barriers)
+        int nT[2] = {};
+        auto issue_qk = [&](int t, int j) {
+            const uint32_t kS = kLo + ((lc + (uint32_t)j) % M::STAGES) * (M::TILE >> 4);
+            const uint32_t qS = qLo + (uint32_t)t * (M::TILE >> 4);
+            const uint32_t dS = tmem + kColS + t * 128;
+#pragma unroll
+            for (int kk = 0; kk < 4 * NB; kk++) {
+                const uint32_t off = ((kk >> 2) * kBlock + (kk & 3) * 32) >> 4;
+                if (leader) mma_ss(dS, desc(kmajorHi, qS + off), desc(kmajorHi, kS + off), idescQK, kk > 0);
+            }
+            if (leader) {
+                mma_commit(bar(B::S + t));
+                if (j + 1 == nT[t]) mma_commit(bar(B::QFREE + t));  // the Q tile is no longer read
+                // last score product that reads this K stage (tile 1 while it is still running, else tile 0)
+                if (t == 1 || j >= nT[1]) mma_commit(bar(B::KEMPTY + (lc + (uint32_t)j) % M::STAGES));
+            }
+            __syncwarp();
+        };
+        auto issue_pv = [&](int t, int j) {
+            const uint32_t vS = vLo + ((lc + (uint32_t)j) % M::STAGES) * (M::TILE >> 4);
+            const uint32_t dO = tmem + kColO + t * 128, aP = tmem + kColS + t * 128;
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++)
+                if (leader) mma_ts(dO, aP + kk * 8, desc(vHi, vS + ((kk * 16 * 128) >> 4)), idescPV, j > 0 || kk > 0);
+            if (!mbar_wait(bar(B::P2 + t), (sc[t] + (uint32_t)j) & 1, abortFlag)) return false;  // second half of P (keys 64..127)
+            fence_after();
+#pragma unroll
+            for (int kk = 4; kk < 8; kk++)
+                if (leader) mma_ts(dO, aP + kk * 8, desc(vHi, vS + ((kk * 16 * 128) >> 4)), idescPV, 1);
+            __syncwarp();
+            return true;
+        };
+        Item w = {};
+        for (int it = 0; okay && get_item(it, w); it++) {
+            nT[0] = w.nT0;
+            nT[1] = w.nT1;
+            for (int t = 0; t < 2 && okay; t++) {
+                if (nT[t] == 0) continue;
+                okay = mbar_wait(bar(B::QREADY + t), uc[t] & 1, abortFlag);
+                if (okay) okay = mbar_wait(bar(B::KFULL + lc % M::STAGES), (lc / M::STAGES) & 1, abortFlag);
+                if (!okay) break;
+                fence_after();
+                issue_qk(t, 0);
+            }
+            for (int j = 0; j < w.nMax && okay; j++) {
+                const uint32_t ring = lc + (uint32_t)j;
+                const int st = ring % M::STAGES;
+                for (int t = 0; t < 2 && okay; t++) {
+                    if (j >= nT[t]) continue;
+                    if (t == 0 || j >= nT[0]) {  // (tile 1 finds the stages its neighbour has already waited for)
+                        okay = mbar_wait(bar(B::VFULL + st), (ring / M::STAGES) & 1, abortFlag);
+                        if (okay && j + 1 < w.nMax) okay = mbar_wait(bar(B::KFULL + (ring + 1) % M::STAGES), ((ring + 1) / M::STAGES) & 1, abortFlag);
+                    }
+                    if (okay) okay = mbar_wait(bar(B::P + t), (sc[t] + (uint32_t)j) & 1, abortFlag);
+                    if (!okay) break;
+                    fence_after();
+                    okay = issue_pv(t, j);
+                    if (!okay) break;
+                    if (j + 1 < nT[t]) issue_qk(t, j + 1);
+                    else if (leader) mma_commit(bar(B::O + t));
+                    // last product that reads this V stage (tile 1 while it is still running, else tile 0)
+                    if (leader && (t == 1 || j >= nT[1])) mma_commit(bar(B::VEMPTY + st));
+                    __syncwarp();
+                }
+            }
+            lc += (uint32_t)w.nMax;
+            for (int t = 0; t < 2; t++) {
+                sc[t] += (uint32_t)nT[t];
+                uc[t] += nT[t] > 0 ? 1u : 0u;
+            }
+        }
+        if (!okay) *abortFlag = 1;
+    } else {
+        // ------------------------------------------------ softmax / epilogue -------------------------------------------------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        const int t = warp >> 2;
+        const int row = threadIdx.x & 127;  // TMEM lane = row of the tile: head (row % PACK), position (row / PACK)
+        const uint32_t laneBase = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t colS = kColS + t * 128, colO = kColO + t * 128;
+        const float scale = p.scaleLog2;
+        bool okay = true;
+        uint32_t sc = 0, uc = 0;  // parities of the key-tile steps / items this group has run so far
+#pragma unroll 1
+        for (int it = 0; okay; it++) {
+            int n, pos, len, row0, kvHead, partial;
+            {
+                Item w;
+                if (!get_item(it, w)) break;
+                n = t == 0 ? w.nT0 : w.nT1;
+                pos = w.pos + t * posTile;
+                len = w.len;
+                row0 = w.row0;
+                kvHead = w.kvHead;
+                partial = w.firstPartial;
+            }
+            if (n == 0) continue;
+            const int seen = p.causal ? min(pos + (row >> p.packLog) + 1, len) : len;  // keys this row sees
+            okay = __all_sync(0xffffffffu, mbar_wait(bar(B::Q + t), uc & 1, abortFlag));
+            mbar_arrive(bar(B::QREADY + t));
+            float mUsed = -INFINITY;  // the maximum the stored P and O are relative to (scaled, log2 domain)
+            float lsum = 0.f;
+            for (int j = 0; j < n && okay; j++) {
+                okay = __all_sync(0xffffffffu, mbar_wait(bar(B::S + t), (sc ^ (uint32_t)j) & 1, abortFlag));
+                if (!okay) break;
+                fence_after();
+                uint32_t sreg[128];
+#pragma unroll
+                for (int c = 0; c < 4; c++) tmem_ld32(laneBase + colS + c * 32, sreg + c * 32);
+                tmem_wait_ld();
+                if (j >= partial) {
+                    const int left = seen - j * kKeys;  // keys of this tile that the row sees
+#pragma unroll
+                    for (int i = 0; i < 128; i++)
+                        if (i >= left) sreg[i] = 0xFF800000u;  // -inf
+                }
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < 128; i += 8) {
+#pragma unroll
+                    for (int u = 0; u < 4; u++) mx4[u] = fmax3(mx4[u], __uint_as_float(sreg[i + 2 * u]), __uint_as_float(sreg[i + 2 * u + 1]));
+                }
+                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale;  // scale > 0
+                // keep the old reference maximum unless the row maximum grew by more than 8 (a factor 256)
+                const bool first = mUsed == -INFINITY;
+                const bool grow = first ? (mx > -INFINITY) : (mx > mUsed + 8.0f);
+                const float mNew = grow ? mx : mUsed;
+                const float alpha = (grow && !first) ? ex2_approx(mUsed - mNew) : 1.0f;
+                if (j > 0 && __any_sync(0xffffffffu, grow && !first)) {
+#pragma unroll 1
+                    for (int c = 0; c < 2 * NB; c++) {
+                        uint32_t oreg[32];
+                        tmem_ld32(laneBase + colO + c * 32, oreg);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) oreg[i] = __float_as_uint(__uint_as_float(oreg[i]) * alpha);
+                        tmem_st32(laneBase + colO + c * 32, oreg);
+                    }
+                }
+                lsum *= alpha;
+                mUsed = mNew;
+                const float negM = first && !grow ? 0.f : -mUsed;  // no score above -inf so far: every exponential is 0
+                const uint64_t SC = pk2(scale, scale), NM = pk2(negM, negM);
+                uint64_t sumA = pk2(0.f, 0.f), sumB = pk2(0.f, 0.f);
+#pragma unroll
+                for (int i = 0; i < 64; i += 2) {
+                    const uint64_t X01 = fma2(pk2(__uint_as_float(sreg[2 * i]), __uint_as_float(sreg[2 * i + 1])), SC, NM);
+                    const uint64_t X23 = fma2(pk2(__uint_as_float(sreg[2 * i + 2]), __uint_as_float(sreg[2 * i + 3])), SC, NM);
+                    float x0, x1, x2, x3;
+                    un2(X01, x0, x1);
+                    un2(X23, x2, x3);
+                    const uint64_t E01 = pk2(ex2_approx(x0), ex2_approx(x1)), E23 = pk2(ex2_approx(x2), ex2_approx(x3));
+                    sumA = add2(sumA, E01);
+                    sumB = add2(sumB, E23);
+                    float e0, e1, e2, e3;
+                    un2(E01, e0, e1);
+                    un2(E23, e2, e3);
+                    sreg[i] = pack2<BF16>(e0, e1);
+                    sreg[i + 1] = pack2<BF16>(e2, e3);
+                    if (i == 30) {
+                        tmem_st32(laneBase + colS, sreg);
+                        tmem_wait_st();
+                        fence_before();
+                        mbar_arrive(bar(B::P + t));
+                    }
+                }
+                tmem_st32(laneBase + colS + 32, sreg + 32);
+                tmem_wait_st();
+                fence_before();
+                mbar_arrive(bar(B::P2 + t));
+                float a0, a1, b0, b1;
+                un2(sumA, a0, a1);
+                un2(sumB, b0, b1);
+                lsum += (a0 + a1) + (b0 + b1);
+            }
+            // wait for the last P V product, normalise, stage in the swizzled box layout.  The staging tile is shared by the groups in turn
+            // (tile 0, tile 1, tile 0 of the next item, ...).  A count, not a barrier's parity: a group that had no tile in some items may
+            // be several turns ahead.
+            if (okay) okay = __all_sync(0xffffffffu, mbar_wait(bar(B::O + t), uc & 1, abortFlag));
+            if (okay) okay = __all_sync(0xffffffffu, turn_wait(smem_u32(&turn), 2 * it + t, abortFlag));
+            if (okay) {
+                fence_after();
+                const float inv = 1.0f / lsum;
+                unsigned char* stage = smem + M::STAGING + row * 128;
+#pragma unroll 1
+                for (int c = 0; c < 2 * NB; c++) {
+                    uint32_t oreg[32];
+                    tmem_ld32(laneBase + colO + c * 32, oreg);
+                    tmem_wait_ld();
+                    float o[32];
+#pragma unroll
+                    for (int i = 0; i < 32; i++) o[i] = __uint_as_float(oreg[i]) * inv;
+                    if (*(volatile int*)&notFinite && c * 32 < p.dim) {
+                        float x[32];  // (memory of its own: o stays in registers)
+#pragma unroll
+                        for (int i = 0; i < 32; i++) x[i] = o[i];
+                        add_not_finite<BF16>(x, p.v + ((size_t)row0 * p.kvHeads + kvHead) * p.dim + c * 32, (size_t)p.kvHeads * p.dim, partial * kKeys, seen,
+                                             min(32, p.dim - c * 32));
+#pragma unroll
+                        for (int i = 0; i < 32; i++) o[i] = x[i];
+                    }
+#pragma unroll
+                    for (int v4 = 0; v4 < 4; v4++) {
+                        Vec16 x;
+#pragma unroll
+                        for (int w = 0; w < 4; w++) x.w[w] = pack2<BF16>(o[v4 * 8 + 2 * w], o[v4 * 8 + 2 * w + 1]);
+                        const int chunk = c * 4 + v4;  // 16-byte chunk of the row
+                        *(Vec16*)(stage + (chunk >> 3) * kBlock + (((chunk & 7) ^ (row & 7)) * 16)) = x;
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(bar(B::STAGED + t));
+            } else {
+                *abortFlag = 1;
+            }
+            sc ^= (uint32_t)n;
+            uc ^= 1u;
+        }
+    }
+    // ---------------------------------------------------- teardown ----------------------------------------------------
+    fence_before();
+    __syncthreads();
+    if (abortShared && threadIdx.x == 0) atomicExch(p.errorFlag, 2);
+    if (warp == 8) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// [total, heads, dim] 16-bit -> 3-D map (dim, head, row) with a box of 64 x boxHeads x boxRows and 128-byte swizzle
+static bool make_map(CUtensorMap* tm, const void* base, bool bf16, uint32_t total, uint32_t heads, uint32_t dim, uint32_t boxHeads, uint32_t boxRows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[3] = {dim, heads, total};
+    cuuint64_t strides[2] = {(cuuint64_t)dim * 2, (cuuint64_t)heads * dim * 2};
+    cuuint32_t box[3] = {64, boxHeads, boxRows};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return fn(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, (void*)base, dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct Call {
+    int dt;
+    const void *q, *k, *v;
+    void* out;
+    Seqs seqs;
+    uint32_t heads, kvHeads, dim, causal, ropeMode;
+    const float *cosT, *sinT;
+};
+
+// the tensor-core path; false where it does not take the shape
+static bool tiles_take(const Call& c) {
+    if (c.dt != DT_BF16 && c.dt != DT_F16) return false;
+    if (c.dim > 128 || c.dim % 8 != 0) return false;                       // TMA: rows and row pitches of 16-byte multiples
+    if (c.ropeMode != 2 && c.dim % 16 != 0) return false;                  // the rotation's vectors
+    const uintptr_t all = (uintptr_t)c.q | (uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.out;
+    return (all & 15u) == 0 && encode_fn() != nullptr;
+}
+
+template <bool BF16>
+static int tiles_launch(Context* ctx, const Call& c, CUDAStatus* status) {
+    constexpr int DT = BF16 ? DT_BF16 : DT_F16;
+    const uint32_t group = c.heads / c.kvHeads;
+    int packLog = 0;
+    while (packLog < 7 && group % (2u << packLog) == 0) packLog++;
+    const int span = 2 * (kRows >> packLog);
+    const uint32_t total = (uint32_t)c.seqs.total;
+    const size_t levels = ((size_t)c.seqs.maxLen + span - 1) / span, most = (size_t)total / span + c.seqs.batch;  // entries at most
+    const size_t qBytes = c.ropeMode != 2 ? (((size_t)total * c.heads * c.dim * 2) + 255) & ~(size_t)255 : 0;
+    const size_t kBytes = c.ropeMode != 2 ? (((size_t)total * c.kvHeads * c.dim * 2) + 255) & ~(size_t)255 : 0;
+    if (most * c.heads > 0x3FFFFFFFull) return fail(status, -2, "packed prefill attention: %zu blocks of %u heads exceed the index range", most, c.heads);
+    const size_t entryBytes = (most * sizeof(Entry) + 255) & ~(size_t)255;
+    Scratch ws;
+    int rc = call_scratch(ctx, qBytes + kBytes + entryBytes + 256 + 2 * levels * 4, 0, &ws, status);
+    if (rc != 0) return rc;
+    uint16_t* qRot = (uint16_t*)ws.base;
+    uint16_t* kRot = (uint16_t*)(ws.base + qBytes);
+    Lists l;
+    l.entries = (Entry*)(ws.base + qBytes + kBytes);
+    l.count = (int*)(ws.base + qBytes + kBytes + entryBytes);
+    l.above = l.count + 64;
+    l.cursor = l.above + levels;
+    l.span = span;
+    l.levels = (int)levels;
+    l.capacity = (int)most;
+    unsigned blocks = 1;
+    if (c.ropeMode != 2) {
+        const size_t want = ((size_t)total + 7) / 8, cap = (size_t)ctx->smCount * 8;
+        blocks += (unsigned)(want < cap ? want : cap);
+    }
+    prologue_kernel<DT><<<blocks, 256, 0, ctx->stream>>>((const uint16_t*)c.q, (const uint16_t*)c.k, qRot, kRot, c.seqs, l, c.cosT, c.sinT, (int)c.heads,
+                                                         (int)c.kvHeads, (int)c.dim, c.ropeMode == 1);
+    rc = check_launch(ctx, status, "packed prefill attention: work list and RoPE");
+    if (rc != 0) return rc;
+    TileParams p;
+    memset(&p, 0, sizeof(p));
+    const void* q = c.ropeMode != 2 ? qRot : c.q;
+    const void* k = c.ropeMode != 2 ? kRot : c.k;
+    const uint32_t pack = 1u << packLog;
+    if (!make_map(&p.tmQ, q, BF16, total, c.heads, c.dim, pack, kRows >> packLog) || !make_map(&p.tmK, k, BF16, total, c.kvHeads, c.dim, 1, kKeys) ||
+        !make_map(&p.tmV, c.v, BF16, total, c.kvHeads, c.dim, 1, kKeys) || !make_map(&p.tmO, c.out, BF16, total, c.heads, c.dim, pack, kRows >> packLog))
+        return fail(status, -7, "packed prefill attention: tensor map encoding failed");
+    p.entries = l.entries;
+    p.count = l.count;
+    p.v = (const uint16_t*)c.v;
+    p.out = (uint16_t*)c.out;
+    p.errorFlag = ctx->errorFlag;
+    p.heads = (int)c.heads; p.kvHeads = (int)c.kvHeads; p.dim = (int)c.dim; p.causal = (int)c.causal;
+    p.packLog = packLog;
+    p.headGroups = (int)(c.heads >> packLog);
+    p.scaleLog2 = (float)(1.4426950408889634 / sqrt((double)c.dim));
+    const size_t items = most * p.headGroups;
+    const unsigned grid = items < (size_t)ctx->smCount ? (unsigned)items : (unsigned)ctx->smCount;  // persistent: one CTA per SM
+#define TILES(NB)                                                                                                                      \
+    do {                                                                                                                               \
+        cudaFuncSetAttribute(tiles_kernel<BF16, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Smem<NB>::TOTAL);               \
+        tiles_kernel<BF16, NB><<<grid, kThreads, Smem<NB>::TOTAL, ctx->stream>>>(p);                                                   \
+    } while (0)
+    if (c.dim > 64) TILES(2);
+    else TILES(1);
+#undef TILES
+    return check_launch(ctx, status, "packed prefill attention");
+}
+
 }  // namespace pk
 
 }  // namespace puter
@@ -154,16 +883,21 @@ extern "C" int cuda_dispatch_rope_packed_attention_prefill(CUDADeviceRef context
     void* out = dev_ptr(outRef);
     if (out == q || out == k || out == v) return fail(status, -2, "%s: out may not be an input", what);
     const pk::Seqs seqs{(const int32_t*)dev_ptr(seqStartsRef), (int)batch, (int)totalTokens, (int)maxSeqLen, ctx->errorFlag};
-    const int cap = ctx->smCount * 8;
+    const float *table = nullptr, *sinT = nullptr;
     if (ropeMode != 2) {
-        const float* table = cached_rope_table(ctx, maxSeqLen, (int)headDim, baseFreq, (long long)startPosition, (int)scaling, scalingFactor,
+        table = cached_rope_table(ctx, maxSeqLen, (int)headDim, baseFreq, (long long)startPosition, (int)scaling, scalingFactor,
                                                lowFreqFactor, highFreqFactor, (int)originalContext, status);
         if (!table) return status ? status->code : -7;
+        sinT = table + (size_t)maxSeqLen * (headDim / 2);
+    }
+    const pk::Call c{elementDType, q, k, v, out, seqs, numHeads, kvHeads, headDim, causal ? 1u : 0u, ropeMode, table, sinT};
+    if (pk::tiles_take(c)) return elementDType == DT_BF16 ? pk::tiles_launch<true>(ctx, c, status) : pk::tiles_launch<false>(ctx, c, status);
+    const int cap = ctx->smCount * 8;
+    if (ropeMode != 2) {
         const size_t qAt = 0, kAt = (qBytes + 255) & ~(size_t)255;
         Scratch ws;
         int rc = call_scratch(ctx, kAt + kvBytes, 0, &ws, status);
         if (rc != 0) return rc;
-        const float* sinT = table + (size_t)maxSeqLen * (headDim / 2);
 #define ROTATE(DT, IN, AT, HEADS) \
     pk::rotate_kernel<DT><<<cap, 256, 0, ctx->stream>>>(IN, ws.base + AT, seqs, table, sinT, (int)(HEADS), (int)headDim, (int)ropeMode)
 #define ROTATE_BOTH(DT)                                                   \
