@@ -24,8 +24,10 @@
 //     the four unused columns take the lower bytes of the queries' integers, so that a lane has whole scores of one head.  The integers
 //     hold a query to 2^-16 of its largest element.  More heads take the f16 form: queries as f16, scaled by a power of two per
 //     (sequence, head) so that a bf16 query of any size fits.
-//   * The weights p_t * step_t enter as f16 (half a step of 2^-11, an eighth of what the 16-bit output keeps), relative to a running power of
-//     two about the largest step, which joins the running maximum of the softmax in rescaling the accumulator.
+//   * The weights p_t * step_t enter as f16, relative to a running power of two about the largest step, which joins the running maximum of
+//     the softmax in rescaling the accumulator.  Their rounding (half a step of 2^-11) multiplies codes of 0 .. 15, more than the
+//     values themselves amount to: 2^-10 of the output, measured, unseen in a bf16 output and five times the rounding of an f16 one.  For
+//     f16 the weights therefore come in two parts, the second in the unused columns (QUAD, free) or in products of its own.
 // Sums, maxima and accumulators are float32.
 //
 // Work: the tiles of 16 tokens of all (KV head, sequence) pairs in one list, cut into equal contiguous ranges, one per CTA, and each
@@ -225,6 +227,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
     constexpr int WV = D / 64;   // words of a token's V codes in a lane
     constexpr int ROW = S::ROW;
     constexpr bool QUAD = S::QUAD;
+    constexpr bool SPLIT = DT == DT_F16;  // weights in two parts
     constexpr int J = QUAD ? 1 : 2;  // heads of a lane: t, or 8nt + 2t and 8nt + 2t + 1
     constexpr int kPart = S::HEADS * D * 4 + S::HEADS * 8;  // a partial in shared memory: accumulators, then (maximum, sum)
     static_assert(kPart <= S::STAGES * S::STAGE, "a warp's partial takes the place of its stages");
@@ -491,7 +494,8 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
             }
 
             // O^T in units of 2^-24 2^ve: word w, pair i: [0], [1] = dim base + 8w + 2i of heads 2t, 2t + 1; [2], [3] = that dim plus 16
-            // times the one behind it; base = g * D / 8.  QUAD: [0], [2] of head t ([1], [3] stay zero)
+            // times the one behind it; base = g * D / 8.  QUAD: [0], [2] of head t ([1], [3]: its weights'
+            // second part, or zero)
             float o[WV][4][NT][4];
             float m[NT][J], l[NT][J], z[NT][J];
 #pragma unroll
@@ -689,7 +693,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
                             for (int i = 0; i < 4; i++) {
                                 o[w][i][nt][0] *= alpha[0];
                                 o[w][i][nt][2] *= alpha[0];
-                                if (!QUAD) {
+                                if (!QUAD || SPLIT) {
                                     o[w][i][nt][1] *= alpha[J - 1];
                                     o[w][i][nt][3] *= alpha[J - 1];
                                 }
@@ -714,11 +718,20 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
                 // ---- O^T += V^T P^T ----
 #pragma unroll
                 for (int mt = 0; mt < MT; mt++) {
-                    uint32_t pb[NT][2];
+                    uint32_t pb[NT][2], pr[NT][2];
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        pb[nt][0] = transpose8(pack16_arith<DT_F16>(se[mt][nt][0], QUAD ? 0.f : se[mt][nt][1]));
-                        pb[nt][1] = transpose8(pack16_arith<DT_F16>(se[mt][nt][2], QUAD ? 0.f : se[mt][nt][3]));
+                        float rest[4] = {0.f, 0.f, 0.f, 0.f};  // what the f16 weights leave
+                        if (SPLIT) {
+#pragma unroll
+                            for (int i = 0; i < 4; i += QUAD ? 2 : 1) rest[i] = se[mt][nt][i] - __half2float(__float2half_rn(se[mt][nt][i]));
+                        }
+                        pb[nt][0] = transpose8(pack16_arith<DT_F16>(se[mt][nt][0], QUAD ? rest[0] : se[mt][nt][1]));
+                        pb[nt][1] = transpose8(pack16_arith<DT_F16>(se[mt][nt][2], QUAD ? rest[2] : se[mt][nt][3]));
+                        if (SPLIT && !QUAD) {
+                            pr[nt][0] = transpose8(pack16_arith<DT_F16>(rest[0], rest[1]));
+                            pr[nt][1] = transpose8(pack16_arith<DT_F16>(rest[2], rest[3]));
+                        }
                     }
                     const uint32_t at = st + kStep * ROW + mt * 16 * ROW;
                     uint32_t va[2], vb[2], vc[2], vd[2];  // tokens of rows 2t, 2t + 1, 2t + 8, 2t + 9
@@ -737,6 +750,10 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
                             for (int nt = 0; nt < NT; nt++) {
                                 mma(o[w][2 * half][nt], x & 0x000F000Fu, x & 0x00FF00FFu, y & 0x000F000Fu, y & 0x00FF00FFu, pb[nt][0], pb[nt][1]);
                                 mma(o[w][2 * half + 1][nt], x8 & 0x000F000Fu, x8, y8 & 0x000F000Fu, y8, pb[nt][0], pb[nt][1]);
+                                if (SPLIT && !QUAD) {
+                                    mma(o[w][2 * half][nt], x & 0x000F000Fu, x & 0x00FF00FFu, y & 0x000F000Fu, y & 0x00FF00FFu, pr[nt][0], pr[nt][1]);
+                                    mma(o[w][2 * half + 1][nt], x8 & 0x000F000Fu, x8, y8 & 0x000F000Fu, y8, pr[nt][0], pr[nt][1]);
+                                }
                             }
                         }
                     }
@@ -770,8 +787,13 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
                     for (int w = 0; w < WV; w++)
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            x[8 * w + 2 * i] = fmaf(o[w][i][nt][j] * 16777216.f, veUp, least);
-                            x[8 * w + 2 * i + 1] = fmaf((o[w][i][nt][2 + j] - o[w][i][nt][j]) * 1048576.f, veUp, least);
+                            float even = o[w][i][nt][j], both = o[w][i][nt][2 + j];
+                            if (QUAD && SPLIT) {
+                                even += o[w][i][nt][1];
+                                both += o[w][i][nt][3];
+                            }
+                            x[8 * w + 2 * i] = fmaf(even * 16777216.f, veUp, least);
+                            x[8 * w + 2 * i + 1] = fmaf((both - even) * 1048576.f, veUp, least);
                         }
                     if (whole) {
                         uint16_t* dst = p.out + ((size_t)b * p.numHeads + head0 + h) * D + g * (D / 8);

@@ -2,7 +2,7 @@
 //
 // A vector x of one (token, KV head) is held as 16 levels between its own extremes (no counterpart in the reference, whose cache is
 // kept in the tensors' type):
-//     least = rn16(min x),  step = rn16((max x - min x) / 15),  code_d = clamp(rint((x_d - least) / step), 0, 15),
+//     least = rn16(min x),  step = rn16((max x - min x) * (1 / 15)),  code_d = clamp(rint((x_d - least) / step), 0, 15),
 //     value_d = least + step * code_d,
 // rn16 = rounding to the 16-bit type of the tensors (their range: a bf16 vector may hold 1e30).  The codes are chosen against the
 // rounded step and least, so that rounding costs no accuracy but the cover of the extremes (at most 15 / 512 of a step in bf16).
@@ -12,8 +12,8 @@
 // [page, kvHead, token, 2] = (step, least).  The head comes before the token so that the 16 tokens that a warp of the decode kernel
 // takes of its head are one run of 16 * D / 2 bytes (and 64 of parameters) instead of 16 pieces.
 //
-// Both kernels stream: a group of D / 8 lanes holds a vector, eight elements a lane, so the extremes of a vector cost log2(D / 8)
-// shuffles and nothing goes through shared memory.
+// Both kernels stream: a group of D / 16 lanes holds a vector, sixteen elements a lane, so the extremes of a vector cost log2(D / 16)
+// shuffles per bound and nothing goes through shared memory.  What bounds them and what was done about it is said at each.
 #include <math.h>
 
 #include "common.cuh"
@@ -47,13 +47,33 @@ __device__ __forceinline__ uint32_t level(float t, float s, float inv) {
     return (uint32_t)__float2int_rn(fminf(fmaxf(y, 0.f), 15.f));
 }
 
-// The eight elements of this lane, one vector per group of LANES lanes: packed codes (element i in bits 4i .. 4i + 3); params = step
-// in the low, least in the high half.
-template <int DT, int LANES>
-__device__ __forceinline__ uint32_t quantise(const float* x, uint32_t& params) {
-    float lo = x[0], hi = x[0];
+// Eight levels, packed: element i in bits 4i .. 4i + 3.  Where no clamp can act (see quantise) the quotient is a product with the
+// reciprocal and one correction, which makes quotients that are ties exact; adding 1.5 * 2^23 rounds to nearest even and leaves the
+// level in the lowest bits, and since shifting and adding is linear the constant above them comes off once at the end.
+__device__ __forceinline__ uint32_t levels8(const float* x, float step, float least, float inv) {
+    constexpr float kMagic = 12582912.f;  // 0x4B400000
+    const uint64_t S = pk2(-step, -step), L = pk2(-least, -least), I = pk2(inv, inv), MAGIC = pk2(kMagic, kMagic);
+    float y[8];
 #pragma unroll
-    for (int i = 1; i < 8; i++) {
+    for (int i = 0; i < 8; i += 2) {
+        const uint64_t t = add2(pk2(x[i], x[i + 1]), L), q0 = mul2(t, I);
+        const uint64_t q1 = fma2(fma2(q0, S, t), I, q0);
+        un2(add2(q1, MAGIC), y[i], y[i + 1]);
+    }
+    uint32_t codes = __float_as_uint(y[7]);
+#pragma unroll
+    for (int i = 6; i >= 0; i--) codes = codes * 16u + __float_as_uint(y[i]);
+    constexpr uint32_t kTop = 0x4B400000u * 0x11111111u;  // the constant in all eight places
+    return codes - kTop;
+}
+
+// The sixteen elements of this lane, one vector per group of LANES lanes: packed codes of elements 0 - 7 and 8 - 15; params = step in the
+// low, least in the high half.
+template <int DT, int LANES>
+__device__ __forceinline__ void quantise(const float* x, uint32_t& c0, uint32_t& c1, uint32_t& params) {
+    float lo = min_nan(x[0], x[1]), hi = max_nan(x[0], x[1]);
+#pragma unroll
+    for (int i = 2; i < 16; i++) {
         lo = min_nan(lo, x[i]);
         hi = max_nan(hi, x[i]);
     }
@@ -62,13 +82,23 @@ __device__ __forceinline__ uint32_t quantise(const float* x, uint32_t& params) {
         lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
-    float step = __fdiv_rn(__fsub_rn(hi, lo), 15.f), least = lo;
+    float step = __fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f), least = lo;
     params = round_pair_arith<DT>(step, least);
     const float inv = 1.0f / step;
-    uint32_t codes = 0;
+    // no element falls below level -0.2 or above 15.25 while the rounding of least (2^-9 of it at most) stays below 0.2 of a step and the
+    // step is a normal number of its type: then rounding alone keeps 0 .. 15
+    const bool plain = fabsf(least) <= 100.f * step && step >= (DT == DT_F16 ? 6.103515625e-5f : 1e-30f) && step < INFINITY;
+    if (__all_sync(0xffffffffu, plain)) {
+        c0 = levels8(x, step, least, inv);
+        c1 = levels8(x + 8, step, least, inv);
+    } else {
+        c0 = c1 = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) codes |= level(__fsub_rn(x[i], least), step, inv) << (4 * i);
-    return codes;
+        for (int i = 0; i < 8; i++) {
+            c0 |= level(__fsub_rn(x[i], least), step, inv) << (4 * i);
+            c1 |= level(__fsub_rn(x[i + 8], least), step, inv) << (4 * i);
+        }
+    }
 }
 
 template <int DT> __device__ __forceinline__ void widen8(const Vec16& v, float* x) {
@@ -76,73 +106,64 @@ template <int DT> __device__ __forceinline__ void widen8(const Vec16& v, float* 
     for (int i = 0; i < 4; i++) unpack16_arith<DT>(v.w[i], x[2 * i], x[2 * i + 1]);
 }
 
-// MODE 0: neighbouring pairs, 1: halves, 2: K comes rotated
+// MODE 0: neighbouring pairs, 1: halves, 2: K comes rotated.
+// Bound: instructions, ~10 per element against the 14 that the memory system leaves time for; every lane has 64 bytes of K and V in flight before it
+// looks at its indices.  (APPEND_FIGURES)
 template <int DT, int D, int MODE>
 __global__ void __launch_bounds__(256) append_kernel(const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
                                                      const int32_t* __restrict__ positions, const int32_t* __restrict__ pageIDs,
                                                      const int32_t* __restrict__ offsets, uint8_t* __restrict__ kCodes,
                                                      uint32_t* __restrict__ kParams, uint8_t* __restrict__ vCodes,
                                                      uint32_t* __restrict__ vParams, const float* __restrict__ cosT,
-                                                     const float* __restrict__ sinT, uint32_t rows, uint32_t kvHeads, uint32_t pageCount,
+                                                     const float* __restrict__ sinT, uint32_t vectors, uint32_t kvHeads, uint32_t pageCount,
                                                      uint32_t pageSize, uint32_t maxPositions, int* __restrict__ errorFlag) {
-    constexpr int LANES = D / 8, HEADS = 32 / LANES;  // lanes per vector, heads per pass of a warp
+    constexpr uint32_t LANES = D / 16, PER = 32 / LANES;  // lanes per vector, vectors of a warp
     const uint32_t lane = threadIdx.x & 31, j = lane % LANES;
-    const uint32_t passes = (kvHeads + HEADS - 1) / HEADS;
-    const size_t units = (size_t)rows * passes, warps = (size_t)gridDim.x * (blockDim.x >> 5);
-    for (size_t u = (size_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); u < units; u += warps) {
-        const size_t row = u / passes;
-        const uint32_t pass = (uint32_t)(u - row * passes), head = pass * HEADS + lane / LANES;
-        const bool live = head < kvHeads;
-        const size_t src = (row * kvHeads + (live ? head : 0)) * D;
+    const size_t stride = (size_t)gridDim.x * (blockDim.x >> 5) * PER;
+    for (size_t first = ((size_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * PER; first < vectors; first += stride) {
+        const bool have = first + lane / LANES < vectors;
+        const uint32_t vec = have ? (uint32_t)first + lane / LANES : vectors - 1;
+        const uint32_t row = vec / kvHeads, head = vec - row * kvHeads;
+        const size_t src = (size_t)vec * D;
+        const uint32_t at0 = MODE == 1 ? 8 * j : 16 * j, at1 = MODE == 1 ? D / 2 + 8 * j : 16 * j + 8;
+        const Vec16 k0 = ld_stream(k + src + at0), k1 = ld_stream(k + src + at1);
+        const Vec16 v0 = ld_stream(v + src + 16 * j), v1 = ld_stream(v + src + 16 * j + 8);
         const int page = pageIDs[row], off = offsets[row], pos = MODE == 2 ? 0 : positions[row];
-        // (fetched before the indices are looked at: they are one more round trip away)
-        uint2 ka, kb;
-        if (MODE == 1) {
-            ka = __ldcs((const uint2*)(k + src + 4 * j));
-            kb = __ldcs((const uint2*)(k + src + D / 2 + 4 * j));
-        } else {
-            const Vec16 t = ld_stream(k + src + 8 * j);
-            ka = make_uint2(t.w[0], t.w[1]);
-            kb = make_uint2(t.w[2], t.w[3]);
-        }
-        const Vec16 vr = ld_stream(v + src + 8 * j);
-        if (page < 0 || (uint32_t)page >= pageCount || off < 0 || (uint32_t)off >= pageSize ||
-            (MODE != 2 && (pos < 0 || (uint32_t)pos >= maxPositions))) {
-            if (lane == 0) atomicExch(errorFlag, 1);
-            continue;
-        }
-        float x[8], y[8];
-        unpack16_arith<DT>(ka.x, x[0], x[1]);
-        unpack16_arith<DT>(ka.y, x[2], x[3]);
-        unpack16_arith<DT>(kb.x, x[4], x[5]);
-        unpack16_arith<DT>(kb.y, x[6], x[7]);
+        const bool good = page >= 0 && (uint32_t)page < pageCount && off >= 0 && (uint32_t)off < pageSize && pos >= 0 &&
+                          (MODE == 2 || (uint32_t)pos < maxPositions);
+        if (!good) atomicExch(errorFlag, 1);
+        float x[16], y[16];
+        widen8<DT>(k0, x);
+        widen8<DT>(k1, x + 8);
         if (MODE != 2) {
-            const float4 c = __ldg((const float4*)(cosT + (size_t)pos * (D / 2) + 4 * j));
-            const float4 s = __ldg((const float4*)(sinT + (size_t)pos * (D / 2) + 4 * j));
-            const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
+            const size_t turn = (size_t)(good ? pos : 0) * (D / 2) + 8 * j;
+            float cs[8], sn[8];
+            *(float4*)cs = __ldg((const float4*)(cosT + turn));
+            *(float4*)(cs + 4) = __ldg((const float4*)(cosT + turn + 4));
+            *(float4*)sn = __ldg((const float4*)(sinT + turn));
+            *(float4*)(sn + 4) = __ldg((const float4*)(sinT + turn + 4));
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int a = MODE == 1 ? i : 2 * i, b = MODE == 1 ? i + 4 : 2 * i + 1;
+            for (int i = 0; i < 8; i++) {
+                const int a = MODE == 1 ? i : 2 * i, b = MODE == 1 ? i + 8 : 2 * i + 1;
                 const float e = x[a], o = x[b];
                 x[a] = sub(mul(e, cs[i]), mul(o, sn[i]));
                 x[b] = add(mul(e, sn[i]), mul(o, cs[i]));
             }
         }
-        uint32_t kp, vp;
-        const uint32_t kc = quantise<DT, LANES>(x, kp);
-        widen8<DT>(vr, y);
-        const uint32_t vc = quantise<DT, LANES>(y, vp);
-        // halves: this lane holds two bytes of either half; neighbours trade so that each stores one word
-        uint32_t kw = kc, kAt = 4 * j;
-        if (MODE == 1) {
-            const uint32_t got = __shfl_xor_sync(0xffffffffu, (j & 1) ? (kc & 0xFFFFu) : (kc >> 16), 1);
-            kw = (j & 1) ? (got | (kc & 0xFFFF0000u)) : ((kc & 0xFFFFu) | (got << 16));
-            kAt = (j & 1) ? D / 4 + 2 * (j - 1) : 2 * j;
-        }
-        if (live) {
+        uint32_t kc0, kc1, kp, vc0, vc1, vp;
+        quantise<DT, (int)LANES>(x, kc0, kc1, kp);
+        widen8<DT>(v0, y);
+        widen8<DT>(v1, y + 8);
+        quantise<DT, (int)LANES>(y, vc0, vc1, vp);
+        if (have && good) {
             const size_t slot = ((size_t)page * kvHeads + head) * pageSize + (uint32_t)off;
-            *(uint32_t*)(kCodes + slot * (D / 2) + kAt) = kw;
-            *(uint32_t*)(vCodes + slot * (D / 2) + 4 * j) = vc;
+            if (MODE == 1) {
+                *(uint32_t*)(kCodes + slot * (D / 2) + 4 * j) = kc0;
+                *(uint32_t*)(kCodes + slot * (D / 2) + D / 4 + 4 * j) = kc1;
+            } else {
+                *(uint2*)(kCodes + slot * (D / 2) + 8 * j) = make_uint2(kc0, kc1);
+            }
+            *(uint2*)(vCodes + slot * (D / 2) + 8 * j) = make_uint2(vc0, vc1);
             if (j == 0) {
                 kParams[slot] = kp;
                 vParams[slot] = vp;
@@ -151,39 +172,74 @@ __global__ void __launch_bounds__(256) append_kernel(const uint16_t* __restrict_
     }
 }
 
-// out[row] = rn16(least + step * code), row r from page table[r / pageSize], slot r % pageSize
-template <int DT, int D>
+// two elements: rn16(least + step * code) by one fused multiply-add of the 16-bit type, which rounds the exact sum once
+template <int DT> __device__ __forceinline__ uint32_t value2(uint32_t byte, uint32_t step2, uint32_t least2) {
+    constexpr uint32_t kOne = DT == DT_BF16 ? 0x3F803F80u : 0x3C003C00u;
+    constexpr uint32_t kBase = DT == DT_BF16 ? 0x43004300u : 0x64006400u;   // 128 / 1024: a unit in the last place is 1
+    uint32_t n = ((byte * 0x1001u) & 0x000F000Fu) | kBase, r;               // low four bits in the low half, high four in the high half
+    if (DT == DT_BF16) {
+        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(n) : "r"(n), "r"(kOne), "r"(kBase | 0x80008000u));
+        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(n), "r"(step2), "r"(least2));
+    } else {
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(n) : "r"(n), "r"(kOne), "r"(kBase | 0x80008000u));
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(n), "r"(step2), "r"(least2));
+    }
+    return r;
+}
+
+// out[row] = rn16(least + step * code), row r from page table[r / pageSize], slot r % pageSize.
+// Bound: the copies in flight (8 bytes of codes a lane turn into 32 bytes of output), so a lane starts UNROLL vectors before it finishes
+// the first, and stores whole 32-byte sectors.  (GATHER_FIGURES)
+template <int DT, int D, bool WIDE>
 __global__ void __launch_bounds__(256) gather_kernel(const uint8_t* __restrict__ codes, const uint32_t* __restrict__ params,
-                                                     const int32_t* __restrict__ table, uint16_t* __restrict__ out, uint32_t rows,
+                                                     const int32_t* __restrict__ table, uint16_t* __restrict__ out, uint32_t vectors,
                                                      uint32_t kvHeads, uint32_t pageCount, uint32_t pageSize, int* __restrict__ errorFlag) {
-    constexpr int LANES = D / 8, HEADS = 32 / LANES;
+    constexpr uint32_t LANES = D / 16, PER = 32 / LANES;
+    constexpr int UNROLL = 4;
     const uint32_t lane = threadIdx.x & 31, j = lane % LANES;
-    const uint32_t passes = (kvHeads + HEADS - 1) / HEADS;
-    const size_t units = (size_t)rows * passes, warps = (size_t)gridDim.x * (blockDim.x >> 5);
-    for (size_t u = (size_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); u < units; u += warps) {
-        const size_t row = u / passes;
-        const uint32_t pass = (uint32_t)(u - row * passes), head = pass * HEADS + lane / LANES;
-        const size_t entry = row / pageSize;
-        const int page = table[entry];
-        if (page < 0 || (uint32_t)page >= pageCount) {
-            if (lane == 0) atomicExch(errorFlag, 1);
-            continue;
-        }
-        if (head >= kvHeads) continue;
-        const size_t slot = ((size_t)page * kvHeads + head) * pageSize + (row - entry * pageSize);
-        const uint32_t c = __ldcs((const uint32_t*)(codes + slot * (D / 2) + 4 * j));
-        float step, least;
-        unpack16_arith<DT>(__ldg(params + slot), step, least);
-        Vec16 o;
+    const size_t stride = (size_t)gridDim.x * (blockDim.x >> 5) * PER;
+    for (size_t first = ((size_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * PER + lane / LANES; first < vectors; first += UNROLL * stride) {
+        uint2 c[UNROLL];
+        uint32_t par[UNROLL];
+        bool good[UNROLL];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            o.w[i] = pack16_arith<DT>(fmaf(step, (float)((c >> (8 * i)) & 15u), least), fmaf(step, (float)((c >> (8 * i + 4)) & 15u), least));
-        st_stream(out + (row * kvHeads + head) * D + 8 * j, o);
+        for (int u = 0; u < UNROLL; u++) {
+            const size_t vec = first + u * stride;
+            good[u] = false;
+            if (vec < vectors) {
+                const uint32_t row = (uint32_t)vec / kvHeads, head = (uint32_t)vec - row * kvHeads, entry = row / pageSize;
+                const int page = __ldg(table + entry);
+                good[u] = page >= 0 && (uint32_t)page < pageCount;
+                if (!good[u]) atomicExch(errorFlag, 1);
+                const size_t slot = good[u] ? ((size_t)page * kvHeads + head) * pageSize + (row - entry * pageSize) : 0;
+                c[u] = __ldcs((const uint2*)(codes + slot * (D / 2) + 8 * j));
+                par[u] = __ldg(params + slot);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            if (!good[u]) continue;
+            const uint32_t step2 = __byte_perm(par[u], 0, 0x1010), least2 = __byte_perm(par[u], 0, 0x3232);
+            uint32_t o[8];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                o[i] = value2<DT>((c[u].x >> (8 * i)) & 255u, step2, least2);
+                o[4 + i] = value2<DT>((c[u].y >> (8 * i)) & 255u, step2, least2);
+            }
+            uint16_t* dst = out + (first + u * stride) * D + 16 * j;
+            if (WIDE) {
+                asm volatile("st.global.L1::no_allocate.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                             ::"l"(dst), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
+            } else {
+                st_stream(dst, Vec16{{o[0], o[1], o[2], o[3]}});
+                st_stream(dst + 8, Vec16{{o[4], o[5], o[6], o[7]}});
+            }
+        }
     }
 }
 
 static int grid_of(Context* ctx, size_t warps) {
-    const size_t blocks = (warps + 7) / 8, cap = (size_t)ctx->smCount * 8;  // 8 blocks of 256 threads fill an SM
+    const size_t blocks = (warps + 8) / 8, cap = (size_t)ctx->smCount * 8;  // 8 blocks of 256 threads fill an SM
     return (int)(blocks < cap ? (blocks ? blocks : 1) : cap);
 }
 
@@ -233,13 +289,14 @@ extern "C" int cuda_dispatch_rope_kv_page_write_q4(CUDADeviceRef contextRef, int
         if (!table) return status ? status->code : -7;
     }
     const float* sinT = table ? table + (size_t)maxPositions * (headDim / 2) : nullptr;
-    const uint32_t heads = 256 / headDim;  // per pass of a warp
-    const int grid = q4::grid_of(ctx, (size_t)rows * ((kvHeads + heads - 1) / heads));
+    if ((size_t)rows * kvHeads > 0xFFFFFFFFull) return fail(status, -2, "rope kv page write (4 bits): %u rows of %u heads exceed 32 bits", rows, kvHeads);
+    const uint32_t vectors = rows * kvHeads;
+    const int grid = q4::grid_of(ctx, (size_t)vectors * headDim / 512);
 #define APPEND_LAUNCH(DT, D, MODE)                                                                                                  \
     q4::append_kernel<DT, D, MODE><<<grid, 256, 0, ctx->stream>>>(                                                                  \
         (const uint16_t*)dev_ptr(kRef), (const uint16_t*)dev_ptr(vRef), MODE == 2 ? nullptr : (const int32_t*)dev_ptr(positionsRef), \
         (const int32_t*)dev_ptr(pageIDsRef), (const int32_t*)dev_ptr(offsetsRef), (uint8_t*)dev_ptr(kCodesRef),                     \
-        (uint32_t*)dev_ptr(kParamsRef), (uint8_t*)dev_ptr(vCodesRef), (uint32_t*)dev_ptr(vParamsRef), table, sinT, rows, kvHeads,   \
+        (uint32_t*)dev_ptr(kParamsRef), (uint8_t*)dev_ptr(vCodesRef), (uint32_t*)dev_ptr(vParamsRef), table, sinT, vectors, kvHeads, \
         pageCount, pageSize, maxPositions, ctx->errorFlag)
 #define APPEND_PICK(DT, D)                                 \
     do {                                                   \
@@ -275,12 +332,19 @@ extern "C" int cuda_dispatch_kv_page_gather_q4(CUDADeviceRef contextRef, int ele
     PUTER_REQUIRE(outputRef, "output", (size_t)outRows * kvHeads * headDim * 2);
     if ((((uintptr_t)dev_ptr(codesRef) | (uintptr_t)dev_ptr(paramsRef) | (uintptr_t)dev_ptr(outputRef)) & 15u) != 0)
         return fail(status, -2, "page gather (4 bits): buffers must be 16-byte aligned");
-    const uint32_t heads = 256 / headDim;
-    const int grid = q4::grid_of(ctx, (size_t)outRows * ((kvHeads + heads - 1) / heads));
-#define GATHER_LAUNCH(DT, D)                                                                                                          \
-    q4::gather_kernel<DT, D><<<grid, 256, 0, ctx->stream>>>((const uint8_t*)dev_ptr(codesRef), (const uint32_t*)dev_ptr(paramsRef),   \
-                                                            (const int32_t*)dev_ptr(pageTableRef), (uint16_t*)dev_ptr(outputRef), outRows, \
-                                                            kvHeads, pageCount, pageSize, ctx->errorFlag)
+    if ((size_t)outRows * kvHeads > 0xFFFFFFFFull) return fail(status, -2, "page gather (4 bits): %u rows of %u heads exceed 32 bits", outRows, kvHeads);
+    const uint32_t vectors = outRows * kvHeads;
+    const int grid = q4::grid_of(ctx, (size_t)vectors * headDim / 512);
+    const bool wide = ((uintptr_t)dev_ptr(outputRef) & 31u) == 0;
+#define GATHER_KERNEL(DT, D, WIDE)                                                                                                    \
+    q4::gather_kernel<DT, D, WIDE><<<grid, 256, 0, ctx->stream>>>((const uint8_t*)dev_ptr(codesRef), (const uint32_t*)dev_ptr(paramsRef), \
+                                                                  (const int32_t*)dev_ptr(pageTableRef), (uint16_t*)dev_ptr(outputRef), \
+                                                                  vectors, kvHeads, pageCount, pageSize, ctx->errorFlag)
+#define GATHER_LAUNCH(DT, D)                          \
+    do {                                              \
+        if (wide) GATHER_KERNEL(DT, D, true);         \
+        else GATHER_KERNEL(DT, D, false);             \
+    } while (0)
     if (elementDType == DT_BF16) {
         if (headDim == 128) GATHER_LAUNCH(DT_BF16, 128);
         else GATHER_LAUNCH(DT_BF16, 64);
@@ -289,5 +353,6 @@ extern "C" int cuda_dispatch_kv_page_gather_q4(CUDADeviceRef contextRef, int ele
         else GATHER_LAUNCH(DT_F16, 64);
     }
 #undef GATHER_LAUNCH
+#undef GATHER_KERNEL
     return check_launch(ctx, status, "page gather (4 bits)");
 }

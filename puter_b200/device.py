@@ -128,7 +128,7 @@ class Device:
 
     def _enter(self):
         if self.follow_torch_stream:
-            s = self._torch.cuda.current_stream(self.ordinal).cuda_stream
+            s = self._torch._C._cuda_getCurrentRawStream(self.ordinal)  # (cuda.current_stream() builds two objects per call: 3 us)
             if s != self._stream:  # the library keeps the stream until told otherwise: only a change costs a call
                 self.lib.cuda_context_set_stream(self.ref, ctypes.c_void_p(s), ctypes.byref(self._status))
                 self._stream = s
@@ -140,7 +140,7 @@ class Device:
         if t is None:
             return None
         assert t.is_cuda and t.is_contiguous(), "device tensors must be contiguous CUDA memory"
-        key = (t.data_ptr(), t.numel() * t.element_size())
+        key = (t.data_ptr(), t.nbytes)
         r = self._refs.get(key)
         if r is None:
             r = ctypes.c_void_p(self.lib.cuda_buffer_wrap(self.ref, ctypes.c_void_p(key[0]), key[1]))

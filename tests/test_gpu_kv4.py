@@ -1,7 +1,7 @@
 """The paged cache in 4 bits: producer, page gather and decode attention against plain implementations.
 
 Quantisation is defined operation by operation in float32, so codes and params are compared bit for bit (numpy float32 rounds like the
-kernel: separate products and sums, IEEE division).  K goes through a cos / sin table: a table entry may differ from numpy's in the last
+kernel: separate products and sums; the span times float32(1 / 15), the levels by IEEE division).  K goes through a cos / sin table: a table entry may differ from numpy's in the last
 bit of float32 on a rare tie of float64, so up to 1 in 10^4 codes may be another one, never by more than one level.
 
 Decode, with u = eps / 2 of the storage type, S = max over tokens of 15 * step (the span of a value's levels), V = max |value|:
@@ -29,7 +29,7 @@ def quantise(x, fmt):
     """(levels uint8 [..., dim], step, least) of float32 vectors."""
     x = np.asarray(x, np.float32)
     lo, hi = x.min(-1, keepdims=True), x.max(-1, keepdims=True)
-    step, least = round16((hi - lo) / np.float32(15), fmt), round16(lo, fmt)
+    step, least = round16((hi - lo) * np.float32(1 / 15), fmt), round16(lo, fmt)
     with np.errstate(divide="ignore", invalid="ignore"):
         y = np.where(step > 0, (x - least) / step, np.float32(0))
     return np.clip(np.rint(y), 0, 15).astype(np.uint8), step, least
