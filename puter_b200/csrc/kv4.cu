@@ -38,6 +38,18 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return d;
 }
 
+// of three
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // nearest level of t >= 0 (up to rounding) in units of s: rint(t / s) with the quotient's own rounding.  The product with the
 // reciprocal is off by less than 4e-6 on 0 .. 15, so only a quotient that close to a tie is divided out: ties are common among
 // 16-bit values, and they go to the even level as the division says.
@@ -73,9 +85,9 @@ template <int DT, int LANES>
 __device__ __forceinline__ void quantise(const float* x, uint32_t& c0, uint32_t& c1, uint32_t& params) {
     float lo = min_nan(x[0], x[1]), hi = max_nan(x[0], x[1]);
 #pragma unroll
-    for (int i = 2; i < 16; i++) {
-        lo = min_nan(lo, x[i]);
-        hi = max_nan(hi, x[i]);
+    for (int i = 2; i < 16; i += 2) {
+        lo = min3_nan(lo, x[i], x[i + 1]);
+        hi = max3_nan(hi, x[i], x[i + 1]);
     }
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) {
@@ -195,7 +207,7 @@ __global__ void __launch_bounds__(256) gather_kernel(const uint8_t* __restrict__
                                                      const int32_t* __restrict__ table, uint16_t* __restrict__ out, uint32_t vectors,
                                                      uint32_t kvHeads, uint32_t pageCount, uint32_t pageSize, int* __restrict__ errorFlag) {
     constexpr uint32_t LANES = D / 16, PER = 32 / LANES;
-    constexpr int UNROLL = 4;
+    constexpr int UNROLL = 2;
     const uint32_t lane = threadIdx.x & 31, j = lane % LANES;
     const size_t stride = (size_t)gridDim.x * (blockDim.x >> 5) * PER;
     for (size_t first = ((size_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * PER + lane / LANES; first < vectors; first += UNROLL * stride) {

@@ -7,7 +7,8 @@
 // Rows that belong to no sequence (before the first start, behind the last) are neither read into a result nor written.
 // A pair of starts that is not 0 <= start <= end <= totalTokens with at most maxSeqLen rows is skipped and raises the error flag.
 //
-// Two kernels.  rows_kernel is a warp per (row, head) for any type and head dimension.  pk::tiles_kernel is the tensor-core form (bf16 / f16,
+// Three kernels.  rows_kernel is a warp per (row, head) for any type and head dimension.  short_kernel is for calls without long sequences: a
+// block per (sequence, KV head), see there.  tiles_kernel is the tensor-core form (bf16 / f16,
 // head dimensions up to 128 that are multiples of 8), built like the prefill kernel for equal lengths: two tiles of 128 rows that take turns
 // on the tensor core, softmax in registers with one row a thread, P handed back through TMEM, K and V through a TMA ring.  What the
 // different lengths change:
@@ -15,7 +16,7 @@
 //     positions: a group of 4 turns 33 tokens into 132 rows instead of 4 x 33 of 128, and short prompts are what packing is for.
 //     A TMA box of 64 dimensions x PACK heads x 128 / PACK rows brings such a tile in; long prompts cost the same either way.
 //   * The work list (sequence, block of 2 * 128 / PACK positions) is built on the device, longest key ranges first, by the first block of the
-//     launch that also rotates: the host never learns the lengths.
+//     launch that also rotates K: the host never learns the lengths.  Q is rotated in its tile (head dimensions 64 and 128).
 //   * Keys behind the end of a sequence and keys that a row may not see are masked by position; their weights are exactly zero.  A value row
 //     that is not finite would still reach every row of the tile through 0 * NaN, so a warp looks through the value tiles that are not
 //     seen by all rows, clears what is not finite, and the rows that do see it add it back at the end.
@@ -268,6 +269,8 @@ struct TileParams {
     uint16_t* out;
     int* errorFlag;
     int heads, kvHeads, dim, causal;
+    const float *cosT, *sinT;  // nullptr: q comes rotated (or no rotation)
+    int halves, posLast;       // last position of the tables
     int packLog, headGroups;  // PACK = 1 << packLog heads per tile, heads / PACK tiles per block of positions
     float scaleLog2;
 };
@@ -314,6 +317,78 @@ __device__ __noinline__ void add_not_finite(float* o, const uint16_t* v, size_t 
             const uint32_t bits = v[(size_t)key * stride + i];
             if (not_finite<BF16>(bits)) o[i] += widen16<BF16>(bits);
         }
+}
+
+// Rotates the 32 rows of a warp in a Q tile once it has landed: the lanes of a row own eight pairs each (halves: a 16-byte piece and its
+// partner half a head further) or four (neighbouring pairs: one piece).  The cos / sin values are fetched before the wait.  Not inlined: its
+// 128 table registers are apart from the scores of the caller.
+template <bool BF16, int NB>
+__device__ __noinline__ bool rotate_q_when_loaded(unsigned char* tile, int row0, int lane, bool halves, const float* cosT, const float* sinT, int pos0,
+                                                   int posLast, int packLog, uint32_t bar, uint32_t parity, volatile int* abortFlag) {
+    constexpr int HALF = 32 * NB;  // pairs of a head
+    float4 tab[16 * NB];
+    if (halves) {
+        const int c = lane % (4 * NB);
+#pragma unroll
+        for (int it = 0; it < 4 * NB; it++) {
+            const size_t at = (size_t)min(pos0 + ((row0 + it * (8 / NB) + lane / (4 * NB)) >> packLog), posLast) * HALF + 8 * c;
+            tab[4 * it] = __ldg((const float4*)(cosT + at));
+            tab[4 * it + 1] = __ldg((const float4*)(cosT + at + 4));
+            tab[4 * it + 2] = __ldg((const float4*)(sinT + at));
+            tab[4 * it + 3] = __ldg((const float4*)(sinT + at + 4));
+        }
+    } else {
+        const int c = lane % (8 * NB);
+#pragma unroll
+        for (int it = 0; it < 8 * NB; it++) {
+            const size_t at = (size_t)min(pos0 + ((row0 + it * (4 / NB) + lane / (8 * NB)) >> packLog), posLast) * HALF + 4 * c;
+            tab[2 * it] = __ldg((const float4*)(cosT + at));
+            tab[2 * it + 1] = __ldg((const float4*)(sinT + at));
+        }
+    }
+    if (!__all_sync(0xffffffffu, mbar_wait(bar, parity, abortFlag))) return false;
+    if (halves) {
+        const int c = lane % (4 * NB);
+#pragma unroll
+        for (int it = 0; it < 4 * NB; it++) {
+            const int row = row0 + it * (8 / NB) + lane / (4 * NB);
+            unsigned char* const line = tile + row * 128;
+            Vec16* const pa = (Vec16*)(line + ((c ^ (row & 7)) * 16));
+            Vec16* const pb = NB == 2 ? (Vec16*)((unsigned char*)pa + kBlock) : (Vec16*)(line + (((c + 4) ^ (row & 7)) * 16));
+            Vec16 a = *pa, b = *pb;
+            const float4 c0 = tab[4 * it], c1 = tab[4 * it + 1], n0 = tab[4 * it + 2], n1 = tab[4 * it + 3];
+            const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, sn[8] = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, n1.z, n1.w};
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const uint64_t E = pk2(widen16<BF16>(a.w[w] & 0xFFFFu), widen16<BF16>(a.w[w] >> 16)), O = pk2(widen16<BF16>(b.w[w] & 0xFFFFu), widen16<BF16>(b.w[w] >> 16));
+                const uint64_t C = pk2(cs[2 * w], cs[2 * w + 1]), S = pk2(sn[2 * w], sn[2 * w + 1]), NS = pk2(-sn[2 * w], -sn[2 * w + 1]);
+                float x0, x1, y0, y1;
+                un2(fma2(O, NS, mul2(E, C)), x0, x1);  // e c - o s
+                un2(fma2(E, S, mul2(O, C)), y0, y1);   // e s + o c
+                a.w[w] = pack2<BF16>(x0, x1);
+                b.w[w] = pack2<BF16>(y0, y1);
+            }
+            *pa = a;
+            *pb = b;
+        }
+    } else {
+        const int c = lane % (8 * NB);
+#pragma unroll
+        for (int it = 0; it < 8 * NB; it++) {
+            const int row = row0 + it * (4 / NB) + lane / (8 * NB);
+            Vec16* const pa = (Vec16*)(tile + (c >> 3) * kBlock + row * 128 + (((c & 7) ^ (row & 7)) * 16));
+            Vec16 a = *pa;
+            const float cs[4] = {tab[2 * it].x, tab[2 * it].y, tab[2 * it].z, tab[2 * it].w}, sn[4] = {tab[2 * it + 1].x, tab[2 * it + 1].y, tab[2 * it + 1].z, tab[2 * it + 1].w};
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float e = widen16<BF16>(a.w[w] & 0xFFFFu), o = widen16<BF16>(a.w[w] >> 16);
+                a.w[w] = pack2<BF16>(sub(mul(e, cs[w]), mul(o, sn[w])), add(mul(e, sn[w]), mul(o, cs[w])));
+            }
+            *pa = a;
+        }
+    }
+    __syncwarp();
+    return true;
 }
 
 template <bool BF16, int NB>
@@ -613,7 +688,13 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
             }
             if (n == 0) continue;
             const int seen = p.causal ? min(pos + (row >> p.packLog) + 1, len) : len;  // keys this row sees
-            okay = __all_sync(0xffffffffu, mbar_wait(bar(B::Q + t), uc & 1, abortFlag));
+            if (p.cosT) {
+                okay = rotate_q_when_loaded<BF16, NB>(smem + M::Q + t * M::TILE, (warp & 3) * 32, lane, p.halves != 0, p.cosT, p.sinT, pos, p.posLast, p.packLog,
+                                                      bar(B::Q + t), uc & 1, abortFlag);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // generic writes -> visible to the tensor core
+            } else {
+                okay = __all_sync(0xffffffffu, mbar_wait(bar(B::Q + t), uc & 1, abortFlag));
+            }
             mbar_arrive(bar(B::QREADY + t));
             float mUsed = -INFINITY;  // the maximum the stored P and O are relative to (scaled, log2 domain)
             float lsum = 0.f;
@@ -744,6 +825,287 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     }
 }
 
+// ---------------------------------------------------------------------------------------------------------------------------------
+// short sequences (no longer than kShortMax): a block per (sequence, KV head)
+// ---------------------------------------------------------------------------------------------------------------------------------
+// The tensor-core kernel spends a pipeline of five barriers and a 128 x 128 tile on a sequence of a few tokens, ~5 us per (sequence, head)
+// and SM.  Here a block brings K (rotated once) and V of its sequence into shared memory and its warps take 16 rows each, the row being
+// (position, query head of the group) so that all heads of the group share them: warp-level products (mma.sync), one launch, no list,
+// no scratch.  Q is rotated in registers.  Elements that are not finite are taken out of V and added back as in the tile kernel.
+// Shared-memory order: K in 16-byte pieces, the upper half of eight exchanged in odd rows (the eight lanes of a load read two rows);
+// V with the dimensions of 32 reordered so that a lane's accumulators are eight neighbouring dimensions, piece ^ (row & 7) for the
+// transposing loads.
+constexpr int kShortMax = 160;
+constexpr int kShortWarps = 4;
+
+__device__ __forceinline__ void mma16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, bool bf16) {
+    if (bf16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix_trans(uint32_t at, uint32_t* r) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
+
+// eight neighbouring elements rotated with their own pairs (interleaved) or with the eight `b` half a head further (halves)
+template <bool BF16>
+__device__ __forceinline__ void rotate8(Vec16& a, Vec16& b, const float* cosRow, const float* sinRow, bool halves) {
+    constexpr int DT = BF16 ? DT_BF16 : DT_F16;
+    if (halves) {
+        float cs[8], sn[8];
+        *(float4*)cs = __ldg((const float4*)cosRow);
+        *(float4*)(cs + 4) = __ldg((const float4*)(cosRow + 4));
+        *(float4*)sn = __ldg((const float4*)sinRow);
+        *(float4*)(sn + 4) = __ldg((const float4*)(sinRow + 4));
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            float e0, e1, o0, o1;
+            unpack16_arith<DT>(a.w[w], e0, e1);
+            unpack16_arith<DT>(b.w[w], o0, o1);
+            a.w[w] = pack16_arith<DT>(sub(mul(e0, cs[2 * w]), mul(o0, sn[2 * w])), sub(mul(e1, cs[2 * w + 1]), mul(o1, sn[2 * w + 1])));
+            b.w[w] = pack16_arith<DT>(add(mul(e0, sn[2 * w]), mul(o0, cs[2 * w])), add(mul(e1, sn[2 * w + 1]), mul(o1, cs[2 * w + 1])));
+        }
+    } else {
+        const float4 c = __ldg((const float4*)cosRow), n = __ldg((const float4*)sinRow);
+        const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {n.x, n.y, n.z, n.w};
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            float e, o;
+            unpack16_arith<DT>(a.w[w], e, o);
+            a.w[w] = pack16_arith<DT>(sub(mul(e, cs[w]), mul(o, sn[w])), add(mul(e, sn[w]), mul(o, cs[w])));
+        }
+    }
+}
+
+struct ShortParams {
+    const uint16_t *q, *k, *v;
+    uint16_t* out;
+    Seqs seqs;
+    const float *cosT, *sinT;
+    int heads, kvHeads, dim, causal, ropeMode, rows;  // rows of shared memory: the longest sequence, a multiple of 32
+    float scaleLog2;
+};
+
+template <bool BF16, int D>
+__global__ void __launch_bounds__(kShortWarps * 32) short_kernel(ShortParams p) {
+    constexpr int PIECES = D / 8;  // 16-byte pieces of a row
+    extern __shared__ __align__(128) unsigned char smemShort[];
+    __shared__ int notFinite;
+    int row0, end;
+    if (!seq_rows(p.seqs, blockIdx.x, row0, end)) return;
+    const int len = end - row0, group = p.heads / p.kvHeads, kvh = blockIdx.y;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int blocks = (len * group + 15) / 16;  // of 16 rows
+    const int firstBlock = blockIdx.z * kShortWarps;
+    if (firstBlock >= blocks) return;
+    // keys that this block's rows see
+    const int stride = gridDim.z * kShortWarps;
+    const int lastBlock = firstBlock + (blocks - 1 - firstBlock) / stride * stride + kShortWarps - 1;
+    const int keys = p.causal ? min(len, (min(lastBlock * 16 + 15, len * group - 1)) / group + 1) : len;
+    const int padded = (keys + 31) & ~31;
+    unsigned char* const kTile = smemShort;
+    unsigned char* const vTile = smemShort + (size_t)p.rows * D * 2;
+    if (threadIdx.x == 0) notFinite = 0;
+    __syncthreads();
+    const int half = p.dim / 2;
+    const bool halves = p.ropeMode == 1;
+    {
+        // (four pieces of a thread are on their way before the first is used: the loop waits for memory once, not per piece)
+        constexpr int KP = PIECES / 2, THREADS = kShortWarps * 32, U = 4;  // a thread takes pieces c and c + KP of a K row: partners in half mode
+        for (int i0 = threadIdx.x; i0 < padded * KP; i0 += U * THREADS) {
+            Vec16 a[U], b[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int i = i0 + u * THREADS, r = i / KP, c = i % KP;
+                a[u] = b[u] = Vec16{};
+                if (r < keys) {
+                    const uint16_t* src = p.k + ((size_t)(row0 + r) * p.kvHeads + kvh) * p.dim;
+                    if (c * 8 < p.dim) a[u] = *(const Vec16*)(src + c * 8);
+                    if ((c + KP) * 8 < p.dim) b[u] = *(const Vec16*)(src + (c + KP) * 8);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int i = i0 + u * THREADS, r = i / KP, c = i % KP;
+                if (r >= padded) break;
+                if (p.ropeMode != 2 && r < keys) {  // (dim == D)
+                    const float* cr = p.cosT + (size_t)r * half;
+                    const float* sr = p.sinT + (size_t)r * half;
+                    if (halves) {
+                        rotate8<BF16>(a[u], b[u], cr + 8 * c, sr + 8 * c, true);
+                    } else {
+                        rotate8<BF16>(a[u], a[u], cr + 4 * c, sr + 4 * c, false);
+                        rotate8<BF16>(b[u], b[u], cr + 4 * (c + KP), sr + 4 * (c + KP), false);
+                    }
+                }
+                const int x = (r & 1) << 2;
+                *(Vec16*)(kTile + ((size_t)r * PIECES + (c ^ x)) * 16) = a[u];
+                *(Vec16*)(kTile + ((size_t)r * PIECES + ((c + KP) ^ x)) * 16) = b[u];
+            }
+        }
+        uint32_t found = 0;
+        for (int i0 = threadIdx.x; i0 < padded * PIECES; i0 += 2 * U * THREADS) {
+            Vec16 a[2 * U];
+#pragma unroll
+            for (int u = 0; u < 2 * U; u++) {
+                const int i = i0 + u * THREADS, r = i / PIECES, c = i % PIECES;
+                a[u] = Vec16{};
+                if (r < keys && c * 8 < p.dim) a[u] = *(const Vec16*)(p.v + ((size_t)(row0 + r) * p.kvHeads + kvh) * p.dim + c * 8);
+            }
+#pragma unroll
+            for (int u = 0; u < 2 * U; u++) {
+                const int i = i0 + u * THREADS, r = i / PIECES, c = i % PIECES;
+                if (r >= padded) break;
+                // dimension 32G + 8a + 2q + e goes to place 32G + 8q + 2a + e
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const uint32_t bad = not_finite<BF16>(a[u].w[q]);
+                    found |= bad;
+                    *(uint32_t*)(vTile + ((size_t)r * PIECES + (((c & ~3) + q) ^ (r & 7))) * 16 + (c & 3) * 4) = a[u].w[q] & ~((bad >> 15) * 0xFFFFu);
+                }
+            }
+        }
+        if (found) notFinite = 1;
+    }
+    __syncthreads();
+    for (int blk = firstBlock + warp; blk < blocks; blk += stride) {
+        const int rA = blk * 16 + g, rB = rA + 8, rows = len * group;
+        const int posA = min(rA, rows - 1) / group, posB = min(rB, rows - 1) / group;
+        const size_t atA = ((size_t)(row0 + posA) * p.heads + kvh * group + min(rA, rows - 1) - posA * group) * p.dim;
+        const size_t atB = ((size_t)(row0 + posB) * p.heads + kvh * group + min(rB, rows - 1) - posB * group) * p.dim;
+        // lane t holds dimensions 32m + 8t .. + 7 of rows g and g + 8; K is read in the same order, so the order of the products is free
+        Vec16 qa[D / 32], qb[D / 32];
+#pragma unroll
+        for (int m = 0; m < D / 32; m++) {
+            const int d = 32 * m + 8 * t;
+            qa[m] = qb[m] = Vec16{};
+            if (d < p.dim) {
+                qa[m] = *(const Vec16*)(p.q + atA + d);
+                qb[m] = *(const Vec16*)(p.q + atB + d);
+            }
+        }
+        if (p.ropeMode != 2) {
+#pragma unroll
+            for (int m = 0; m < D / 64; m++) {
+                const int c = halves ? 32 * m + 8 * t : 16 * m + 4 * t;
+                rotate8<BF16>(qa[m], qa[m + D / 64], p.cosT + (size_t)posA * half + c, p.sinT + (size_t)posA * half + c, halves);
+                rotate8<BF16>(qb[m], qb[m + D / 64], p.cosT + (size_t)posB * half + c, p.sinT + (size_t)posB * half + c, halves);
+                if (!halves) {
+                    const int c2 = c + D / 4;
+                    rotate8<BF16>(qa[m + D / 64], qa[m], p.cosT + (size_t)posA * half + c2, p.sinT + (size_t)posA * half + c2, false);
+                    rotate8<BF16>(qb[m + D / 64], qb[m], p.cosT + (size_t)posB * half + c2, p.sinT + (size_t)posB * half + c2, false);
+                }
+            }
+        }
+        const int seenA = p.causal ? posA + 1 : len, seenB = p.causal ? posB + 1 : len;
+        const int last = p.causal ? min(blk * 16 + 15, rows - 1) / group + 1 : len;  // keys that any of the rows sees
+        float o[D / 8][4];
+#pragma unroll
+        for (int n = 0; n < D / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+        float mA = -INFINITY, mB = -INFINITY, lA = 0.f, lB = 0.f;
+        for (int key0 = 0; key0 < last; key0 += 32) {
+            float s[4][4];
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+                const int key = key0 + 8 * n + g;
+#pragma unroll
+                for (int m = 0; m < D / 32; m++) {
+                    const Vec16 b = *(const Vec16*)(kTile + ((size_t)key * PIECES + ((4 * m + t) ^ ((key & 1) << 2))) * 16);
+                    mma16(s[n], qa[m].w[0], qb[m].w[0], qa[m].w[1], qb[m].w[1], b.w[0], b.w[1], BF16);
+                    mma16(s[n], qa[m].w[2], qb[m].w[2], qa[m].w[3], qb[m].w[3], b.w[2], b.w[3], BF16);
+                }
+            }
+            float topA = -INFINITY, topB = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < 4; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int key = key0 + 8 * n + 2 * t + e;
+                    s[n][e] = key < seenA ? s[n][e] * p.scaleLog2 : -INFINITY;
+                    s[n][2 + e] = key < seenB ? s[n][2 + e] * p.scaleLog2 : -INFINITY;
+                    topA = fmaxf(topA, s[n][e]);
+                    topB = fmaxf(topB, s[n][2 + e]);
+                }
+            topA = fmaxf(topA, __shfl_xor_sync(0xffffffffu, topA, 1));
+            topB = fmaxf(topB, __shfl_xor_sync(0xffffffffu, topB, 1));
+            topA = fmaxf(topA, __shfl_xor_sync(0xffffffffu, topA, 2));
+            topB = fmaxf(topB, __shfl_xor_sync(0xffffffffu, topB, 2));
+            const float nA = fmaxf(mA, topA), nB = fmaxf(mB, topB);
+            const float fromA = nA == -INFINITY ? 0.f : nA, fromB = nB == -INFINITY ? 0.f : nB;  // nothing but scores of -inf so far
+            const float aA = ex2_approx(mA - fromA), aB = ex2_approx(mB - fromB);
+            mA = nA;
+            mB = nB;
+            if (key0 > 0 && __any_sync(0xffffffffu, aA != 1.f || aB != 1.f)) {
+                lA *= aA;
+                lB *= aB;
+#pragma unroll
+                for (int n = 0; n < D / 8; n++) {
+                    o[n][0] *= aA;
+                    o[n][1] *= aA;
+                    o[n][2] *= aB;
+                    o[n][3] *= aB;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < 4; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    s[n][e] = ex2_approx(s[n][e] - fromA);
+                    s[n][2 + e] = ex2_approx(s[n][2 + e] - fromB);
+                    lA += s[n][e];
+                    lB += s[n][2 + e];
+                }
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) {
+                const uint32_t p0 = pack2<BF16>(s[2 * ks][0], s[2 * ks][1]), p1 = pack2<BF16>(s[2 * ks][2], s[2 * ks][3]);
+                const uint32_t p2 = pack2<BF16>(s[2 * ks + 1][0], s[2 * ks + 1][1]), p3 = pack2<BF16>(s[2 * ks + 1][2], s[2 * ks + 1][3]);
+                const int key = key0 + 16 * ks + (lane & 15);
+#pragma unroll
+                for (int n = 0; n < D / 8; n += 2) {
+                    uint32_t b[4];  // dimensions 8n .. + 7 of keys 0 - 7 and 8 - 15, then the next eight dimensions
+                    ldmatrix_trans(smem_u32(vTile + ((size_t)key * PIECES + ((n + (lane >> 4)) ^ (key & 7))) * 16), b);
+                    mma16(o[n], p0, p1, p2, p3, b[0], b[1], BF16);
+                    mma16(o[n + 1], p0, p1, p2, p3, b[2], b[3], BF16);
+                }
+            }
+        }
+        lA += __shfl_xor_sync(0xffffffffu, lA, 1);
+        lB += __shfl_xor_sync(0xffffffffu, lB, 1);
+        lA += __shfl_xor_sync(0xffffffffu, lA, 2);
+        lB += __shfl_xor_sync(0xffffffffu, lB, 2);
+        const float iA = 1.0f / lA, iB = 1.0f / lB;
+#pragma unroll
+        for (int m = 0; m < D / 32; m++) {
+            const int d = 32 * m + 8 * t;
+            if (d >= p.dim) continue;
+            float x[8], y[8];
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                x[2 * q] = o[4 * m + q][0] * iA;
+                x[2 * q + 1] = o[4 * m + q][1] * iA;
+                y[2 * q] = o[4 * m + q][2] * iB;
+                y[2 * q + 1] = o[4 * m + q][3] * iB;
+            }
+            if (notFinite) {
+                const uint16_t* v = p.v + ((size_t)row0 * p.kvHeads + kvh) * p.dim + d;
+                float xs[8], ys[8];  // (memory of their own: x and y stay in registers)
+#pragma unroll
+                for (int i = 0; i < 8; i++) { xs[i] = x[i]; ys[i] = y[i]; }
+                add_not_finite<BF16>(xs, v, (size_t)p.kvHeads * p.dim, 0, seenA, 8);
+                add_not_finite<BF16>(ys, v, (size_t)p.kvHeads * p.dim, 0, seenB, 8);
+#pragma unroll
+                for (int i = 0; i < 8; i++) { x[i] = xs[i]; y[i] = ys[i]; }
+            }
+            if (rA < rows) *(Vec16*)(p.out + atA + d) = Vec16{{pack2<BF16>(x[0], x[1]), pack2<BF16>(x[2], x[3]), pack2<BF16>(x[4], x[5]), pack2<BF16>(x[6], x[7])}};
+            if (rB < rows) *(Vec16*)(p.out + atB + d) = Vec16{{pack2<BF16>(y[0], y[1]), pack2<BF16>(y[2], y[3]), pack2<BF16>(y[4], y[5]), pack2<BF16>(y[6], y[7])}};
+        }
+    }
+}
+
 // [total, heads, dim] 16-bit -> 3-D map (dim, head, row) with a box of 64 x boxHeads x boxRows and 128-byte swizzle
 static bool make_map(CUtensorMap* tm, const void* base, bool bf16, uint32_t total, uint32_t heads, uint32_t dim, uint32_t boxHeads, uint32_t boxRows) {
     EncodeTiledFn fn = encode_fn();
@@ -774,6 +1136,38 @@ static bool tiles_take(const Call& c) {
     return (all & 15u) == 0 && encode_fn() != nullptr;
 }
 
+// By rows per (sequence, KV head), measured on both sides (us, short against tiles): 200 sequences of up to 96 rows 22 : 72, 64 of 128 rows 26 : 36,
+// of 256 rows (64 tokens, group 4) 50 : 42; and where all blocks of 64 rows fit the SMs at once the short latency decides: one sequence of
+// 33 tokens 7.7 : 13.8, of 128 12.5 : 14.9, of 256 20.9 : 16.6.
+static bool short_takes(Context* ctx, const Call& c) {
+    if (!tiles_take(c) || c.seqs.maxLen > kShortMax || c.kvHeads > 65535 || (c.ropeMode != 2 && c.dim != 64 && c.dim != 128)) return false;
+    const size_t rows = (size_t)c.seqs.maxLen * (c.heads / c.kvHeads), pairs = (size_t)c.seqs.batch * c.kvHeads;
+    return rows <= 160 || (c.seqs.maxLen <= 128 && pairs * rows <= 64 * (size_t)ctx->smCount);
+}
+
+template <bool BF16>
+static int short_launch(Context* ctx, const Call& c, CUDAStatus* status) {
+    const uint32_t group = c.heads / c.kvHeads, D = c.dim > 64 ? 128 : 64;
+    ShortParams p{(const uint16_t*)c.q, (const uint16_t*)c.k, (const uint16_t*)c.v, (uint16_t*)c.out, c.seqs, c.cosT, c.sinT, (int)c.heads, (int)c.kvHeads,
+                  (int)c.dim, (int)c.causal, (int)c.ropeMode, (c.seqs.maxLen + 31) & ~31, (float)(1.4426950408889634 / sqrt((double)c.dim))};
+    // several blocks per (sequence, KV head) while there are too few to fill the GPU twice; each has four blocks of 16 rows at least
+    const size_t pairs = (size_t)c.seqs.batch * c.kvHeads, most = ((size_t)c.seqs.maxLen * group + 16 * kShortWarps - 1) / (16 * kShortWarps);
+    size_t split = (2 * (size_t)ctx->smCount + pairs - 1) / pairs;
+    if (split > most) split = most;
+    if (split > 65535) split = 65535;
+    const size_t smem = (size_t)p.rows * D * 4;
+    const dim3 grid((unsigned)c.seqs.batch, c.kvHeads, (unsigned)split);
+#define SHORT(D)                                                                                                                        \
+    do {                                                                                                                                \
+        cudaFuncSetAttribute(short_kernel<BF16, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);                            \
+        short_kernel<BF16, D><<<grid, kShortWarps * 32, smem, ctx->stream>>>(p);                                                        \
+    } while (0)
+    if (D == 128) SHORT(128);
+    else SHORT(64);
+#undef SHORT
+    return check_launch(ctx, status, "packed prefill attention (short)");
+}
+
 template <bool BF16>
 static int tiles_launch(Context* ctx, const Call& c, CUDAStatus* status) {
     constexpr int DT = BF16 ? DT_BF16 : DT_F16;
@@ -783,7 +1177,8 @@ static int tiles_launch(Context* ctx, const Call& c, CUDAStatus* status) {
     const int span = 2 * (kRows >> packLog);
     const uint32_t total = (uint32_t)c.seqs.total;
     const size_t levels = ((size_t)c.seqs.maxLen + span - 1) / span, most = (size_t)total / span + c.seqs.batch;  // entries at most
-    const size_t qBytes = c.ropeMode != 2 ? (((size_t)total * c.heads * c.dim * 2) + 255) & ~(size_t)255 : 0;
+    const bool fused = c.ropeMode != 2 && (c.dim == 64 || c.dim == 128);  // q is rotated in its tile: a pass over q would cost as much as reading it all
+    const size_t qBytes = c.ropeMode != 2 && !fused ? (((size_t)total * c.heads * c.dim * 2) + 255) & ~(size_t)255 : 0;
     const size_t kBytes = c.ropeMode != 2 ? (((size_t)total * c.kvHeads * c.dim * 2) + 255) & ~(size_t)255 : 0;
     if (most * c.heads > 0x3FFFFFFFull) return fail(status, -2, "packed prefill attention: %zu blocks of %u heads exceed the index range", most, c.heads);
     const size_t entryBytes = (most * sizeof(Entry) + 255) & ~(size_t)255;
@@ -805,13 +1200,13 @@ static int tiles_launch(Context* ctx, const Call& c, CUDAStatus* status) {
         const size_t want = ((size_t)total + 7) / 8, cap = (size_t)ctx->smCount * 8;
         blocks += (unsigned)(want < cap ? want : cap);
     }
-    prologue_kernel<DT><<<blocks, 256, 0, ctx->stream>>>((const uint16_t*)c.q, (const uint16_t*)c.k, qRot, kRot, c.seqs, l, c.cosT, c.sinT, (int)c.heads,
+    prologue_kernel<DT><<<blocks, 256, 0, ctx->stream>>>((const uint16_t*)c.q, (const uint16_t*)c.k, qRot, kRot, c.seqs, l, c.cosT, c.sinT, fused ? 0 : (int)c.heads,
                                                          (int)c.kvHeads, (int)c.dim, c.ropeMode == 1);
     rc = check_launch(ctx, status, "packed prefill attention: work list and RoPE");
     if (rc != 0) return rc;
     TileParams p;
     memset(&p, 0, sizeof(p));
-    const void* q = c.ropeMode != 2 ? qRot : c.q;
+    const void* q = c.ropeMode != 2 && !fused ? qRot : c.q;
     const void* k = c.ropeMode != 2 ? kRot : c.k;
     const uint32_t pack = 1u << packLog;
     if (!make_map(&p.tmQ, q, BF16, total, c.heads, c.dim, pack, kRows >> packLog) || !make_map(&p.tmK, k, BF16, total, c.kvHeads, c.dim, 1, kKeys) ||
@@ -823,6 +1218,10 @@ static int tiles_launch(Context* ctx, const Call& c, CUDAStatus* status) {
     p.out = (uint16_t*)c.out;
     p.errorFlag = ctx->errorFlag;
     p.heads = (int)c.heads; p.kvHeads = (int)c.kvHeads; p.dim = (int)c.dim; p.causal = (int)c.causal;
+    p.cosT = fused ? c.cosT : nullptr;
+    p.sinT = c.sinT;
+    p.halves = c.ropeMode == 1;
+    p.posLast = c.seqs.maxLen - 1;
     p.packLog = packLog;
     p.headGroups = (int)(c.heads >> packLog);
     p.scaleLog2 = (float)(1.4426950408889634 / sqrt((double)c.dim));
@@ -891,6 +1290,7 @@ extern "C" int cuda_dispatch_rope_packed_attention_prefill(CUDADeviceRef context
         sinT = table + (size_t)maxSeqLen * (headDim / 2);
     }
     const pk::Call c{elementDType, q, k, v, out, seqs, numHeads, kvHeads, headDim, causal ? 1u : 0u, ropeMode, table, sinT};
+    if (pk::short_takes(ctx, c)) return elementDType == DT_BF16 ? pk::short_launch<true>(ctx, c, status) : pk::short_launch<false>(ctx, c, status);
     if (pk::tiles_take(c)) return elementDType == DT_BF16 ? pk::tiles_launch<true>(ctx, c, status) : pk::tiles_launch<false>(ctx, c, status);
     const int cap = ctx->smCount * 8;
     if (ropeMode != 2) {

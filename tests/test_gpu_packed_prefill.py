@@ -93,6 +93,35 @@ def check(got, q, k, v, starts, heads, kv, dim, fmt, causal, rope):
 RAGGED = [1, 0, 2, 31, 32, 33, 127, 128, 129, 0, 255, 256, 257, 300, 5]
 
 
+SHORT = [1, 0, 2, 31, 32, 33, 127, 128, 129, 0, 255, 256, 7, 15, 16, 17]
+
+
+@pytest.mark.parametrize("fmt", [2, 1])
+@pytest.mark.parametrize("longest", [17, 40, 128, 160])
+@pytest.mark.parametrize("heads,kv,dim", [(32, 8, 128), (8, 8, 64), (6, 2, 128), (16, 1, 64), (10, 2, 96), (28, 4, 128), (15, 5, 64), (2, 1, 8)])
+def test_calls_without_long_sequences(d, fmt, longest, heads, kv, dim):
+    """Few rows per KV head take the kernel for short sequences."""
+    lens = [n for n in SHORT if n <= longest]
+    q, k, v, starts = make(fmt, lens, heads, kv, dim, 7 * heads + dim, lead=3, tail=5)
+    for causal in (True, False):
+        got = call(d, q, k, v, starts, heads, kv, dim, fmt, causal=causal, longest=longest)
+        check(got, q, k, v, starts, heads, kv, dim, fmt, causal, None)
+    assert d.take_error() == 0
+
+
+@pytest.mark.parametrize("fmt", [2, 1])
+@pytest.mark.parametrize("mode", [0, 1])
+@pytest.mark.parametrize("dim", [128, 64])
+def test_rope_of_short_sequences(d, fmt, mode, dim):
+    import puter_b200
+
+    rope = puter_b200.RoPEConfig(BaseFreq=500000.0, Mode=mode, StartPosition=70)
+    q, k, v, starts = make(fmt, [1, 65, 0, 128, 33], 12, 4, dim, 5 + mode)
+    got = call(d, q, k, v, starts, 12, 4, dim, fmt, rope=rope, longest=128)
+    check(got, q, k, v, starts, 12, 4, dim, fmt, True, rope)
+    assert d.take_error() == 0
+
+
 @pytest.mark.parametrize("fmt", [2, 1])
 @pytest.mark.parametrize("heads,kv,dim", [(32, 8, 128), (8, 8, 128), (6, 2, 128), (16, 1, 128), (12, 12, 64), (28, 4, 64), (10, 2, 96), (4, 2, 80), (2, 1, 8)])
 def test_ragged_lengths_and_head_layouts(d, fmt, heads, kv, dim):
@@ -153,18 +182,19 @@ def test_many_sequences(d):
     assert d.take_error() == 0
 
 
+@pytest.mark.parametrize("longest", [None, 130])
 @pytest.mark.parametrize("dim", [128, 64])
-def test_rows_outside_every_sequence_stay_and_do_not_leak(d, dim):
+def test_rows_outside_every_sequence_stay_and_do_not_leak(d, dim, longest):
     """NaN and infinities before the first, behind the last and in the neighbouring sequence change nothing."""
     lens = [130, 7, 64, 129]
     q, k, v, starts = make(2, lens, 8, 2, dim, 21, lead=9, tail=200)
-    clean = call(d, q, k, v, starts, 8, 2, dim, 2)
+    clean = call(d, q, k, v, starts, 8, 2, dim, 2, longest=longest)
     check(clean, q, k, v, starts, 8, 2, dim, 2, True, None)
     for t in (q, k, v):
         t[:9] = float("nan")
         t[9 + sum(lens):] = float("inf")
         t[9 + 130:9 + 137] = float("nan")  # the whole second sequence
-    got = call(d, q, k, v, starts, 8, 2, dim, 2)
+    got = call(d, q, k, v, starts, 8, 2, dim, 2, longest=longest)
     keep = torch.ones(q.shape[0], dtype=torch.bool, device="cuda")
     keep[139:146] = False
     assert torch.equal(got[keep], clean[keep])
@@ -172,10 +202,12 @@ def test_rows_outside_every_sequence_stay_and_do_not_leak(d, dim):
     assert d.take_error() == 0
 
 
+@pytest.mark.parametrize("length", [290, 128])  # the tile kernel, the kernel for short sequences
 @pytest.mark.parametrize("at", [0, 60, 127, 128, 200])
-def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(d, at):
+def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(d, at, length):
     """A NaN key or value at position `at` leaves every earlier row of its own sequence as it was."""
-    q, k, v, starts = make(2, [290], 8, 2, 128, 31)
+    q, k, v, starts = make(2, [length], 8, 2, 128, 31)
+    at = min(at, length - 1)
     clean = call(d, q, k, v, starts, 8, 2, 128, 2)
     for t, x in ((k, float("nan")), (v, float("nan")), (v, float("inf"))):
         old = t[at].clone()
