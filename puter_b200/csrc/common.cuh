@@ -9,6 +9,7 @@
 #include <stdint.h>
 #include <string.h>
 #include <stdio.h>
+#include <atomic>
 
 #include "../../include/puter_b200.h"
 
@@ -102,6 +103,14 @@ inline size_t dtype_size(int dt) {
         case CUDAElementDTypeFloat8E5M2: return 1;
     }
     return 0;
+}
+
+// Lets KERNEL use `bytes` of dynamic shared memory, asking the runtime once per device (the call costs as much as a launch).
+template <auto KERNEL> inline void allow_smem(int device, int bytes) {
+    static std::atomic<unsigned long long> done{0};
+    const unsigned long long bit = device >= 0 && device < 64 ? 1ull << device : 0;
+    if (bit && (done.load(std::memory_order_relaxed) & bit)) return;
+    if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
 }
 
 #define PUTER_ENTER(ctxVar)                          \

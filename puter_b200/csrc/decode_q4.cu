@@ -1056,8 +1056,10 @@ static int launch(Context* ctx, Params& p, CUDAStatus* status) {
     }
     // PUTER_DECODE_NO_COOPERATIVE (any value) forces the plain launch: the path a refused cooperative launch takes, reachable for tests
     const bool cooperative = getenv("PUTER_DECODE_NO_COOPERATIVE") == nullptr;
-    const auto kernel = p.pageSize % kTile == 0 ? decode_kernel<DT, S, true> : decode_kernel<DT, S, false>;
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    const bool paged = p.pageSize % kTile == 0;
+    const auto kernel = paged ? decode_kernel<DT, S, true> : decode_kernel<DT, S, false>;
+    if (paged) allow_smem<decode_kernel<DT, S, true>>(ctx->device, S::SMEM);
+    else allow_smem<decode_kernel<DT, S, false>>(ctx->device, S::SMEM);
     p.together = 1;
     void* args[] = {&p};
     if (!cooperative || cudaLaunchCooperativeKernel((const void*)kernel, dim3(grid), dim3(S::WARPS * 32), args, S::SMEM, ctx->stream) != cudaSuccess) {

@@ -165,8 +165,15 @@ __device__ void suffix_sum(int* x, int n, bool exclusive) {
     }
 }
 
+constexpr int kListLevels = 2048;  // whose counts fit shared memory
+
 // Entries by level (block number within the sequence: what decides its number of keys), highest first; within a level in any order.
-__device__ void build_list(const Seqs& s, const Lists& l) {
+__device__ void build_list(const Seqs& s, Lists l) {
+    __shared__ int levels[2][kListLevels];
+    if (l.levels <= kListLevels) {  // the five passes then wait for the starts alone
+        l.above = levels[0];
+        l.cursor = levels[1];
+    }
     for (int i = threadIdx.x; i < l.levels; i += blockDim.x) l.above[i] = l.cursor[i] = 0;
     __syncthreads();
     for (int b = threadIdx.x; b < s.batch; b += blockDim.x) {
@@ -192,6 +199,36 @@ __device__ void build_list(const Seqs& s, const Lists& l) {
     }
 }
 
+// eight neighbouring elements rotated with their own pairs (interleaved) or with the eight `b` half a head further (halves)
+template <bool BF16>
+__device__ __forceinline__ void rotate8(Vec16& a, Vec16& b, const float* cosRow, const float* sinRow, bool halves) {
+    constexpr int DT = BF16 ? DT_BF16 : DT_F16;
+    if (halves) {
+        float cs[8], sn[8];
+        *(float4*)cs = __ldg((const float4*)cosRow);
+        *(float4*)(cs + 4) = __ldg((const float4*)(cosRow + 4));
+        *(float4*)sn = __ldg((const float4*)sinRow);
+        *(float4*)(sn + 4) = __ldg((const float4*)(sinRow + 4));
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            float e0, e1, o0, o1;
+            unpack16_arith<DT>(a.w[w], e0, e1);
+            unpack16_arith<DT>(b.w[w], o0, o1);
+            a.w[w] = pack16_arith<DT>(sub(mul(e0, cs[2 * w]), mul(o0, sn[2 * w])), sub(mul(e1, cs[2 * w + 1]), mul(o1, sn[2 * w + 1])));
+            b.w[w] = pack16_arith<DT>(add(mul(e0, sn[2 * w]), mul(o0, cs[2 * w])), add(mul(e1, sn[2 * w + 1]), mul(o1, cs[2 * w + 1])));
+        }
+    } else {
+        const float4 c = __ldg((const float4*)cosRow), n = __ldg((const float4*)sinRow);
+        const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {n.x, n.y, n.z, n.w};
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            float e, o;
+            unpack16_arith<DT>(a.w[w], e, o);
+            a.w[w] = pack16_arith<DT>(sub(mul(e, cs[w]), mul(o, sn[w])), add(mul(e, sn[w]), mul(o, cs[w])));
+        }
+    }
+}
+
 // Rotates [total, qHeads + kHeads, D] (two tensors, one row of both at a time, a warp per row) with 16-byte vectors.
 template <int DT>
 __global__ void __launch_bounds__(256) prologue_kernel(const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, uint16_t* __restrict__ qOut,
@@ -204,40 +241,37 @@ __global__ void __launch_bounds__(256) prologue_kernel(const uint16_t* __restric
     const int lane = threadIdx.x & 31, half = dim / 2, perHead = halfMode ? half / 8 : dim / 8;  // vectors, or pairs of vectors
     const int items = (qHeads + kHeads) * perHead;
     for (int row = (blockIdx.x - 1) * 8 + (threadIdx.x >> 5); row < s.total; row += (gridDim.x - 1) * 8) {
-        int s0, s1;
-        if (!seq_rows(s, seq_of(s, row), s0, s1) || row < s0 || row >= s1) continue;
-        const float* cr = cosT + (size_t)(row - s0) * half;
-        const float* sr = sinT + (size_t)(row - s0) * half;
-        for (int it = lane; it < items; it += 32) {
-            const int head = it / perHead, j = it - head * perHead;
-            const uint16_t* src = head < qHeads ? q + ((size_t)row * qHeads + head) * dim : k + ((size_t)row * kHeads + head - qHeads) * dim;
-            uint16_t* dst = head < qHeads ? qOut + ((size_t)row * qHeads + head) * dim : kOut + ((size_t)row * kHeads + head - qHeads) * dim;
-            if (halfMode) {
-                Vec16 a = ld_stream(src + 8 * j), b = ld_stream(src + half + 8 * j);
-                const float4 c0 = __ldg((const float4*)(cr + 8 * j)), c1 = __ldg((const float4*)(cr + 8 * j + 4));
-                const float4 n0 = __ldg((const float4*)(sr + 8 * j)), n1 = __ldg((const float4*)(sr + 8 * j + 4));
-                const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, sn[8] = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, n1.z, n1.w};
+        // two items of a lane are on their way before the search for the row's sequence, which is a chain of loads of its own
+        constexpr int U = 2;
+        int s0 = 0;
+        for (int it0 = lane; it0 < items; it0 += 32 * U) {
+            Vec16 a[U], b[U];
+            uint16_t* dst[U];
+            int j[U];
 #pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    float e0, e1, o0, o1;
-                    unpack16_arith<DT>(a.w[w], e0, e1);
-                    unpack16_arith<DT>(b.w[w], o0, o1);
-                    a.w[w] = pack16_arith<DT>(sub(mul(e0, cs[2 * w]), mul(o0, sn[2 * w])), sub(mul(e1, cs[2 * w + 1]), mul(o1, sn[2 * w + 1])));
-                    b.w[w] = pack16_arith<DT>(add(mul(e0, sn[2 * w]), mul(o0, cs[2 * w])), add(mul(e1, sn[2 * w + 1]), mul(o1, cs[2 * w + 1])));
-                }
-                *(Vec16*)(dst + 8 * j) = a;
-                *(Vec16*)(dst + half + 8 * j) = b;
-            } else {
-                Vec16 a = ld_stream(src + 8 * j);
-                const float4 c = __ldg((const float4*)(cr + 4 * j)), n = __ldg((const float4*)(sr + 4 * j));
-                const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {n.x, n.y, n.z, n.w};
+            for (int u = 0; u < U; u++) {
+                const int it = min(it0 + 32 * u, items - 1), head = it / perHead;
+                j[u] = it - head * perHead;
+                const bool ofQ = head < qHeads;
+                const size_t at = ofQ ? ((size_t)row * qHeads + head) * dim : ((size_t)row * kHeads + head - qHeads) * dim;
+                const uint16_t* src = (ofQ ? q : k) + at;
+                dst[u] = (ofQ ? qOut : kOut) + at;
+                a[u] = ld_stream(src + 8 * j[u]);
+                if (halfMode) b[u] = ld_stream(src + half + 8 * j[u]);
+            }
+            if (it0 == lane) {
+                int s1;
+                if (!seq_rows(s, seq_of(s, row), s0, s1) || row < s0 || row >= s1) break;  // uniform over the warp
+            }
+            const float* cr = cosT + (size_t)(row - s0) * half;
+            const float* sr = sinT + (size_t)(row - s0) * half;
 #pragma unroll
-                for (int w = 0; w < 4; w++) {
-                    float e, o;
-                    unpack16_arith<DT>(a.w[w], e, o);
-                    a.w[w] = pack16_arith<DT>(sub(mul(e, cs[w]), mul(o, sn[w])), add(mul(e, sn[w]), mul(o, cs[w])));
-                }
-                *(Vec16*)(dst + 8 * j) = a;
+            for (int u = 0; u < U; u++) {
+                if (it0 + 32 * u >= items) break;
+                const int c = (halfMode ? 8 : 4) * j[u];
+                rotate8<DT == DT_BF16>(a[u], b[u], cr + c, sr + c, halfMode != 0);
+                *(Vec16*)(dst[u] + 8 * j[u]) = a[u];
+                if (halfMode) *(Vec16*)(dst[u] + half + 8 * j[u]) = b[u];
             }
         }
     }
@@ -850,36 +884,6 @@ __device__ __forceinline__ void ldmatrix_trans(uint32_t at, uint32_t* r) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
 
-// eight neighbouring elements rotated with their own pairs (interleaved) or with the eight `b` half a head further (halves)
-template <bool BF16>
-__device__ __forceinline__ void rotate8(Vec16& a, Vec16& b, const float* cosRow, const float* sinRow, bool halves) {
-    constexpr int DT = BF16 ? DT_BF16 : DT_F16;
-    if (halves) {
-        float cs[8], sn[8];
-        *(float4*)cs = __ldg((const float4*)cosRow);
-        *(float4*)(cs + 4) = __ldg((const float4*)(cosRow + 4));
-        *(float4*)sn = __ldg((const float4*)sinRow);
-        *(float4*)(sn + 4) = __ldg((const float4*)(sinRow + 4));
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-            float e0, e1, o0, o1;
-            unpack16_arith<DT>(a.w[w], e0, e1);
-            unpack16_arith<DT>(b.w[w], o0, o1);
-            a.w[w] = pack16_arith<DT>(sub(mul(e0, cs[2 * w]), mul(o0, sn[2 * w])), sub(mul(e1, cs[2 * w + 1]), mul(o1, sn[2 * w + 1])));
-            b.w[w] = pack16_arith<DT>(add(mul(e0, sn[2 * w]), mul(o0, cs[2 * w])), add(mul(e1, sn[2 * w + 1]), mul(o1, cs[2 * w + 1])));
-        }
-    } else {
-        const float4 c = __ldg((const float4*)cosRow), n = __ldg((const float4*)sinRow);
-        const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {n.x, n.y, n.z, n.w};
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-            float e, o;
-            unpack16_arith<DT>(a.w[w], e, o);
-            a.w[w] = pack16_arith<DT>(sub(mul(e, cs[w]), mul(o, sn[w])), add(mul(e, sn[w]), mul(o, cs[w])));
-        }
-    }
-}
-
 struct ShortParams {
     const uint16_t *q, *k, *v;
     uint16_t* out;
@@ -1159,7 +1163,7 @@ static int short_launch(Context* ctx, const Call& c, CUDAStatus* status) {
     const dim3 grid((unsigned)c.seqs.batch, c.kvHeads, (unsigned)split);
 #define SHORT(D)                                                                                                                        \
     do {                                                                                                                                \
-        cudaFuncSetAttribute(short_kernel<BF16, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);                            \
+        allow_smem<short_kernel<BF16, D>>(ctx->device, kShortMax * D * 4);                                                              \
         short_kernel<BF16, D><<<grid, kShortWarps * 32, smem, ctx->stream>>>(p);                                                        \
     } while (0)
     if (D == 128) SHORT(128);
@@ -1227,9 +1231,10 @@ static int tiles_launch(Context* ctx, const Call& c, CUDAStatus* status) {
     p.scaleLog2 = (float)(1.4426950408889634 / sqrt((double)c.dim));
     const size_t items = most * p.headGroups;
     const unsigned grid = items < (size_t)ctx->smCount ? (unsigned)items : (unsigned)ctx->smCount;  // persistent: one CTA per SM
+    // (started early, beside the launch before it, this kernel cost 10 of 305 us: its blocks need an SM each and wait for the other's to drain)
 #define TILES(NB)                                                                                                                      \
     do {                                                                                                                               \
-        cudaFuncSetAttribute(tiles_kernel<BF16, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Smem<NB>::TOTAL);               \
+        allow_smem<tiles_kernel<BF16, NB>>(ctx->device, (int)Smem<NB>::TOTAL);                                                         \
         tiles_kernel<BF16, NB><<<grid, kThreads, Smem<NB>::TOTAL, ctx->stream>>>(p);                                                   \
     } while (0)
     if (c.dim > 64) TILES(2);

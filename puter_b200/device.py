@@ -153,7 +153,12 @@ class Device:
             for old in self._refs.values():
                 self.lib.cuda_buffer_release(old)
             self._refs.clear()
-        args = build_args([self._ref(t) for t in tensors])
+        # a handle that is there was made of CUDA memory; whether this view of it is contiguous is asked every time
+        known, refs = self._refs, []
+        for t in tensors:
+            r = known.get((t.data_ptr(), t.nbytes)) if t is not None and t.is_contiguous() else None
+            refs.append(r if r is not None else self._ref(t))
+        args = build_args(refs)
         rc = getattr(self.lib, name)(self.ref, *args, ctypes.byref(self._status))
         self._check(rc)
 
