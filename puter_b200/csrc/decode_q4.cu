@@ -27,7 +27,10 @@
 //   * The weights p_t * step_t enter as f16, relative to a running power of two about the largest step, which joins the running maximum of
 //     the softmax in rescaling the accumulator.  Their rounding (half a step of 2^-11) multiplies codes of 0 .. 15, more than the
 //     values themselves amount to: 2^-10 of the output, measured, unseen in a bf16 output and five times the rounding of an f16 one.  For
-//     f16 the weights therefore come in two parts, the second in the unused columns (QUAD, free) or in products of its own.
+//     f16 the weights therefore come in two parts, the second in the unused columns (QUAD, free) or in products of its own, and V
+//     enters as n - 8, one more 16-bit subtraction per operand: sums of n itself are far larger than what is left of them once
+//     sum(p_t least_t) joins them, and the matrix unit cuts its sums off (100001 tokens, 16 heads: error 1.2e-3 of the output with
+//     n, 2.1e-4, the rounding of the output, with n - 8; 46 -> 48 us).
 // Sums, maxima and accumulators are float32.
 //
 // Work: the tiles of 16 tokens of all (KV head, sequence) pairs in one list, cut into equal contiguous ranges, one per CTA, and each
@@ -125,6 +128,14 @@ __device__ __forceinline__ void imma0(int* c, uint32_t a0, uint32_t a1, uint32_t
         : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
+// low and high four bits of the lower byte of each half, less 8, as f16: 1024 + n and 64 + n are one logic instruction away
+__device__ __forceinline__ uint32_t sub16(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t low8(uint32_t x) { return sub16((x & 0x000F000Fu) | 0x64006400u, 0x64086408u); }
+__device__ __forceinline__ uint32_t high8(uint32_t x) { return sub16((x & 0x00F000F0u) | 0x54005400u, 0x54805480u); }
 // lowest signed byte of v; v is left with the rest: v = rest * 256 + byte
 __device__ __forceinline__ uint32_t limb(int& v) {
     const int b = (int)(int8_t)v;
@@ -727,7 +738,10 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
                     exponentials();
                 }
 #pragma unroll
-                for (int i = 0; i < 2 * MT; i++) vs[i] *= veInv;
+                for (int i = 0; i < 2 * MT; i++) {
+                    if (SPLIT) vl[i] = fmaf(8.f, vs[i], vl[i]);
+                    vs[i] *= veInv;
+                }
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -771,13 +785,20 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
                         for (int half = 0; half < 2; half++) {
                             const uint32_t x = __byte_perm(va[w], vb[w], half ? 0x7632 : 0x5410), y = __byte_perm(vc[w], vd[w], half ? 0x7632 : 0x5410);
                             const uint32_t x8 = __byte_perm(x, 0, 0x4341), y8 = __byte_perm(y, 0, 0x4341);
+                            uint32_t a[2][4];  // dimensions 0 and 1, 2 and 3 of the word: even and whole byte, or even - 8 and odd - 8
+                            if (SPLIT) {
+                                a[0][0] = low8(x); a[0][1] = high8(x); a[0][2] = low8(y); a[0][3] = high8(y);
+                                a[1][0] = low8(x8); a[1][1] = high8(x8); a[1][2] = low8(y8); a[1][3] = high8(y8);
+                            } else {
+                                a[0][0] = x & 0x000F000Fu; a[0][1] = x & 0x00FF00FFu; a[0][2] = y & 0x000F000Fu; a[0][3] = y & 0x00FF00FFu;
+                                a[1][0] = x8 & 0x000F000Fu; a[1][1] = x8; a[1][2] = y8 & 0x000F000Fu; a[1][3] = y8;
+                            }
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) {
-                                mma(o[w][2 * half][nt], x & 0x000F000Fu, x & 0x00FF00FFu, y & 0x000F000Fu, y & 0x00FF00FFu, pb[nt][0], pb[nt][1]);
-                                mma(o[w][2 * half + 1][nt], x8 & 0x000F000Fu, x8, y8 & 0x000F000Fu, y8, pb[nt][0], pb[nt][1]);
-                                if (SPLIT && !QUAD) {
-                                    mma(o[w][2 * half][nt], x & 0x000F000Fu, x & 0x00FF00FFu, y & 0x000F000Fu, y & 0x00FF00FFu, pr[nt][0], pr[nt][1]);
-                                    mma(o[w][2 * half + 1][nt], x8 & 0x000F000Fu, x8, y8 & 0x000F000Fu, y8, pr[nt][0], pr[nt][1]);
+#pragma unroll
+                                for (int i = 0; i < 2; i++) {
+                                    mma(o[w][2 * half + i][nt], a[i][0], a[i][1], a[i][2], a[i][3], pb[nt][0], pb[nt][1]);
+                                    if (SPLIT && !QUAD) mma(o[w][2 * half + i][nt], a[i][0], a[i][1], a[i][2], a[i][3], pr[nt][0], pr[nt][1]);
                                 }
                             }
                         }
@@ -817,8 +838,8 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
                                 even += o[w][i][nt][1];
                                 both += o[w][i][nt][3];
                             }
-                            x[8 * w + 2 * i] = fmaf(even * 16777216.f, veUp, least);
-                            x[8 * w + 2 * i + 1] = fmaf((both - even) * 1048576.f, veUp, least);
+                            x[8 * w + 2 * i] = fmaf(SPLIT ? even : even * 16777216.f, veUp, least);
+                            x[8 * w + 2 * i + 1] = fmaf(SPLIT ? both : (both - even) * 1048576.f, veUp, least);
                         }
                     if (whole) {
                         uint16_t* dst = p.out + ((size_t)b * p.numHeads + head0 + h) * D + g * (D / 8);
