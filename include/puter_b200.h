@@ -413,7 +413,7 @@ int cuda_dispatch_paged_decode_attention_q4(CUDADeviceRef contextRef, int elemen
    Per sequence as cuda_dispatch_rope_attention_prefill: positions startPosition .. restart with every sequence, causal or not,
    ropeMode 2 = inputs already rotated.  float32, f16, bf16; headDim <= 256.  Rows of no sequence are left as they were.  A pair of starts
    that is no range of the packed rows, or is longer than maxSeqLen, is skipped and raises the error flag (1); where the starts are
-   not non-decreasing the other rows of the call are not valid either.  out may not be one of the inputs. */
+   not non-decreasing the other rows of the call are not valid either.  out may not overlap an input. */
 int cuda_dispatch_rope_packed_attention_prefill(CUDADeviceRef contextRef, int elementDType, CUDABufferRef queryRef, CUDABufferRef keyRef,
                                                 CUDABufferRef valueRef, CUDABufferRef seqStartsRef, CUDABufferRef outRef, uint32_t batch,
                                                 uint32_t totalTokens, uint32_t maxSeqLen, uint32_t numHeads, uint32_t kvHeads,

@@ -31,6 +31,7 @@ struct RopeTable {
     size_t bytes;
     double key[10];
     int valid, pinned;
+    cudaEvent_t built;
     unsigned long long used;
     RopeTable* next;
 };
@@ -111,6 +112,17 @@ template <auto KERNEL> inline void allow_smem(int device, int bytes) {
     const unsigned long long bit = device >= 0 && device < 64 ? 1ull << device : 0;
     if (bit && (done.load(std::memory_order_relaxed) & bit)) return;
     if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+}
+
+// vectors of a paged pool; ~0 where the product leaves 64 bits
+constexpr size_t kMostVectors = (size_t)1 << 48;
+inline size_t pool_vectors(uint32_t pageCount, uint32_t pageSize, uint32_t kvHeads) {
+    const size_t perHead = (size_t)pageCount * pageSize;
+    return perHead > kMostVectors / kvHeads ? ~(size_t)0 : perHead * kvHeads;
+}
+
+inline bool overlap(const void* a, size_t aBytes, const void* b, size_t bBytes) {
+    return (uintptr_t)a < (uintptr_t)b + bBytes && (uintptr_t)b < (uintptr_t)a + aBytes;
 }
 
 #define PUTER_ENTER(ctxVar)                          \

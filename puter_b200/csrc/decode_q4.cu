@@ -1055,7 +1055,6 @@ static int launch(Context* ctx, Params& p, CUDAStatus* status) {
     const unsigned grid = (unsigned)ctx->smCount;
     p.blocks = (p.group + S::HEADS - 1) / S::HEADS;
     p.units = p.kvHeads * p.blocks;
-    if ((long long)p.units * p.batch > 0x7FFFFFFFll) return fail(status, -2, "%s: batch times heads exceeds 31 bits", what);
     const size_t slots = (size_t)grid * (S::WARPS + 2);
     const size_t accBytes = slots * S::HEADS * S::D * 4, mlBytes = slots * S::HEADS * 8;
     const size_t prefixBytes = p.batch > kPrefixSmem ? ((size_t)p.batch + 2) * 4 : 0;
@@ -1113,7 +1112,8 @@ extern "C" int cuda_dispatch_paged_decode_attention_q4(CUDADeviceRef contextRef,
         return fail(status, -6, "%s: supported are bf16 / f16 queries and head dimensions 64 and 128 (got dtype %d, head dimension %u)", what,
                     elementDType, headDim);
     if (pageSize == 0 || pageCount == 0 || maxPagesPerSeq == 0) return fail(status, -2, "%s: empty page geometry", what);
-    const size_t slots = (size_t)pageCount * pageSize * kvHeads;
+    if ((size_t)batch * numHeads > 0x7FFFFFFFull) return fail(status, -2, "%s: %u sequences of %u heads exceed 31 bits", what, batch, numHeads);
+    const size_t slots = pool_vectors(pageCount, pageSize, kvHeads);
     if (slots > 0xFFFFFFFFull || (size_t)maxPagesPerSeq * pageSize > 0x7FFFFFE0ull || batch > 0x7FFFFFFEu)
         return fail(status, -2, "%s: a pool of %zu vectors or a context of %zu tokens exceeds the index range", what, slots,
                     (size_t)maxPagesPerSeq * pageSize);
@@ -1133,6 +1133,8 @@ extern "C" int cuda_dispatch_paged_decode_attention_q4(CUDADeviceRef contextRef,
     if ((((uintptr_t)dev_ptr(kCodesRef) | (uintptr_t)dev_ptr(vCodesRef) | (uintptr_t)dev_ptr(kParamsRef) | (uintptr_t)dev_ptr(vParamsRef) |
           (uintptr_t)dev_ptr(queryRef) | (uintptr_t)dev_ptr(outRef)) & 15u) != 0)
         return fail(status, -2, "%s: pools, query and output must be 16-byte aligned", what);
+    if ((((uintptr_t)dev_ptr(pageTableRef) | (uintptr_t)dev_ptr(ctxLensRef) | (uintptr_t)flag) & 3u) != 0)
+        return fail(status, -2, "%s: pageTable, ctxLens and errorFlag must be 4-byte aligned", what);
     q4d::Params p{};
     p.q = (const uint16_t*)dev_ptr(queryRef);
     p.kCodes = (const uint8_t*)dev_ptr(kCodesRef);

@@ -22,8 +22,8 @@ namespace puter {
 
 int validate_rope(CUDAStatus* status, double base, uint32_t halfMode, uint32_t scaling, double factor, double low, double high,
                   uint32_t origCtx);
-const float* cached_rope_table(Context* ctx, size_t seqLen, int headDim, double base, long long startPos, int scaling, double factor,
-                               double low, double high, int origCtx, CUDAStatus* status);
+const float* cached_rope_table_at_least(Context* ctx, size_t positions, int headDim, double base, long long startPos, int scaling,
+                                        double factor, double low, double high, int origCtx, const float** sinT, CUDAStatus* status);
 
 namespace q4 {
 
@@ -282,7 +282,9 @@ extern "C" int cuda_dispatch_rope_kv_page_write_q4(CUDADeviceRef contextRef, int
         if (maxPositions == 0) return fail(status, -2, "rope kv page write (4 bits): maxPositions must be positive");
         PUTER_REQUIRE(positionsRef, "positions", (size_t)rows * 4);
     }
-    const size_t inner = (size_t)kvHeads * headDim, slots = (size_t)pageCount * pageSize * kvHeads;
+    if ((size_t)rows * kvHeads > 0xFFFFFFFFull) return fail(status, -2, "rope kv page write (4 bits): %u rows of %u heads exceed 32 bits", rows, kvHeads);
+    const size_t inner = (size_t)kvHeads * headDim, slots = pool_vectors(pageCount, pageSize, kvHeads);
+    if (slots > kMostVectors) return fail(status, -2, "rope kv page write (4 bits): %u pages of %u tokens and %u heads", pageCount, pageSize, kvHeads);
     PUTER_REQUIRE(kRef, "k", (size_t)rows * inner * 2);
     PUTER_REQUIRE(vRef, "v", (size_t)rows * inner * 2);
     PUTER_REQUIRE(pageIDsRef, "pageIDs", (size_t)rows * 4);
@@ -294,14 +296,14 @@ extern "C" int cuda_dispatch_rope_kv_page_write_q4(CUDADeviceRef contextRef, int
     if ((((uintptr_t)dev_ptr(kRef) | (uintptr_t)dev_ptr(vRef) | (uintptr_t)dev_ptr(kCodesRef) | (uintptr_t)dev_ptr(vCodesRef) |
           (uintptr_t)dev_ptr(kParamsRef) | (uintptr_t)dev_ptr(vParamsRef)) & 15u) != 0)
         return fail(status, -2, "rope kv page write (4 bits): buffers must be 16-byte aligned");
-    const float* table = nullptr;
+    if ((((uintptr_t)(ropeMode == 2 ? nullptr : dev_ptr(positionsRef)) | (uintptr_t)dev_ptr(pageIDsRef) | (uintptr_t)dev_ptr(offsetsRef)) & 3u) != 0)
+        return fail(status, -2, "rope kv page write (4 bits): positions, pageIDs and offsets must be 4-byte aligned");
+    const float *table = nullptr, *sinT = nullptr;
     if (ropeMode != 2) {
-        table = cached_rope_table(ctx, maxPositions, (int)headDim, baseFreq, 0, (int)scaling, scalingFactor, lowFreqFactor, highFreqFactor,
-                                  (int)originalContext, status);
+        table = cached_rope_table_at_least(ctx, maxPositions, (int)headDim, baseFreq, 0, (int)scaling, scalingFactor, lowFreqFactor, highFreqFactor,
+                                           (int)originalContext, &sinT, status);
         if (!table) return status ? status->code : -7;
     }
-    const float* sinT = table ? table + (size_t)maxPositions * (headDim / 2) : nullptr;
-    if ((size_t)rows * kvHeads > 0xFFFFFFFFull) return fail(status, -2, "rope kv page write (4 bits): %u rows of %u heads exceed 32 bits", rows, kvHeads);
     const uint32_t vectors = rows * kvHeads;
     const int grid = q4::grid_of(ctx, (size_t)vectors * headDim / 512);
 #define APPEND_LAUNCH(DT, D, MODE)                                                                                                  \
@@ -337,14 +339,16 @@ extern "C" int cuda_dispatch_kv_page_gather_q4(CUDADeviceRef contextRef, int ele
     if (pageCount == 0 || pageSize == 0 || kvHeads == 0 || outRows == 0) return ok(status);
     if (elementDType != DT_F16 && elementDType != DT_BF16) return fail(status, -6, "page gather (4 bits): unsupported dtype %d", elementDType);
     if (headDim != 64 && headDim != 128) return fail(status, -6, "page gather (4 bits): head dimension %u is not 64 or 128", headDim);
-    const size_t slots = (size_t)pageCount * pageSize * kvHeads;
+    if ((size_t)outRows * kvHeads > 0xFFFFFFFFull) return fail(status, -2, "page gather (4 bits): %u rows of %u heads exceed 32 bits", outRows, kvHeads);
+    const size_t slots = pool_vectors(pageCount, pageSize, kvHeads);
+    if (slots > kMostVectors) return fail(status, -2, "page gather (4 bits): %u pages of %u tokens and %u heads", pageCount, pageSize, kvHeads);
     PUTER_REQUIRE(codesRef, "codes", slots * (headDim / 2));
     PUTER_REQUIRE(paramsRef, "params", slots * 4);
     PUTER_REQUIRE(pageTableRef, "pageTable", (((size_t)outRows + pageSize - 1) / pageSize) * 4);
     PUTER_REQUIRE(outputRef, "output", (size_t)outRows * kvHeads * headDim * 2);
     if ((((uintptr_t)dev_ptr(codesRef) | (uintptr_t)dev_ptr(paramsRef) | (uintptr_t)dev_ptr(outputRef)) & 15u) != 0)
         return fail(status, -2, "page gather (4 bits): buffers must be 16-byte aligned");
-    if ((size_t)outRows * kvHeads > 0xFFFFFFFFull) return fail(status, -2, "page gather (4 bits): %u rows of %u heads exceed 32 bits", outRows, kvHeads);
+    if (((uintptr_t)dev_ptr(pageTableRef) & 3u) != 0) return fail(status, -2, "page gather (4 bits): pageTable must be 4-byte aligned");
     const uint32_t vectors = outRows * kvHeads;
     const int grid = q4::grid_of(ctx, (size_t)vectors * headDim / 512);
     const bool wide = ((uintptr_t)dev_ptr(outputRef) & 31u) == 0;

@@ -30,8 +30,8 @@ namespace puter {
 
 int validate_rope(CUDAStatus* status, double base, uint32_t halfMode, uint32_t scaling, double factor, double low, double high,
                   uint32_t origCtx);
-const float* cached_rope_table(Context* ctx, size_t seqLen, int headDim, double base, long long startPos, int scaling, double factor,
-                               double low, double high, int origCtx, CUDAStatus* status);
+const float* cached_rope_table_at_least(Context* ctx, size_t positions, int headDim, double base, long long startPos, int scaling,
+                                        double factor, double low, double high, int origCtx, const float** sinT, CUDAStatus* status);
 
 namespace pk {
 
@@ -1274,6 +1274,7 @@ extern "C" int cuda_dispatch_rope_packed_attention_prefill(CUDADeviceRef context
         if (headDim % 2 != 0) return fail(status, -2, "rope: head dimension must be even");
     }
     if (maxSeqLen > totalTokens) maxSeqLen = totalTokens;
+    if ((size_t)totalTokens * numHeads > (size_t)1 << 48) return fail(status, -2, "%s: %u tokens of %u heads", what, totalTokens, numHeads);
     const size_t es = dtype_size(elementDType), qBytes = (size_t)totalTokens * numHeads * headDim * es,
                  kvBytes = (size_t)totalTokens * kvHeads * headDim * es;
     PUTER_REQUIRE(queryRef, "query", qBytes);
@@ -1285,14 +1286,16 @@ extern "C" int cuda_dispatch_rope_packed_attention_prefill(CUDADeviceRef context
     const void* k = dev_ptr(keyRef);
     const void* v = dev_ptr(valueRef);
     void* out = dev_ptr(outRef);
-    if (out == q || out == k || out == v) return fail(status, -2, "%s: out may not be an input", what);
+    if (overlap(out, qBytes, q, qBytes) || overlap(out, qBytes, k, kvBytes) || overlap(out, qBytes, v, kvBytes))
+        return fail(status, -2, "%s: out may not overlap an input", what);
+    if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & (es - 1)) != 0 || ((uintptr_t)dev_ptr(seqStartsRef) & 3u) != 0)
+        return fail(status, -2, "%s: a buffer is not aligned to its elements", what);
     const pk::Seqs seqs{(const int32_t*)dev_ptr(seqStartsRef), (int)batch, (int)totalTokens, (int)maxSeqLen, ctx->errorFlag};
     const float *table = nullptr, *sinT = nullptr;
     if (ropeMode != 2) {
-        table = cached_rope_table(ctx, maxSeqLen, (int)headDim, baseFreq, (long long)startPosition, (int)scaling, scalingFactor,
-                                               lowFreqFactor, highFreqFactor, (int)originalContext, status);
+        table = cached_rope_table_at_least(ctx, maxSeqLen, (int)headDim, baseFreq, (long long)startPosition, (int)scaling, scalingFactor,
+                                           lowFreqFactor, highFreqFactor, (int)originalContext, &sinT, status);
         if (!table) return status ? status->code : -7;
-        sinT = table + (size_t)maxSeqLen * (headDim / 2);
     }
     const pk::Call c{elementDType, q, k, v, out, seqs, numHeads, kvHeads, headDim, causal ? 1u : 0u, ropeMode, table, sinT};
     if (pk::short_takes(ctx, c)) return elementDType == DT_BF16 ? pk::short_launch<true>(ctx, c, status) : pk::short_launch<false>(ctx, c, status);

@@ -438,59 +438,121 @@ int build_rope_table(Context* ctx, float* table, size_t seqLen, int headDim, dou
 // number of positions) that is not among the last few.  A decoder applies the same RoPE to q and k of every layer, so the
 // float64 angle evaluation runs once per configuration instead of once per call; several tables are kept because a layer may
 // alternate between two (prefill over its own length, cache writes over the whole range of positions).
-// A captured launch keeps the pointer: its table is pinned, and a table that is missing during a capture is refused, since
-// building it there would only record the work.
-static constexpr int kRopeTables = 4;  // unpinned tables kept
+// A captured launch keeps the pointer: its table is finished before the capture goes on (a replay may run on a stream that knows
+// nothing of the one it was built on), never overwritten, and kept until the context closes.
+static constexpr int kRopeTables = 4;  // tables that no captured launch reads, kept at a time
 
-const float* cached_rope_table(Context* ctx, size_t seqLen, int headDim, double base, long long startPos, int scaling, double factor,
-                               double low, double high, int origCtx, CUDAStatus* status) {
-    const double key[10] = {(double)seqLen, (double)headDim, base, (double)startPos, (double)scaling, scaling ? factor : 0.0,
-                            scaling ? low : 0.0, scaling ? high : 0.0, scaling ? (double)origCtx : 0.0, 0.0};
-    const size_t need = seqLen * (size_t)(headDim / 2) * 2 * sizeof(float);
+// Work that is not to be recorded while the context's stream is being captured.
+struct OutsideCapture {
+    Context* ctx;
+    cudaStream_t stream;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    explicit OutsideCapture(Context* c) : ctx(c), stream(c->stream) {
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        ctx->stream = ctx->uploadStream;
+    }
+    ~OutsideCapture() {
+        ctx->stream = stream;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+    }
+};
+
+// exact: the table must have seqLen positions, its sines lying behind them; otherwise a longer one serves too
+static const RopeTable* rope_table(Context* ctx, size_t seqLen, bool exact, int headDim, double base, long long startPos, int scaling,
+                                   double factor, double low, double high, int origCtx, CUDAStatus* status) {
+    double key[10] = {(double)seqLen, (double)headDim, base, (double)startPos, (double)scaling, scaling ? factor : 0.0,
+                      scaling ? low : 0.0, scaling ? high : 0.0, scaling ? (double)origCtx : 0.0, 0.0};
     const bool capturing = stream_capturing(ctx, nullptr);
     RopeTable* oldest = nullptr;
     int unpinned = 0;
     for (RopeTable* t = ctx->ropeTables; t; t = t->next) {
-        if (t->valid && memcmp(key, t->key, sizeof(key)) == 0) {
+        if (t->valid && memcmp(key + 1, t->key + 1, sizeof(key) - sizeof(key[0])) == 0 && (exact ? t->key[0] == key[0] : t->key[0] >= key[0])) {
             t->used = ++ctx->ropeClock;
-            if (capturing) t->pinned = 1;
-            return t->data;
+            if (capturing && !t->pinned) {
+                OutsideCapture now(ctx);
+                if (cudaEventSynchronize(t->built) != cudaSuccess) {
+                    fail(status, -7, "rope: waiting for the table failed: %s", cudaGetErrorString(cudaGetLastError()));
+                    return nullptr;
+                }
+                t->pinned = 1;
+            }
+            return t;
         }
         if (!t->pinned) {
             unpinned++;
             if (!oldest || t->used < oldest->used) oldest = t;
         }
     }
-    if (capturing) {
-        fail(status, -2, "rope: no cos / sin table for this configuration yet: make one call with it before the capture");
-        return nullptr;
+    if (!exact) {  // to the next power of two, so that calls of all lengths share a few
+        size_t up = 64;
+        while (up < seqLen) up *= 2;
+        seqLen = up;
+        key[0] = (double)up;
     }
-    RopeTable* t = unpinned >= kRopeTables ? oldest : nullptr;
+    const size_t need = seqLen * (size_t)(headDim / 2) * 2 * sizeof(float);
+    RopeTable* t = unpinned >= kRopeTables && !capturing ? oldest : nullptr;
     if (!t) {
         t = new RopeTable();
+        if (cudaEventCreateWithFlags(&t->built, cudaEventDisableTiming) != cudaSuccess) {
+            delete t;
+            fail(status, -7, "rope: event creation failed: %s", cudaGetErrorString(cudaGetLastError()));
+            return nullptr;
+        }
         t->next = ctx->ropeTables;
         ctx->ropeTables = t;
     }
     t->valid = 0;
-    if (t->bytes < need) {
-        if (t->data) {
-            cudaStreamSynchronize(ctx->stream);  // earlier launches may still read the old table
-            cudaFree(t->data);
-            t->data = nullptr;
-            t->bytes = 0;
-        }
-        if (cudaMalloc((void**)&t->data, need) != cudaSuccess) {
-            cudaGetLastError();
-            t->data = nullptr;
-            fail(status, -7, "rope: table allocation of %zu bytes failed", need);
-            return nullptr;
-        }
-        t->bytes = need;
+    if (t->bytes < need && t->data) {
+        cudaStreamSynchronize(ctx->stream);  // earlier launches may still read the old table
+        cudaFree(t->data);
+        t->data = nullptr;
+        t->bytes = 0;
     }
-    if (build_rope_table(ctx, t->data, seqLen, headDim, base, startPos, scaling, factor, low, high, origCtx, status) != 0) return nullptr;
+    auto fill = [&]() {
+        if (!t->data) {
+            if (cudaMalloc((void**)&t->data, need) != cudaSuccess) {
+                cudaGetLastError();
+                t->data = nullptr;
+                fail(status, -7, "rope: table allocation of %zu bytes failed", need);
+                return false;
+            }
+            t->bytes = need;
+        }
+        if (build_rope_table(ctx, t->data, seqLen, headDim, base, startPos, scaling, factor, low, high, origCtx, status) != 0) return false;
+        cudaError_t err = cudaEventRecord(t->built, ctx->stream);
+        if (err == cudaSuccess && capturing) err = cudaEventSynchronize(t->built);
+        if (err != cudaSuccess) {
+            cudaGetLastError();
+            fail(status, -7, "rope: building the table failed: %s", cudaGetErrorString(err));
+            return false;
+        }
+        return true;
+    };
+    if (capturing) {
+        OutsideCapture now(ctx);
+        if (!fill()) return nullptr;
+        t->pinned = 1;
+    } else if (!fill()) {
+        return nullptr;
+    }
     memcpy(t->key, key, sizeof(key));
     t->valid = 1;
     t->used = ++ctx->ropeClock;
+    return t;
+}
+
+const float* cached_rope_table(Context* ctx, size_t seqLen, int headDim, double base, long long startPos, int scaling, double factor,
+                               double low, double high, int origCtx, CUDAStatus* status) {
+    const RopeTable* t = rope_table(ctx, seqLen, true, headDim, base, startPos, scaling, factor, low, high, origCtx, status);
+    return t ? t->data : nullptr;
+}
+
+// A table of at least `positions` positions; *sinT: its sines.  For callers whose lengths change from call to call.
+const float* cached_rope_table_at_least(Context* ctx, size_t positions, int headDim, double base, long long startPos, int scaling,
+                                        double factor, double low, double high, int origCtx, const float** sinT, CUDAStatus* status) {
+    const RopeTable* t = rope_table(ctx, positions, false, headDim, base, startPos, scaling, factor, low, high, origCtx, status);
+    if (!t) return nullptr;
+    *sinT = t->data + (size_t)t->key[0] * (headDim / 2);
     return t->data;
 }
 

@@ -205,6 +205,7 @@ void cuda_close_device(CUDADeviceRef device) {
     for (RopeTable* t = ctx->ropeTables; t;) {
         RopeTable* next = t->next;
         cudaFree(t->data);
+        cudaEventDestroy(t->built);
         delete t;
         t = next;
     }
@@ -357,11 +358,14 @@ int cuda_context_set_stream(CUDADeviceRef device, void* cudaStream, CUDAStatus* 
         // the context's scratch (workspace, RoPE table, decode counters) may still be read by kernels queued on the old stream:
         // whatever the new stream launches is ordered after them
         cudaSetDevice(ctx->device);
-        // (a stream under capture runs nothing now, and an event may not tie it to work outside its capture)
-        const bool from = stream_capturing(ctx, nullptr);
+        // (a stream under capture runs nothing now, and an event may not tie it to work outside its capture: two streams of one capture
+        // are ordered in the graph, since they share its scratch)
+        unsigned long long idFrom = 0, idTo = 0;
+        const bool from = stream_capturing(ctx, &idFrom);
         cudaStream_t last = ctx->stream;
         ctx->stream = next;
-        if (!from && !stream_capturing(ctx, nullptr) && cudaEventRecord(ctx->streamSwitchEvent, last) == cudaSuccess)
+        const bool to = stream_capturing(ctx, &idTo);
+        if (from == to && (!from || idFrom == idTo) && cudaEventRecord(ctx->streamSwitchEvent, last) == cudaSuccess)
             cudaStreamWaitEvent(next, ctx->streamSwitchEvent, 0);
         cudaGetLastError();
     }

@@ -345,6 +345,87 @@ def test_decode_repeats_its_bits_and_replays_from_graphs(d):
     assert d.take_error() == 0
 
 
+@pytest.mark.parametrize("group,kv", [(16, 2), (2, 4), (7, 1)])
+def test_decode_of_long_contexts_in_f16(d, group, kv):
+    """What many tokens leave of values that nearly cancel is small: the error stays that of the output's rounding, 2^-11 of it.
+    The weights (two f16 parts, 2^-22) and float32 sums of codes less 8 (a few hundred terms per warp, 2^-24 each, of sums no larger
+    than the square root of their number) together stay below another 2^-11."""
+    t = make(1, [60001], kv, 128, 16, group, 11)
+    got = decode(d, t, kv, 128, 16, group, 1)
+    q, kc, kp, vc, vp, table, ctx = t
+    pages = table[0, :-(-60001 // 16)].long()
+    k, v = values64(kc, kp, pages, 60001), values64(vc, vp, pages, 60001)
+    s = torch.einsum("hgd,nhd->hgn", q[0].double().view(kv, group, 128), k) / 128 ** 0.5
+    want = torch.einsum("hgn,nhd->hgd", torch.softmax(s, -1), v).reshape(-1)
+    assert float((got[0].double() - want).norm()) <= 2.0 ** -10 * float(want.norm())
+
+
+@pytest.mark.parametrize("fmt", [2, 1])
+@pytest.mark.parametrize("kv,group,dim,page", [(8, 4, 128, 16), (2, 16, 64, 20), (4, 7, 128, 64)])
+def test_decode_with_a_plain_launch(d, monkeypatch, fmt, kv, group, dim, page):
+    """Where a cooperative launch is refused, the last block to arrive joins a pair's parts."""
+    t = make(fmt, [9000, 1, 700, 33, 0, 2500], kv, dim, page, group, 21)
+    monkeypatch.setenv("PUTER_DECODE_NO_COOPERATIVE", "1")
+    first = decode(d, t, kv, dim, page, group, fmt)
+    check_decode(first, t, kv, dim, page, group, fmt)
+    assert torch.equal(decode(d, t, kv, dim, page, group, fmt), first)
+    monkeypatch.delenv("PUTER_DECODE_NO_COOPERATIVE")
+    check_decode(decode(d, t, kv, dim, page, group, fmt), t, kv, dim, page, group, fmt)
+    assert d.take_error() == 0
+
+
+def test_decode_where_the_output_is_the_query(d):
+    """Every part of a pair has read the query before its output is written."""
+    t = make(2, [5000, 3, 800] * 20, 8, 128, 16, 4, 31)
+    want = decode(d, t, 8, 128, 16, 4, 2)
+    for _ in range(3):
+        q = t[0].clone()
+        decode(d, (q, *t[1:]), 8, 128, 16, 4, 2, out=q)
+        assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("fmt", [2, 1])
+def test_gather_to_an_odd_address(d, fmt):
+    """16 but not 32 bytes aligned: the narrower stores."""
+    codes, params = pool(5, 3, 16, 128, fmt, 4)
+    table = torch.tensor([4, 0, 2], dtype=torch.int32, device="cuda")
+    n = 40 * 3 * 128
+    room = torch.full((n + 16,), 7.0, dtype=TYPES[fmt], device="cuda")
+    assert room.data_ptr() % 32 == 0
+    outs = [room[at:at + n] for at in (0, 8)]
+    got = []
+    for out in outs:
+        d.KVPageGatherQ4(codes, params, table, out, 5, 16, 3, 128, 40, fmt)
+        got.append(out.clone())
+    assert torch.equal(got[0], got[1]) and bool((room[n + 8:] == 7).all())
+
+
+def test_append_in_a_graph_follows_its_inputs(d):
+    """A captured step of one token per sequence, replayed with other tokens at other places (slots, positions and values come from
+    memory); the RoPE table is made during the capture."""
+    import puter_b200
+
+    kv, dim, page, pages, fmt = 2, 128, 16, 6, 2
+    rope = puter_b200.RoPEConfig(Mode=1, BaseFreq=4321.0)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    xs = [torch.randn(3, kv * dim, device="cuda", generator=g).bfloat16() for _ in range(4)]
+    where = [([5, 0, 2], [0, 15, 7], [80, 15, 39]), ([1, 3, 4], [4, 5, 6], [4, 99, 0])]
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    k, v = torch.zeros_like(xs[0]), torch.zeros_like(xs[0])
+    ids, off, pos = i32([0, 0, 0]), i32([0, 1, 2]), i32([0, 0, 0])
+    mine, plain = [[*pool(pages, kv, page, dim, fmt, 1), *pool(pages, kv, page, dim, fmt, 2)] for _ in range(2)]
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        d.RoPEKVPageWriteQ4(rope, k, v, pos, ids, off, *mine, 3, kv, dim, pages, page, 100, fmt)
+    for n, (p, o, at) in enumerate(where):
+        k.copy_(xs[2 * n]), v.copy_(xs[2 * n + 1]), ids.copy_(i32(p)), off.copy_(i32(o)), pos.copy_(i32(at))
+        graph.replay()
+        append(d, rope, xs[2 * n], xs[2 * n + 1], at, p, o, *plain, fmt, max_pos=100)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(mine, plain)) and d.take_error() == 0
+
+
 def test_refusals(d):
     import puter_b200
 

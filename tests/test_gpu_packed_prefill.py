@@ -313,18 +313,58 @@ def test_two_captured_graphs_and_eager_calls_do_not_share_scratch(d):
     assert d.take_error() == 0
 
 
-def test_capture_without_its_rope_table_is_refused(d):
+def test_capture_makes_the_rope_table_that_is_missing(d):
+    """A first call with a RoPE setting may be a captured one: the table is there before any replay, and stays while others come and go."""
     import puter_b200
 
-    t = make(2, [30], 4, 2, 128, 1)
-    torch.cuda.synchronize()
-    graph = torch.cuda.CUDAGraph()
-    with pytest.raises(puter_b200.DeviceError) as e:
-        with torch.cuda.graph(graph):
-            call(d, *t, 4, 2, 128, 2, rope=puter_b200.RoPEConfig(Mode=1, BaseFreq=777.0))
-    assert e.value.code == -2 and "before the capture" in e.value.message
+    t = make(2, [30, 200], 4, 2, 128, 1)
     rope = puter_b200.RoPEConfig(Mode=1, BaseFreq=777.0)
-    check(call(d, *t, 4, 2, 128, 2, rope=rope), *t, 4, 2, 128, 2, True, rope)
+    out, graph = torch.full_like(t[0], 7.0), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        call(d, *t, 4, 2, 128, 2, rope=rope, out=out)
+    for base in (11.0, 12.0, 13.0, 14.0, 15.0, 16.0):
+        other = puter_b200.RoPEConfig(Mode=1, BaseFreq=base)
+        check(call(d, *t, 4, 2, 128, 2, rope=other), *t, 4, 2, 128, 2, True, other)
+    graph.replay()
+    torch.cuda.synchronize()
+    check(out, *t, 4, 2, 128, 2, True, rope)
+    assert d.take_error() == 0
+
+
+def test_two_streams_of_one_capture(d):
+    """Both calls use the scratch of the capture: the graph orders them, whatever the program's own streams leave open."""
+    ts = [make(2, [300, 20], 8, 2, 128, 1), make(2, [250, 90], 8, 2, 128, 2)]
+    import puter_b200
+
+    rope = puter_b200.RoPEConfig(Mode=1, BaseFreq=10000.0)
+    wants = [call(d, *t, 8, 2, 128, 2, rope=rope) for t in ts]
+    outs, graph, side = [torch.full_like(t[0], 7.0) for t in ts], torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        call(d, *ts[0], 8, 2, 128, 2, rope=rope, out=outs[0])
+        with torch.cuda.stream(side):
+            call(d, *ts[1], 8, 2, 128, 2, rope=rope, out=outs[1])
+        torch.cuda.current_stream().wait_stream(side)
+    for _ in range(5):
+        for o in outs:
+            o.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, wants))
+
+
+def test_lengths_and_settings_of_rope_from_call_to_call(d):
+    """Tables are shared by calls of different lengths and told apart by every setting."""
+    import puter_b200
+
+    for lens in ([40, 300], [17], [700], [300, 1], [1500, 40], [64], [65]):
+        for rope in (puter_b200.RoPEConfig(Mode=1, BaseFreq=10000.0), puter_b200.RoPEConfig(Mode=0, BaseFreq=10000.0),
+                     puter_b200.RoPEConfig(Mode=1, BaseFreq=10000.0, StartPosition=9), puter_b200.RoPEConfig(Mode=1, BaseFreq=300.0)):
+            for dim in (128, 64):
+                t = make(2, lens, 4, 2, dim, len(lens))
+                check(call(d, *t, 4, 2, dim, 2, rope=rope, longest=max(lens)), *t, 4, 2, dim, 2, True, rope)
 
 
 def test_calls_on_other_streams_follow_one_another(d):

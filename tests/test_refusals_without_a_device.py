@@ -92,6 +92,47 @@ def test_gather_and_decode(env):
         assert decode(**kw)[0] == 0
 
 
+TOP = (1 << 32) - 1
+
+
+def test_sizes_whose_products_leave_64_bits(env):
+    """Never a small product of large sizes that a small buffer would satisfy."""
+    buf, call = env
+    big = [buf(BIG) for _ in range(9)]
+    for pages, page, kv in [(1 << 31, 1 << 30, 8), (TOP, TOP, 2), (1 << 31, 1 << 31, 4), (1 << 31, TOP, 2)]:
+        code, message = call("rope_kv_page_write_q4", 2, *big[:2], 0, *big[3:5], *big[5:], 1, kv, 128, pages, page, 9, 2, 1e4, 0, 0.0, 0.0, 0.0, 0, 0)
+        assert code == -2, message
+        assert call("kv_page_gather_q4", 2, *big[:4], pages, page, kv, 128, 1, 0)[0] == -2
+        assert call("paged_decode_attention_q4", 2, *big[:8], 0, 1, 1, pages, page, kv, kv, 128, 0)[0] == -2
+    assert call("rope_kv_page_write_q4", 2, *big[:2], 0, *big[3:5], *big[5:], TOP, TOP, 128, 1, 1, 9, 2, 1e4, 0, 0.0, 0.0, 0.0, 0, 0)[0] == -2
+    assert call("kv_page_gather_q4", 2, *big[:4], 1, 1, TOP, 128, TOP, 0)[0] == -2
+    assert call("paged_decode_attention_q4", 2, *big[:8], 0, 1 << 31, 1, 1, 1, TOP, 1, 128, 0)[0] == -2
+    assert call("rope_packed_attention_prefill", 2, *big[:4], big[4], 1, (1 << 31) - 1, 10, TOP, 1, 128, 1, 2, 1e4, 0, 0, 0.0, 0.0, 0.0, 0, 0)[0] == -2
+
+
+def test_alignment_and_overlap(env):
+    buf, call = env
+    odd, big = buf(BIG, (1 << 20) + 2), buf(BIG)
+
+    def append(positions=big, ids=big, offsets=big):
+        return call("rope_kv_page_write_q4", 2, big, big, positions, ids, offsets, *[big] * 4, 1, 1, 64, 1, 1, 9, 1, 1e4, 0, 0.0, 0.0, 0.0, 0, 0)
+
+    for kw in (dict(positions=odd), dict(ids=odd), dict(offsets=odd)):
+        assert append(**kw)[0] == -2 and "aligned" in append(**kw)[1]
+    assert "aligned" in call("kv_page_gather_q4", 2, big, big, odd, big, 1, 1, 1, 64, 1, 0)[1]
+    for k in (6, 7, 9):
+        args = [big] * 8 + [0]
+        args[k - 1 if k < 9 else 8] = odd
+        assert "aligned" in call("paged_decode_attention_q4", 2, *args, 1, 1, 1, 1, 1, 1, 64, 0)[1], k
+
+    def prompt(q=buf(BIG, 1 << 20), k=buf(BIG, 2 << 20), v=buf(BIG, 3 << 20), starts=big, out=buf(BIG, 5 << 20), fmt=2):
+        return call("rope_packed_attention_prefill", fmt, q, k, v, starts, out, 1, 16, 16, 4, 2, 64, 1, 2, 1e4, 0, 0, 0.0, 0.0, 0.0, 0, 0)
+
+    for at in ((1 << 20) + 16, (1 << 20) - 16, (2 << 20) + 4080, (3 << 20) - 8176):
+        assert prompt(out=buf(BIG, at))[0] == -2 and "overlap" in prompt(out=buf(BIG, at))[1], at
+    assert "aligned" in prompt(starts=odd)[1] and "aligned" in prompt(out=buf(BIG, (5 << 20) + 1))[1] and "aligned" in prompt(k=odd, fmt=0)[1]
+
+
 def test_python_refuses_windows_and_alibi():
     from puter_b200 import device as D
 
