@@ -254,6 +254,24 @@ class Backend {
         check(cuda_dispatch_kv_page_gather(ctx_, (int)f, ref(storage), ref(pageTable), ref(output), (uint32_t)pageCount,
                                            (uint32_t)pageSize, (uint32_t)inner, (uint32_t)outRows, (uint64_t)storageOffset, 0, &st), st);
     }
+    // the cache in 4 bits (no reference counterpart): rope == nullptr means K comes rotated, positions may then be null
+    void RoPEKVPageWriteQ4(const RoPEConfig* rope, void* k, void* v, void* positions, void* pageIDs, void* offsets, void* kCodes,
+                           void* kParams, void* vCodes, void* vParams, int rows, int kvHeads, int headDim, int pageCount, int pageSize,
+                           int maxPositions, DType f) {
+        const RoPEConfig c = rope ? *rope : RoPEConfig{};
+        CUDAStatus st;
+        check(cuda_dispatch_rope_kv_page_write_q4(ctx_, (int)f, ref(k), ref(v), positions ? ref(positions) : nullptr, ref(pageIDs), ref(offsets),
+                                                  ref(kCodes), ref(kParams), ref(vCodes), ref(vParams), (uint32_t)rows, (uint32_t)kvHeads,
+                                                  (uint32_t)headDim, (uint32_t)pageCount, (uint32_t)pageSize, (uint32_t)maxPositions,
+                                                  rope ? (uint32_t)c.Mode : 2u, c.BaseFreq, (uint32_t)c.Scaling, c.ScalingFactor, c.LowFreqFactor,
+                                                  c.HighFreqFactor, (uint32_t)c.OriginalContext, 0, &st), st);
+    }
+    void KVPageGatherQ4(void* codes, void* params, void* pageTable, void* output, int pageCount, int pageSize, int kvHeads, int headDim,
+                        int outRows, DType f) {
+        CUDAStatus st;
+        check(cuda_dispatch_kv_page_gather_q4(ctx_, (int)f, ref(codes), ref(params), ref(pageTable), ref(output), (uint32_t)pageCount,
+                                              (uint32_t)pageSize, (uint32_t)kvHeads, (uint32_t)headDim, (uint32_t)outRows, 0, &st), st);
+    }
     // ---- device.Attention ----
     void MultiHeadAttention(MultiHeadAttentionConfig c, void* query, void* key, void* value, void* output, int seqQ, int seqK, DType f) {
         if (c.ALiBiSlope != 0.f) throw DeviceError(-6, "attention: ALiBi is not on this library's path");
@@ -284,6 +302,30 @@ class Backend {
                                                    ref(ctxLens), kScale ? ref(kScale) : nullptr, vScale ? ref(vScale) : nullptr,
                                                    ref(output), nullptr, (uint32_t)batch, (uint32_t)maxPagesPerSeq, (uint32_t)pageCount,
                                                    (uint32_t)pageSize, (uint32_t)c.NumHeads, (uint32_t)kv, (uint32_t)c.HeadDim, 0, &st), st);
+    }
+    void PagedDecodeAttentionQ4(MultiHeadAttentionConfig c, void* query, void* kCodes, void* kParams, void* vCodes, void* vParams,
+                                void* pageTable, void* ctxLens, void* output, int batch, int maxPagesPerSeq, int pageCount, int pageSize,
+                                DType f) {
+        if (c.ALiBiSlope != 0.f || c.WindowSize != 0) throw DeviceError(-6, "paged decode attention (4 bits): no ALiBi and no sliding window");
+        const int kv = c.KVHeadCount > 0 ? c.KVHeadCount : c.NumHeads;
+        CUDAStatus st;
+        check(cuda_dispatch_paged_decode_attention_q4(ctx_, (int)f, ref(query), ref(kCodes), ref(kParams), ref(vCodes), ref(vParams),
+                                                      ref(pageTable), ref(ctxLens), ref(output), nullptr, (uint32_t)batch,
+                                                      (uint32_t)maxPagesPerSeq, (uint32_t)pageCount, (uint32_t)pageSize, (uint32_t)c.NumHeads,
+                                                      (uint32_t)kv, (uint32_t)c.HeadDim, 0, &st), st);
+    }
+    // prompts of different lengths packed one behind the other; rope == nullptr: q and k come rotated
+    void RoPEPackedAttentionPrefill(const RoPEConfig* rope, MultiHeadAttentionConfig c, void* query, void* key, void* value,
+                                    void* seqStarts, void* output, int batch, int totalTokens, int maxSeqLen, DType f) {
+        if (c.ALiBiSlope != 0.f || c.WindowSize != 0) throw DeviceError(-6, "packed prefill attention: no ALiBi and no sliding window");
+        const int kv = c.KVHeadCount > 0 ? c.KVHeadCount : c.NumHeads;
+        const RoPEConfig r = rope ? *rope : RoPEConfig{};
+        CUDAStatus st;
+        check(cuda_dispatch_rope_packed_attention_prefill(ctx_, (int)f, ref(query), ref(key), ref(value), ref(seqStarts), ref(output),
+                                                          (uint32_t)batch, (uint32_t)totalTokens, (uint32_t)maxSeqLen, (uint32_t)c.NumHeads,
+                                                          (uint32_t)kv, (uint32_t)c.HeadDim, c.Causal ? 1u : 0u, rope ? (uint32_t)r.Mode : 2u,
+                                                          r.BaseFreq, (int64_t)r.StartPosition, (uint32_t)r.Scaling, r.ScalingFactor,
+                                                          r.LowFreqFactor, r.HighFreqFactor, (uint32_t)r.OriginalContext, 0, &st), st);
     }
     // convert package on device memory (execution/shape_cast_intrinsic.go:57-114)
     void Convert(void* dst, void* src, long long count, DType dstFormat, DType srcFormat) {
