@@ -33,8 +33,8 @@
 //     n, 2.1e-4, the rounding of the output, with n - 8; 46 -> 48 us).
 // Sums, maxima and accumulators are float32.
 //
-// Work: the tiles of 16 tokens of all (KV head, sequence) pairs in one list, cut into equal contiguous ranges, one per CTA, and each
-// CTA's range into equal ranges, one per warp.  A warp owns its pipeline (stages of 32 tokens, copies running ahead across sequence
+// Work: the tiles of 16 tokens of all (KV head, sequence) pairs in one list, every pair a few tiles longer for what its start costs, cut into
+// equal contiguous ranges, one per CTA, and each CTA's range into equal ranges, one per warp.  A warp owns its pipeline (stages of 32 tokens, copies running ahead across sequence
 // boundaries, page entries one step further ahead), so there is no block-wide barrier before the end.  Where pages hold whole tiles the
 // copies are bulk copies, four per tile (codes and params of K and V), each issued by a lane of its own: ~20 instructions per step where
 // 16-byte copies with a page lookup per token take ~90.  A pair that lies inside a warp's range is written by the warp.  Otherwise the warps
@@ -42,6 +42,7 @@
 // for the pair's counter and takes its share of the output's 32-dimension slices (a cooperative launch makes all CTAs resident; where it
 // is refused the CTA that arrives last joins everything).  Fixed order either way: the same bits from call to call.  One CTA joining 38
 // others' parts of 16 heads took 18 us, all of them together 3.
+#include <limits.h>
 #include <math.h>
 #include <stdlib.h>
 
@@ -63,7 +64,7 @@ struct Params {
     const int32_t *table, *ctxLens;
     uint16_t* out;
     int* errorFlag;
-    const int* tileStart;  // [batch + 2] exclusive prefix of tiles and the most of one, or nullptr: scanned in shared memory
+    const int* tileStart;  // [batch + 3] exclusive prefix of tiles, the most and the fewest of one, or nullptr: scanned in shared memory
     float* acc;            // partial accumulators [slots, heads of a block, D]: one slot per warp, then two per CTA
     float2* ml;            // (maximum in the log2 domain, sum) [slots, heads of a block]
     int* counters;         // arrivals (and departures) per (unit, sequence): zero on entry and on exit
@@ -165,24 +166,26 @@ __device__ __forceinline__ int seq_ctx(const Params& p, int b) {
     return (int)ctx;
 }
 
-// exclusive prefix sum of tiles per sequence: out[0 .. batch], and the most tiles of one in out[batch + 1]; lens (may be null): the cut contexts.  Every thread of the block calls it.
-__device__ void block_prefix(const Params& p, int* out, int* lens) {
-    __shared__ int sums[32], tops[32];
+// exclusive prefix sum of tiles per sequence: out[0 .. batch], the most tiles of one in out[batch + 1] and the fewest of one that is not
+// empty in out[batch + 2]; lens (may be null): the cut contexts.  Every thread of the block calls it.
+__device__ void block_prefix(const Params& p, int start, int* out, int* lens) {
+    __shared__ int sums[32], tops[32], bottoms[32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int carry = 0, top = 0;
+    int carry = 0, top = 0, bottom = INT_MAX;
     for (int base = 0; base < p.batch; base += blockDim.x) {
         const int b = base + threadIdx.x, ctx = b < p.batch ? seq_ctx(p, b) : 0;
-        const int tiles = (int)(((long long)ctx + kTile - 1) / kTile);
+        const int tiles = ctx > 0 ? (int)(((long long)ctx + kTile - 1) / kTile) + start : 0;
         int incl = tiles;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int n = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += n;
         }
-        const int most = __reduce_max_sync(0xffffffffu, tiles);
+        const int most = __reduce_max_sync(0xffffffffu, tiles), fewest = __reduce_min_sync(0xffffffffu, tiles ? tiles : INT_MAX);
         if (lane == 31) {
             sums[warp] = incl;
             tops[warp] = most;
+            bottoms[warp] = fewest;
         }
         __syncthreads();
         const int used = (min(p.batch - base, (int)blockDim.x) + 31) / 32;
@@ -191,6 +194,7 @@ __device__ void block_prefix(const Params& p, int* out, int* lens) {
             if (w < warp) before += sums[w];
             carry += sums[w];
             top = max(top, tops[w]);
+            bottom = min(bottom, bottoms[w]);
         }
         if (b < p.batch) {
             out[b] = before + incl - tiles;
@@ -201,10 +205,11 @@ __device__ void block_prefix(const Params& p, int* out, int* lens) {
     if (threadIdx.x == 0) {
         out[p.batch] = carry;
         out[p.batch + 1] = top;
+        out[p.batch + 2] = bottom;
     }
     __syncthreads();
 }
-__global__ void __launch_bounds__(1024) prefix_kernel(Params p, int* out) { block_prefix(p, out, nullptr); }
+__global__ void __launch_bounds__(1024) prefix_kernel(Params p, int start, int* out) { block_prefix(p, start, out, nullptr); }
 
 // a / b for b > 0; 64-bit divisions take a hundred instructions and are hardly ever needed
 __device__ __forceinline__ long long quotient(long long a, long long b) {
@@ -228,6 +233,10 @@ struct Shape {
     static constexpr int D = D_, NT = NT_ ? NT_ : 1, WARPS = WARPS_, MT = MT_;
     static constexpr bool QUAD = NT_ == 0;
     static constexpr int STEP = 16 * MT;            // tokens per step of a warp
+    // A pair counts this many tiles more than it has, which nobody works on: what a warp spends on another pair's queries, partial and cold
+    // pipeline.  Two steps measured best of none, one, two and three (us, none against two): 256 sequences of up to 2000 tokens 51 : 32, 100 of up
+    // to 4000 at 8 heads per KV head 46 : 26, 48 of up to 3000 with 12 KV heads of 64 23 : 17.5, 64 of 512 to 32768 tokens 114.9 : 110.9.
+    static constexpr int START = 2 * MT;
     static constexpr int ROW = D / 2;               // bytes of a token's codes
     static constexpr int STAGE = 2 * STEP * ROW + 2 * STEP * 4;
     static constexpr int STAGES = kStageBytes / (WARPS * STAGE);
@@ -241,7 +250,7 @@ __device__ __forceinline__ float weight(float2 ml, float M) { return ml.x == -IN
 // PAGED: pages hold whole tiles (page size a multiple of 16): bulk copies.  Otherwise 16-byte copies with a page lookup per token.
 template <int DT, typename S, bool PAGED>
 __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
-    constexpr int D = S::D, NT = S::NT, MT = S::MT, kStep = S::STEP;
+    constexpr int D = S::D, NT = S::NT, MT = S::MT, kStep = S::STEP, kStart = S::START;
     constexpr int WK = D / 32;   // words of a token's K codes in a lane
     constexpr int WV = D / 64;   // words of a token's V codes in a lane
     constexpr int ROW = S::ROW;
@@ -251,7 +260,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
     constexpr int kPart = S::HEADS * D * 4 + S::HEADS * 8;  // a partial in shared memory: accumulators, then (maximum, sum)
     static_assert(kPart <= S::STAGES * S::STAGE, "a warp's partial takes the place of its stages");
     extern __shared__ __align__(128) unsigned char smemRaw[];
-    __shared__ int sStart[kPrefixSmem + 2], sCtx[kPrefixSmem];
+    __shared__ int sStart[kPrefixSmem + 3], sCtx[kPrefixSmem];
     __shared__ int sSeg[32];       // entry 2w + i: the pair of warp w's partial i (0: it began before the warp's range, 1: it goes on behind it)
     __shared__ int sNear[S::WARPS];  // which of the two lies in shared memory
     __shared__ int sB[32], sUnit[32], sWhere[32];  // of an entry: sequence, unit; pair inside the CTA's range (2) or begun before it (0) or going on behind it (1)
@@ -259,7 +268,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
     __shared__ __align__(8) uint64_t sBar[S::WARPS * S::STAGES];
     const int* ts = p.tileStart;
     if (!ts) {
-        block_prefix(p, sStart, sCtx);
+        block_prefix(p, kStart, sStart, sCtx);
         ts = sStart;
     }
     auto ctx_of = [&](int b) { return p.tileStart ? seq_ctx(p, b) : sCtx[b]; };
@@ -287,9 +296,35 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
         }
         return unit * T + (r - ts[a] < ts[a + 1] - r ? ts[a] : ts[a + 1]);
     };
-    const long long clo = edge(blockIdx.x), chi = edge(blockIdx.x + 1);
+    // Few large pairs (eight CTAs each at least) get whole CTAs, in proportion and rounded: a CTA that ends one pair and begins another is
+    // 4 us late, and every owner of both waits for it.  What the rounding adds to a range, each^2 / (2 fewest) tiles or so, is kept
+    // to some 64 (3 us of streaming).  Two sequences of 16384 tokens with 32 heads on 2 KV heads 23.7 -> 18.6 us, on 8 24.4 -> 22.0.
+    const bool owned = !aligned && split.each >= 2 * kStart && ts[p.batch + 2] >= 8 * split.each && split.each * split.each <= 128ll * ts[p.batch + 2] && total * (parts + 1ll) >> 32 == 0;
+    auto owner = [&](long long at) { return (int)(((uint32_t)at * parts + (uint32_t)total / 2) / (uint32_t)total); };  // first CTA of the pair that begins at tile `at`
+    long long clo, chi, from = 0;  // from: where the warps' ranges begin
+    if (owned) {
+        // the last pair whose first CTA is not behind this one: at * parts + total / 2 < (i + 1) * total
+        const uint32_t i = blockIdx.x, last = ((i + 1) * (uint32_t)total - (uint32_t)total / 2 - 1) / (uint32_t)parts, unit = last / (uint32_t)T;
+        const int r = (int)(last - unit * (uint32_t)T);
+        int a = 0, z = p.batch;
+        while (z - a > 1) {
+            const int m = (a + z) >> 1;
+            if (ts[m] <= r) a = m;
+            else z = m;
+        }
+        const long long at = unit * T + ts[a], tiles = ts[a + 1] - ts[a];
+        const int first = owner(at);
+        const Split inside(tiles, owner(at + tiles) - first);
+        clo = at + inside.begin((int)i - first);
+        chi = at + inside.begin((int)i - first + 1);
+        from = (int)i == first ? clo + kStart : clo;
+    } else {
+        clo = edge(blockIdx.x);
+        chi = edge(blockIdx.x + 1);
+        from = aligned ? clo + kStart : clo;
+    }
     if (clo >= chi) return;
-    const long long lo = clo + warp * (chi - clo) / S::WARPS, hi = clo + (warp + 1) * (chi - clo) / S::WARPS;
+    const long long lo = from + warp * (chi - from) / S::WARPS, hi = from + (warp + 1) * (chi - from) / S::WARPS;
     if (threadIdx.x < 32) sSeg[threadIdx.x] = -1;
     if (threadIdx.x < S::WARPS) sNear[threadIdx.x] = -1;
     if (threadIdx.x < 2) sShared[threadIdx.x] = -1;
@@ -333,7 +368,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
         const uint32_t dstOff = (part < 2 ? part * kStep * ROW : 2 * kStep * ROW + (part - 2) * kStep * 4) + tileOf * kTile * perSlot;
         // Moves to the next step and starts fetching its page entries.
         auto look_ahead = [&]() {
-            if (iTok >= iEnd) {
+            while (iTok >= iEnd) {
                 if (iNext >= hi) return;
                 long long r = iNext - (long long)iUnit * T;
                 if (r >= T) {
@@ -345,9 +380,9 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
                 while (ts[ib + 1] <= r) ib++;
                 const long long s0 = ts[ib], s1 = ts[ib + 1], stop = hi - (long long)iUnit * T, e = s1 < stop ? s1 : stop;
                 const int ctx = ctx_of(ib);
-                const long long end = (e - s0) * kTile;
+                const long long end = (e - s0 - kStart) * kTile;
                 iTable = p.table + (size_t)ib * p.maxPages;
-                iTok = (int)((r - s0) * kTile);
+                iTok = r - s0 > kStart ? (int)((r - s0 - kStart) * kTile) : 0;
                 iEnd = (int)(end < ctx ? end : ctx);
                 iNext = (long long)iUnit * T + e;
             }
@@ -406,6 +441,13 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
             if (!PAGED) asm volatile("cp.async.commit_group;" ::: "memory");
         };
         look_ahead();
+        {  // the first pair's queries set out with the page entries instead of behind them
+            const int kvh = cUnit / p.blocks, head0 = kvh * p.group + (cUnit - kvh * p.blocks) * S::HEADS, heads = min(p.group - (cUnit - kvh * p.blocks) * S::HEADS, S::HEADS);
+            constexpr int LINES = S::HEADS * D * 2 / 128;
+            uint32_t unused;
+            if (lane < LINES && lane * 64 < heads * D)
+                asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(unused) : "l"(p.q + ((size_t)cb * p.numHeads + head0) * D + lane * 64));
+        }
 #pragma unroll
         for (int s = 0; s < S::STAGES - 1; s++) issue();
 
@@ -425,9 +467,13 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
             if (r >= T) { cUnit++; cb = 0; r -= T; }
             while (ts[cb + 1] <= r) cb++;
             const int b = cb;
-            const long long s0 = ts[b], s1 = ts[b + 1], stop = hi - (long long)cUnit * T, e = s1 < stop ? s1 : stop;
+            const long long s0 = ts[b] + kStart, s1 = ts[b + 1], stop = hi - (long long)cUnit * T, e = s1 < stop ? s1 : stop;
+            if (e <= s0) {
+                cur = (long long)cUnit * T + e;
+                continue;
+            }
             const int ctx = ctx_of(b);
-            const int tok0 = (int)((r - s0) * kTile);
+            const int tok0 = r > s0 ? (int)((r - s0) * kTile) : 0;
             const long long endTok = (e - s0) * kTile;
             const int tokEnd = (int)(endTok < ctx ? endTok : ctx);
             const int kvh = cUnit / p.blocks, block = cUnit % p.blocks;
@@ -915,22 +961,33 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
             float den = ml.y * k, num[E] = {};
 #pragma unroll
             for (int off = 16; off > 0; off >>= 1) den += __shfl_xor_sync(0xffffffffu, den, off);
-#pragma unroll 2
-            for (int i = 0; i < n; i++) {
-                const float wt = __shfl_sync(0xffffffffu, k, i);
-                const float* from = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)at, i);
-                if (!((members >> (2 * (w0 + i))) & 3)) continue;  // uniform
+            for (int i0 = 0; i0 < n; i0 += 4) {  // four parts on their way at a time: some lie in the scratch
+                float x[4][E], wt[4];
 #pragma unroll
-                for (int d = 0; d < E; d++) num[d] = fmaf(from[lane + 32 * d], wt, num[d]);
+                for (int u = 0; u < 4; u++) {
+                    const int i = i0 + u;
+                    wt[u] = __shfl_sync(0xffffffffu, k, i & 31);
+                    const float* from = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)at, i & 31) + lane * E;
+#pragma unroll
+                    for (int d = 0; d < E; d++) x[u][d] = 0.f;
+                    if (i < n && ((members >> (2 * (w0 + i))) & 3)) {  // uniform
+                        if (E == 4) *(float4*)x[u] = *(const float4*)from;
+                        else *(float2*)x[u] = *(const float2*)from;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+#pragma unroll
+                    for (int d = 0; d < E; d++) num[d] = fmaf(x[u][d], wt[u], num[d]);
             }
             const long long slot = (ctaSlots + 2ll * blockIdx.x + where) * S::HEADS + h;
             if (where == 2) {
-                uint16_t* dst = p.out + ((size_t)sB[e0] * p.numHeads + kvh * p.group + head) * D + lane;
+                uint32_t* dst = (uint32_t*)(p.out + ((size_t)sB[e0] * p.numHeads + kvh * p.group + head) * D + lane * E);
 #pragma unroll
-                for (int d = 0; d < E; d++) Storage<DT>::store(dst, 32 * d, num[d] / den);
+                for (int d = 0; d < E; d += 2) dst[d / 2] = pack16_arith<DT>(num[d] / den, num[d + 1] / den);
             } else {
 #pragma unroll
-                for (int d = 0; d < E; d++) p.acc[slot * D + lane + 32 * d] = num[d];
+                for (int d = 0; d < E; d += 2) *(float2*)(p.acc + slot * D + lane * E + d) = make_float2(num[d], num[d + 1]);
                 if (lane == 0) p.ml[slot] = make_float2(M, den);
             }
         }
@@ -943,7 +1000,8 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
         int go = 0;
         if (e >= 0) {
             const long long at = (long long)sUnit[e] * T;
-            const int first = split.holding(at + ts[sB[e]]), owners = split.holding(at + ts[sB[e] + 1] - 1) - first + 1;
+            const long long begin = at + ts[sB[e]], end = at + ts[sB[e] + 1];
+            const int first = owned ? owner(begin) : split.holding(begin + kStart), owners = (owned ? owner(end) : split.holding(end - 1) + 1) - first;
             int* const counter = p.counters + sSeg[e];
             sFirst[threadIdx.x] = first;
             sOwners[threadIdx.x] = owners;
@@ -1057,7 +1115,7 @@ static int launch(Context* ctx, Params& p, CUDAStatus* status) {
     p.units = p.kvHeads * p.blocks;
     const size_t slots = (size_t)grid * (S::WARPS + 2);
     const size_t accBytes = slots * S::HEADS * S::D * 4, mlBytes = slots * S::HEADS * 8;
-    const size_t prefixBytes = p.batch > kPrefixSmem ? ((size_t)p.batch + 2) * 4 : 0;
+    const size_t prefixBytes = p.batch > kPrefixSmem ? ((size_t)p.batch + 3) * 4 : 0;
     const size_t counterBytes = (size_t)p.units * p.batch * 4;
     Scratch ws;
     int rc = call_scratch(ctx, accBytes + mlBytes + prefixBytes, counterBytes, &ws, status);
@@ -1069,7 +1127,7 @@ static int launch(Context* ctx, Params& p, CUDAStatus* status) {
         return fail(status, -7, "%s: clearing the arrival counters failed", what);
     if (prefixBytes) {
         int* prefix = (int*)(ws.base + accBytes + mlBytes);
-        prefix_kernel<<<1, 1024, 0, ctx->stream>>>(p, prefix);
+        prefix_kernel<<<1, 1024, 0, ctx->stream>>>(p, S::START, prefix);
         rc = check_launch(ctx, status, "paged decode attention (4 bits): prefix");
         if (rc != 0) return rc;
         p.tileStart = prefix;
@@ -1117,6 +1175,8 @@ extern "C" int cuda_dispatch_paged_decode_attention_q4(CUDADeviceRef contextRef,
     if (slots > 0xFFFFFFFFull || (size_t)maxPagesPerSeq * pageSize > 0x7FFFFFE0ull || batch > 0x7FFFFFFEu)
         return fail(status, -2, "%s: a pool of %zu vectors or a context of %zu tokens exceeds the index range", what, slots,
                     (size_t)maxPagesPerSeq * pageSize);
+    if ((size_t)batch * ((size_t)maxPagesPerSeq * pageSize / q4d::kTile + 16) > 0x7FFFFFFFull)  // tiles are counted in 31 bits
+        return fail(status, -2, "%s: %u contexts of up to %zu tokens exceed the index range", what, batch, (size_t)maxPagesPerSeq * pageSize);
     PUTER_REQUIRE(queryRef, "query", (size_t)batch * numHeads * headDim * 2);
     PUTER_REQUIRE(outRef, "out", (size_t)batch * numHeads * headDim * 2);
     PUTER_REQUIRE(kCodesRef, "kCodes", slots * (headDim / 2));

@@ -248,6 +248,15 @@ def test_decode_batches(d, lens):
     assert d.take_error() == 0
 
 
+@pytest.mark.parametrize("kv,group", [(2, 16), (8, 4), (4, 8), (1, 3)])
+@pytest.mark.parametrize("lens", [[9000], [30000, 28000], [20000, 0, 17000, 0], [7000, 6900, 5000], [1, 40, 2, 3, 17, 1, 1, 90, 2000] * 12, [3000] + [1] * 60])
+def test_decode_where_blocks_divide_pairs(d, kv, group, lens):
+    """Whole blocks per pair, blocks that end one pair and begin another, blocks of many pairs; starts that cost more than their pair."""
+    t = make(2, lens, kv, 128, 16, group, 13)
+    check_decode(decode(d, t, kv, 128, 16, group, 2), t, kv, 128, 16, group, 2)
+    assert d.take_error() == 0
+
+
 @pytest.mark.parametrize("fmt", [2, 1])
 def test_decode_peaked_scores_and_steps_of_very_different_size(d, fmt):
     kv, group, dim, page = 4, 4, 128, 16

@@ -107,6 +107,7 @@ def test_sizes_whose_products_leave_64_bits(env):
     assert call("rope_kv_page_write_q4", 2, *big[:2], 0, *big[3:5], *big[5:], TOP, TOP, 128, 1, 1, 9, 2, 1e4, 0, 0.0, 0.0, 0.0, 0, 0)[0] == -2
     assert call("kv_page_gather_q4", 2, *big[:4], 1, 1, TOP, 128, TOP, 0)[0] == -2
     assert call("paged_decode_attention_q4", 2, *big[:8], 0, 1 << 31, 1, 1, 1, TOP, 1, 128, 0)[0] == -2
+    assert call("paged_decode_attention_q4", 2, *big[:8], 0, 1 << 16, 1 << 16, 100, 16, 8, 8, 128, 0)[0] == -2  # more tiles than 31 bits count
     assert call("rope_packed_attention_prefill", 2, *big[:4], big[4], 1, (1 << 31) - 1, 10, TOP, 1, 128, 1, 2, 1e4, 0, 0, 0.0, 0.0, 0.0, 0, 0)[0] == -2
 
 
