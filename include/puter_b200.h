@@ -141,8 +141,9 @@ int cuda_context_reset_stream(CUDADeviceRef device, CUDAStatus* status);
 int cuda_context_set_exact(CUDADeviceRef device, int exact, CUDAStatus* status);
 /* NEW: synchronises the context's stream, returns the device-side error flag in *outFlag and clears it:
    1 = some call since the last read met an out-of-range page id / offset or an over-long context and skipped it;
-   3 = a bounded wait on a row copy ran out (row-pipeline kernels); 4 = a bounded wait between the CTAs of a paged decode
-   step ran out (an owner of a split sequence never arrived): the outputs of that call are not valid */
+   2 = a bounded wait inside a tensor-core prefill ran out; 3 = a bounded wait on a copy ran out (row-pipeline kernels, decode over the
+   cache in 4 bits); 4 = a bounded wait between the CTAs of a paged decode step ran out (an owner of a split sequence never arrived):
+   the outputs of that call are not valid */
 int cuda_context_take_error(CUDADeviceRef device, int* outFlag, CUDAStatus* status);
 /* NEW: number of kernels this context has launched (diagnostics / benchmarks) */
 unsigned long long cuda_context_launch_count(CUDADeviceRef device);
