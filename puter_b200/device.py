@@ -86,6 +86,9 @@ class SharedBuffer:
             self.ref = None
 
 
+_NO_TOKEN = ctypes.c_uint64(0)  # completionToken
+
+
 class Device:
     """One context on one GPU.  ``Device()`` opens the current torch CUDA device."""
 
@@ -147,8 +150,7 @@ class Device:
             self._refs[key] = r
         return r
 
-    def _call(self, name, tensors, build_args):
-        self._enter()
+    def _handles(self, tensors):
         if len(self._refs) >= 4096:  # bound the cache (between calls only): handles are cheap to rebuild
             for old in self._refs.values():
                 self.lib.cuda_buffer_release(old)
@@ -158,9 +160,21 @@ class Device:
         for t in tensors:
             r = known.get((t.data_ptr(), t.nbytes)) if t is not None and t.is_contiguous() else None
             refs.append(r if r is not None else self._ref(t))
-        args = build_args(refs)
+        return refs
+
+    def _call(self, name, tensors, build_args):
+        self._enter()
+        args = build_args(self._handles(tensors))
         rc = getattr(self.lib, name)(self.ref, *args, ctypes.byref(self._status))
         self._check(rc)
+
+    def _call_plain(self, name, format, tensors, rest):
+        """_call of an entry point (context, format, buffers, rest, token, status): `rest` in the declared types, integers of 32 bits as they are."""
+        self._enter()
+        fn = getattr(self.lib.__dict__.get("plain", self.lib), name)
+        rc = fn(self.ref, format, *self._handles(tensors), *rest, _NO_TOKEN, ctypes.byref(self._status))
+        if rc != 0:
+            self._check(rc)
 
     # ---- memory shared between the per-GPU processes of a box ----------------------------------------
     def alloc_shared(self, nbytes: int) -> SharedBuffer:
@@ -420,15 +434,15 @@ class Device:
         (positions may be None).  Codes are [pageCount, kvHeads, pageSize, headDim / 2] bytes, params [pageCount, kvHeads, pageSize, 2]
         of `format` = (step, least); an element is least + step * code."""
         rc = rope or RoPEConfig()
-        mode = 2 if rope is None else int(rc.Mode)
-        self._call("cuda_dispatch_rope_kv_page_write_q4", [k, v, positions, pageIDs, offsets, kCodes, kParams, vCodes, vParams],
-                   lambda r: (format, *r, rows, kvHeads, headDim, pageCount, pageSize, maxPositions, mode, float(rc.BaseFreq), int(rc.Scaling),
-                              float(rc.ScalingFactor), float(rc.LowFreqFactor), float(rc.HighFreqFactor), int(rc.OriginalContext), 0))
+        f64 = ctypes.c_double
+        self._call_plain("cuda_dispatch_rope_kv_page_write_q4", format, (k, v, positions, pageIDs, offsets, kCodes, kParams, vCodes, vParams),
+                         (rows, kvHeads, headDim, pageCount, pageSize, maxPositions, 2 if rope is None else int(rc.Mode), f64(rc.BaseFreq),
+                          int(rc.Scaling), f64(rc.ScalingFactor), f64(rc.LowFreqFactor), f64(rc.HighFreqFactor), int(rc.OriginalContext)))
 
     def KVPageGatherQ4(self, codes, params, pageTable, output, pageCount, pageSize, kvHeads, headDim, outRows, format):
         """KVPageGather from the cache in 4 bits: output [outRows, kvHeads * headDim] of `format`, rounded once."""
-        self._call("cuda_dispatch_kv_page_gather_q4", [codes, params, pageTable, output],
-                   lambda r: (format, *r, pageCount, pageSize, kvHeads, headDim, outRows, 0))
+        self._call_plain("cuda_dispatch_kv_page_gather_q4", format, (codes, params, pageTable, output),
+                         (pageCount, pageSize, kvHeads, headDim, outRows))
 
     # ---- Attention ------------------------------------------------------------------------------------
     def MultiHeadAttention(self, config: MultiHeadAttentionConfig, query, key, value, output, seqQ, seqK, format):
@@ -465,11 +479,11 @@ class Device:
             raise DeviceError(-6, "packed prefill attention: no ALiBi and no sliding window")
         kv = attn.KVHeadCount if attn.KVHeadCount > 0 else attn.NumHeads
         rc = rope or RoPEConfig()
-        mode = 2 if rope is None else int(rc.Mode)
-        self._call("cuda_dispatch_rope_packed_attention_prefill", [query, key, value, seqStarts, output],
-                   lambda r: (format, *r, batch, totalTokens, maxSeqLen, attn.NumHeads, kv, attn.HeadDim, int(attn.Causal), mode,
-                              float(rc.BaseFreq), int(rc.StartPosition), int(rc.Scaling), float(rc.ScalingFactor),
-                              float(rc.LowFreqFactor), float(rc.HighFreqFactor), int(rc.OriginalContext), 0))
+        f64 = ctypes.c_double
+        self._call_plain("cuda_dispatch_rope_packed_attention_prefill", format, (query, key, value, seqStarts, output),
+                         (batch, totalTokens, maxSeqLen, attn.NumHeads, kv, attn.HeadDim, int(attn.Causal), 2 if rope is None else int(rc.Mode),
+                          f64(rc.BaseFreq), ctypes.c_int64(rc.StartPosition), int(rc.Scaling), f64(rc.ScalingFactor), f64(rc.LowFreqFactor),
+                          f64(rc.HighFreqFactor), int(rc.OriginalContext)))
 
     def PagedDecodeAttentionQ4(self, attn: MultiHeadAttentionConfig, query, kCodes, kParams, vCodes, vParams, pageTable, ctxLens, output,
                                batch, maxPagesPerSeq, pageCount, pageSize, format, errorFlag=None):
@@ -477,9 +491,9 @@ class Device:
         if attn.ALiBiSlope != 0 or attn.WindowSize != 0:
             raise DeviceError(-6, "paged decode attention (4 bits): no ALiBi and no sliding window")
         kv = attn.KVHeadCount if attn.KVHeadCount > 0 else attn.NumHeads
-        self._call("cuda_dispatch_paged_decode_attention_q4",
-                   [query, kCodes, kParams, vCodes, vParams, pageTable, ctxLens, output, errorFlag],
-                   lambda r: (format, *r, batch, maxPagesPerSeq, pageCount, pageSize, attn.NumHeads, kv, attn.HeadDim, 0))
+        self._call_plain("cuda_dispatch_paged_decode_attention_q4", format,
+                         (query, kCodes, kParams, vCodes, vParams, pageTable, ctxLens, output, errorFlag),
+                         (batch, maxPagesPerSeq, pageCount, pageSize, attn.NumHeads, kv, attn.HeadDim))
 
     def PagedDecodeAttention(self, attn: MultiHeadAttentionConfig, query, kPages, vPages, pageTable, ctxLens, output, batch,
                              maxPagesPerSeq, pageCount, pageSize, format, kvFormat=None, kScale=None, vScale=None, errorFlag=None):
