@@ -888,6 +888,20 @@ __device__ __forceinline__ void ldmatrix_trans(uint32_t at, uint32_t* r) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// sum + 0 * v for two elements: 0 while all are finite, NaN from the first that is not
+template <bool BF16> __device__ __forceinline__ uint32_t times0(uint32_t v, uint32_t sum) {
+    uint32_t d;
+    if (BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(v), "r"(0u), "r"(sum));
+    else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(v), "r"(0u), "r"(sum));
+    return d;
+}
+
 struct ShortParams {
     const uint16_t *q, *k, *v;
     uint16_t* out;
@@ -970,15 +984,22 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(ShortParams p) 
                 // dimension 32G + 8a + 2q + e goes to place 32G + 8q + 2a + e
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
-                    const uint32_t bad = not_finite<BF16>(a[u].w[q]);
-                    found |= bad;
-                    *(uint32_t*)(vTile + ((size_t)r * PIECES + (((c & ~3) + q) ^ (r & 7))) * 16 + (c & 3) * 4) = a[u].w[q] & ~((bad >> 15) * 0xFFFFu);
+                    found = times0<BF16>(a[u].w[q], found);
+                    *(uint32_t*)(vTile + ((size_t)r * PIECES + (((c & ~3) + q) ^ (r & 7))) * 16 + (c & 3) * 4) = a[u].w[q];
                 }
             }
         }
-        if (found) notFinite = 1;
+        if (found & 0x7FFF7FFFu) notFinite = 1;
     }
     __syncthreads();
+    if (notFinite) {
+        for (int i = threadIdx.x; i < padded * PIECES * 4; i += kShortWarps * 32) {
+            uint32_t* const w = (uint32_t*)vTile + i;
+            const uint32_t bad = not_finite<BF16>(*w);
+            *w &= ~((bad >> 15) * 0xFFFFu);
+        }
+        __syncthreads();
+    }
     for (int blk = firstBlock + warp; blk < blocks; blk += stride) {
         const int rA = blk * 16 + g, rB = rA + 8, rows = len * group;
         const int posA = min(rA, rows - 1) / group, posB = min(rB, rows - 1) / group;
@@ -1010,6 +1031,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(ShortParams p) 
         }
         const int seenA = p.causal ? posA + 1 : len, seenB = p.causal ? posB + 1 : len;
         const int last = p.causal ? min(blk * 16 + 15, rows - 1) / group + 1 : len;  // keys that any of the rows sees
+        const int allSee = p.causal ? blk * 16 / group + 1 : len;                    // and that all of them see
         float o[D / 8][4];
 #pragma unroll
         for (int n = 0; n < D / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -1027,22 +1049,27 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(ShortParams p) 
                     mma16(s[n], qa[m].w[2], qb[m].w[2], qa[m].w[3], qb[m].w[3], b.w[2], b.w[3], BF16);
                 }
             }
-            float topA = -INFINITY, topB = -INFINITY;
+            if (key0 + 32 > allSee) {
 #pragma unroll
-            for (int n = 0; n < 4; n++)
+                for (int n = 0; n < 4; n++)
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const int key = key0 + 8 * n + 2 * t + e;
-                    s[n][e] = key < seenA ? s[n][e] * p.scaleLog2 : -INFINITY;
-                    s[n][2 + e] = key < seenB ? s[n][2 + e] * p.scaleLog2 : -INFINITY;
-                    topA = fmaxf(topA, s[n][e]);
-                    topB = fmaxf(topB, s[n][2 + e]);
-                }
+                    for (int e = 0; e < 2; e++) {
+                        const int key = key0 + 8 * n + 2 * t + e;
+                        if (key >= seenA) s[n][e] = -INFINITY;
+                        if (key >= seenB) s[n][2 + e] = -INFINITY;
+                    }
+            }
+            float topA = fmaxf(s[0][0], s[0][1]), topB = fmaxf(s[0][2], s[0][3]);
+#pragma unroll
+            for (int n = 1; n < 4; n++) {
+                topA = max3(topA, s[n][0], s[n][1]);
+                topB = max3(topB, s[n][2], s[n][3]);
+            }
             topA = fmaxf(topA, __shfl_xor_sync(0xffffffffu, topA, 1));
             topB = fmaxf(topB, __shfl_xor_sync(0xffffffffu, topB, 1));
             topA = fmaxf(topA, __shfl_xor_sync(0xffffffffu, topA, 2));
             topB = fmaxf(topB, __shfl_xor_sync(0xffffffffu, topB, 2));
-            const float nA = fmaxf(mA, topA), nB = fmaxf(mB, topB);
+            const float nA = fmaxf(mA, topA * p.scaleLog2), nB = fmaxf(mB, topB * p.scaleLog2);
             const float fromA = nA == -INFINITY ? 0.f : nA, fromB = nB == -INFINITY ? 0.f : nB;  // nothing but scores of -inf so far
             const float aA = ex2_approx(mA - fromA), aB = ex2_approx(mB - fromB);
             mA = nA;
@@ -1062,13 +1089,14 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(ShortParams p) 
             for (int n = 0; n < 4; n++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    s[n][e] = ex2_approx(s[n][e] - fromA);
-                    s[n][2 + e] = ex2_approx(s[n][2 + e] - fromB);
+                    s[n][e] = ex2_approx(fmaf(s[n][e], p.scaleLog2, -fromA));
+                    s[n][2 + e] = ex2_approx(fmaf(s[n][2 + e], p.scaleLog2, -fromB));
                     lA += s[n][e];
                     lB += s[n][2 + e];
                 }
 #pragma unroll
             for (int ks = 0; ks < 2; ks++) {
+                if (ks == 1 && key0 + 16 >= last) break;
                 const uint32_t p0 = pack2<BF16>(s[2 * ks][0], s[2 * ks][1]), p1 = pack2<BF16>(s[2 * ks][2], s[2 * ks][3]);
                 const uint32_t p2 = pack2<BF16>(s[2 * ks + 1][0], s[2 * ks + 1][1]), p3 = pack2<BF16>(s[2 * ks + 1][2], s[2 * ks + 1][3]);
                 const int key = key0 + 16 * ks + (lane & 15);
