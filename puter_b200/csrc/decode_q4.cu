@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
             if (lane < LINES && lane * 64 < heads * D)
                 asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(unused) : "l"(p.q + ((size_t)cb * p.numHeads + head0) * D + lane * 64));
         }
-#pragma unroll
+#pragma unroll 1
         for (int s = 0; s < S::STAGES - 1; s++) issue();
 
         // rows of a tile: row r is token rowTok(r): neighbouring rows differ in the lowest bit of their token, so the K loads of eight lanes
