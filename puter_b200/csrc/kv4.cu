@@ -121,7 +121,8 @@ template <int DT> __device__ __forceinline__ void widen8(const Vec16& v, float* 
 // MODE 0: neighbouring pairs, 1: halves, 2: K comes rotated.
 // Bound: instructions, ~10 per element against the 14 that the memory system leaves time for; every lane has 64 bytes of K and V in flight before it
 // looks at its indices.  59748 rows of 8 KV heads of 128 in bf16, rotated: 70 us for 310 MB, 4.5 TB/s (47 us at the copy rate; issue slots 60 %,
-// logic pipe 49 %); 64 rows 2.7 us.  The next vectors fetched a round ahead made it slower (78 us), more registers per thread changed nothing.
+// logic pipe 49 %); 64 rows 2.7 us.  The next vectors fetched a round ahead made it slower (78 us in
+// registers, 74 through shared memory).
 template <int DT, int D, int MODE>
 __global__ void __launch_bounds__(256) append_kernel(const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
                                                      const int32_t* __restrict__ positions, const int32_t* __restrict__ pageIDs,
