@@ -156,11 +156,11 @@ class Device:
                 self.lib.cuda_buffer_release(old)
             self._refs.clear()
         # a handle that is there was made of CUDA memory; whether this view of it is contiguous is asked every time
-        known, refs = self._refs, []
-        for t in tensors:
-            r = known.get((t.data_ptr(), t.nbytes)) if t is not None and t.is_contiguous() else None
-            refs.append(r if r is not None else self._ref(t))
-        return refs
+        known = self._refs
+        try:
+            return [None if t is None else known[t.data_ptr(), t.nbytes] if t.is_contiguous() else self._ref(t) for t in tensors]
+        except KeyError:  # a handle to be made
+            return [self._ref(t) for t in tensors]
 
     def _call(self, name, tensors, build_args):
         self._enter()
