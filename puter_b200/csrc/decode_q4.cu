@@ -37,8 +37,9 @@
 // on 2 KV heads 40; one of 1024 tokens 12 us, of which 2 are the launch, 2 the prefix, 3 the first copies, 3 the step itself, 2 the joins.
 //
 // Work: the tiles of 16 tokens of all (KV head, sequence) pairs in one list, every pair a few tiles longer for what its start costs, cut into
-// equal contiguous ranges, one per CTA, and each CTA's range into equal ranges, one per warp.  A warp owns its pipeline (stages of 32 tokens, copies running ahead across sequence
-// boundaries, page entries one step further ahead), so there is no block-wide barrier before the end.  Where pages hold whole tiles the
+// equal contiguous ranges, one per CTA, and each CTA's range into equal ranges, one per warp.  A warp owns its pipeline (stages of 32
+// tokens, copies running ahead across sequence boundaries, page entries one step further ahead), so there is no block-wide barrier
+// before the end.  Where pages hold whole tiles the
 // copies are bulk copies, four per tile (codes and params of K and V), each issued by a lane of its own: ~20 instructions per step where
 // 16-byte copies with a page lookup per token take ~90.  A pair that lies inside a warp's range is written by the warp.  Otherwise the warps
 // of a CTA put their partials (maximum, sum, accumulator) together, and the CTAs that share a pair join theirs together: each waits, bounded,
@@ -302,8 +303,12 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
     // Few large pairs (eight CTAs each at least) get whole CTAs, in proportion and rounded: a CTA that ends one pair and begins another is
     // 4 us late, and every owner of both waits for it.  What the rounding adds to a range, each^2 / (2 fewest) tiles or so, is kept
     // to some 64 (3 us of streaming).  Two sequences of 16384 tokens with 32 heads on 2 KV heads 23.7 -> 18.6 us, on 8 24.4 -> 22.0.
-    const bool owned = !aligned && split.each >= 2 * kStart && ts[p.batch + 2] >= 8 * split.each && split.each * split.each <= 128ll * ts[p.batch + 2] && total * (parts + 1ll) >> 32 == 0;
-    auto owner = [&](long long at) { return (int)(((uint32_t)at * parts + (uint32_t)total / 2) / (uint32_t)total); };  // first CTA of the pair that begins at tile `at`
+    // (each >= 2 kStart: the first CTA of a pair has tiles of its own; the products below fit 32 bits)
+    const long long fewest = ts[p.batch + 2];
+    const bool owned = !aligned && split.each >= 2 * kStart && fewest >= 8 * split.each && split.each * split.each <= 128 * fewest &&
+                       total * (parts + 1ll) >> 32 == 0;
+    // first CTA of the pair that begins at tile `at`
+    auto owner = [&](long long at) { return (int)(((uint32_t)at * parts + (uint32_t)total / 2) / (uint32_t)total); };
     long long clo, chi, from = 0;  // from: where the warps' ranges begin
     if (owned) {
         // the last pair whose first CTA is not behind this one: at * parts + total / 2 < (i + 1) * total
@@ -445,7 +450,8 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
         };
         look_ahead();
         {  // the first pair's queries set out with the page entries instead of behind them
-            const int kvh = cUnit / p.blocks, head0 = kvh * p.group + (cUnit - kvh * p.blocks) * S::HEADS, heads = min(p.group - (cUnit - kvh * p.blocks) * S::HEADS, S::HEADS);
+            const int kvh = cUnit / p.blocks, block = cUnit - kvh * p.blocks;
+            const int head0 = kvh * p.group + block * S::HEADS, heads = min(p.group - block * S::HEADS, S::HEADS);
             constexpr int LINES = S::HEADS * D * 2 / 128;
             uint32_t unused;
             if (lane < LINES && lane * 64 < heads * D)
