@@ -175,6 +175,31 @@ def test_bad_rows_and_pages_are_skipped_and_flagged(d):
     assert bool((out[16:32] == 7).all()) and not bool((out[:16] == 7).all()) and not bool((out[32:] == 7).all())
 
 
+def test_offsets_behind_4_gigabytes(d):
+    """Producer, gather and decode attention in the last pages of pools whose byte offsets pass 32 bits."""
+    kv, dim, page, group, fmt, pages = 8, 128, 16, 4, 2, 560000  # 4.6 GB of codes a side
+    g = torch.Generator(device="cuda").manual_seed(61)
+    pools = [torch.empty(pages, kv, page, dim // 2, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    params = [torch.zeros(pages, kv, page, 2, dtype=TYPES[fmt], device="cuda") for _ in range(2)]
+    rows = 40
+    k, v = (torch.randn(rows, kv * dim, device="cuda", generator=g).to(TYPES[fmt]) for _ in range(2))
+    where = [pages - 1, 7, pages - 3]
+    append(d, None, k, v, None, [where[r // page] for r in range(rows)], [r % page for r in range(rows)], pools[0], params[0], pools[1], params[1], fmt)
+    table = torch.tensor([where], dtype=torch.int32, device="cuda")
+    outs = []
+    for codes, par, x in zip(pools, params, (k, v)):
+        out = torch.full((rows, kv * dim), 7.0, dtype=TYPES[fmt], device="cuda")
+        d.KVPageGatherQ4(codes, par, table.view(-1), out, pages, page, kv, dim, rows, fmt)
+        n, step, least = quantise(x.float().cpu().numpy().reshape(rows, kv, dim), fmt)
+        want = torch.from_numpy(least.astype(np.float64) + step.astype(np.float64) * n).to(TYPES[fmt]).reshape(rows, -1)
+        assert torch.equal(out.cpu(), want)
+        outs.append(out)
+    t = (torch.randn(1, kv * group * dim, device="cuda", generator=g).to(TYPES[fmt]), pools[0], params[0], pools[1], params[1], table,
+         torch.tensor([rows], dtype=torch.int32, device="cuda"))
+    check_decode(decode(d, t, kv, dim, page, group, fmt), t, kv, dim, page, group, fmt)
+    assert d.take_error() == 0
+
+
 # ---------------------------------------------------------------------------------------------------------------------- decode
 def make(fmt, lens, kv, dim, page, group, seed, sharp=1.0):
     g = torch.Generator(device="cuda").manual_seed(seed)
@@ -351,6 +376,47 @@ def test_decode_repeats_its_bits_and_replays_from_graphs(d):
             g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(o, w) for o, w in zip(outs, wants))
+    assert d.take_error() == 0
+
+
+def test_two_graphs_of_decode_steps_replayed_at_the_same_time(d):
+    """Each graph has its own scratch; a launch that waits for its other blocks has all of them on the GPU."""
+    shapes = [(8, 128, 16, 4, 2), (2, 128, 16, 16, 1)]
+    ts = [make(2, [3000, 17, 900, 12000], 8, 128, 16, 4, 41), make(1, [5000, 8000], 2, 128, 16, 16, 42)]
+    wants = [decode(d, t, *s) for t, s in zip(ts, shapes)]
+    outs, graphs = [torch.full_like(t[0], 7.0) for t in ts], []
+    torch.cuda.synchronize()
+    for t, s, o in zip(ts, shapes, outs):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            for _ in range(10):
+                decode(d, t, *s, out=o)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, wants)) and d.take_error() == 0
+
+
+def test_a_decode_replay_follows_its_lengths_and_pages(d):
+    """Lengths, page table and queries come from memory: the step grows from token to token, one sequence ends, another is added."""
+    kv, dim, page, group, fmt = 4, 128, 16, 4, 2
+    q, kc, kp, vc, vp, table, ctx = make(fmt, [900, 40, 2000, 16], kv, dim, page, group, 51)
+    table = torch.cat([table, table[:, -1:].repeat(1, 3)], 1)
+    out, graph = torch.full_like(q, 7.0), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        decode(d, (q, kc, kp, vc, vp, table, ctx), kv, dim, page, group, fmt, out=out)
+    for lens in ([900, 40, 2000, 16], [901, 41, 2001, 17], [0, 42, 2002, 0], [1, 2000, 0, 2000], [0, 0, 0, 0]):
+        out.fill_(7)
+        ctx.copy_(torch.tensor(lens, dtype=torch.int32))
+        table.copy_(torch.randint(0, kc.shape[0], table.shape, device="cuda").to(torch.int32))
+        q.copy_(torch.randn(q.shape, device="cuda").to(q.dtype))
+        graph.replay()
+        torch.cuda.synchronize()
+        check_decode(out, (q, kc, kp, vc, vp, table, ctx), kv, dim, page, group, fmt)
     assert d.take_error() == 0
 
 

@@ -332,6 +332,28 @@ def test_capture_makes_the_rope_table_that_is_missing(d):
     assert d.take_error() == 0
 
 
+@pytest.mark.parametrize("longest", [600, 128])  # the tile kernel, the kernel for short sequences
+def test_a_replay_follows_other_lengths(d, longest):
+    """Lengths come from memory: a captured call of up to `longest` tokens per sequence serves other batches of its size, empty ones too."""
+    import puter_b200
+
+    rope = puter_b200.RoPEConfig(Mode=1, BaseFreq=10000.0)
+    total = 700
+    q, k, v, _ = make(2, [total], 8, 2, 128, 9)
+    starts = torch.zeros(7, dtype=torch.int32, device="cuda")
+    out, graph = torch.full_like(q, 7.0), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        call(d, q, k, v, starts, 8, 2, 128, 2, rope=rope, longest=longest, out=out)
+    for at in ([0, 100, 100, 228, 230, 231, 300], [5, 5, 5, 5, 5, 5, 5], [0, 1, 2, 3, 131, 259, 259 + min(longest, 441)], [700 - longest, 700, 700, 700, 700, 700, 700]):
+        out.fill_(7)
+        starts.copy_(torch.tensor(at, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out, q, k, v, starts, 8, 2, 128, 2, True, rope)
+    assert d.take_error() == 0
+
+
 def test_two_streams_of_one_capture(d):
     """Both calls use the scratch of the capture: the graph orders them, whatever the program's own streams leave open."""
     ts = [make(2, [300, 20], 8, 2, 128, 1), make(2, [250, 90], 8, 2, 128, 2)]
