@@ -332,6 +332,23 @@ def test_capture_makes_the_rope_table_that_is_missing(d):
     assert d.take_error() == 0
 
 
+@pytest.mark.parametrize("length", [300, 60])  # the tile kernel, the kernel for short sequences
+def test_rows_behind_2_to_the_31_elements(d, length):
+    import puter_b200
+
+    heads, kv, dim, total = 32, 8, 128, 530000  # 2.17e9 elements of q
+    rope = puter_b200.RoPEConfig(Mode=1, BaseFreq=10000.0)
+    q, k, v = (torch.zeros(total, h * dim, dtype=torch.bfloat16, device="cuda") for h in (heads, kv, kv))
+    live = 3 * length
+    for t in (q, k, v):
+        t[-live:].normal_()
+    starts = torch.tensor([total - live, total - 2 * length - 7, total - length, total], dtype=torch.int32, device="cuda")
+    out = call(d, q, k, v, starts, heads, kv, dim, 2, rope=rope, longest=length + 7)
+    tail = [t[-live:].clone() for t in (q, k, v)]
+    check(out[-live:], *tail, starts - (total - live), heads, kv, dim, 2, True, rope)
+    assert bool((out[:4096] == 7).all()) and bool((out[-live - 4096:-live] == 7).all()) and d.take_error() == 0
+
+
 @pytest.mark.parametrize("longest", [600, 128])  # the tile kernel, the kernel for short sequences
 def test_a_replay_follows_other_lengths(d, longest):
     """Lengths come from memory: a captured call of up to `longest` tokens per sequence serves other batches of its size, empty ones too."""
