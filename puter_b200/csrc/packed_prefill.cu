@@ -874,7 +874,10 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
 // V with the dimensions of 32 reordered so that a lane's accumulators are eight neighbouring dimensions, piece ^ (row & 7) for the
 // transposing loads.
 constexpr int kShortMax = 160;
-constexpr int kShortWarps = 4;
+// Warps of a block.  The registers of 128 dimensions leave room for twelve warps on an SM: two blocks of six share K and V more often than three
+// of four (30 sequences of up to 160 tokens, 16 heads 52 -> 42 us, one of 33 tokens 7.4 -> 7.1, 64 of up to 32 14.3 -> 14.7; eight: 53, 6.9, 19.3).
+// With 64 dimensions four: 200 sequences of up to 96 tokens 21.2 us, 64 of 128 26.5 (three: 20.2 and 32.8, six: 24.7 and 28).
+template <int D> constexpr int kShortWarps = D == 128 ? 6 : 4;
 
 __device__ __forceinline__ void mma16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, bool bf16) {
     if (bf16)
@@ -912,8 +915,9 @@ struct ShortParams {
 };
 
 template <bool BF16, int D>
-__global__ void __launch_bounds__(kShortWarps * 32) short_kernel(ShortParams p) {
+__global__ void __launch_bounds__(kShortWarps<D> * 32) short_kernel(ShortParams p) {
     constexpr int PIECES = D / 8;  // 16-byte pieces of a row
+    constexpr int WARPS = kShortWarps<D>;
     extern __shared__ __align__(128) unsigned char smemShort[];
     __shared__ int notFinite;
     int row0, end;
@@ -921,11 +925,11 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(ShortParams p) 
     const int len = end - row0, group = p.heads / p.kvHeads, kvh = blockIdx.y;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int blocks = (len * group + 15) / 16;  // of 16 rows
-    const int firstBlock = blockIdx.z * kShortWarps;
+    const int firstBlock = blockIdx.z * WARPS;
     if (firstBlock >= blocks) return;
     // keys that this block's rows see
-    const int stride = gridDim.z * kShortWarps;
-    const int lastBlock = firstBlock + (blocks - 1 - firstBlock) / stride * stride + kShortWarps - 1;
+    const int stride = gridDim.z * WARPS;
+    const int lastBlock = firstBlock + (blocks - 1 - firstBlock) / stride * stride + WARPS - 1;
     const int keys = p.causal ? min(len, (min(lastBlock * 16 + 15, len * group - 1)) / group + 1) : len;
     const int padded = (keys + 31) & ~31;
     unsigned char* const kTile = smemShort;
@@ -936,7 +940,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(ShortParams p) 
     const bool halves = p.ropeMode == 1;
     {
         // (four pieces of a thread are on their way before the first is used: the loop waits for memory once, not per piece)
-        constexpr int KP = PIECES / 2, THREADS = kShortWarps * 32, U = 4;  // a thread takes pieces c and c + KP of a K row: partners in half mode
+        constexpr int KP = PIECES / 2, THREADS = WARPS * 32, U = 4;  // a thread takes pieces c and c + KP of a K row: partners in half mode
         for (int i0 = threadIdx.x; i0 < padded * KP; i0 += U * THREADS) {
             Vec16 a[U], b[U];
 #pragma unroll
@@ -993,7 +997,7 @@ __global__ void __launch_bounds__(kShortWarps * 32) short_kernel(ShortParams p) 
     }
     __syncthreads();
     if (notFinite) {
-        for (int i = threadIdx.x; i < padded * PIECES * 4; i += kShortWarps * 32) {
+        for (int i = threadIdx.x; i < padded * PIECES * 4; i += WARPS * 32) {
             uint32_t* const w = (uint32_t*)vTile + i;
             const uint32_t bad = not_finite<BF16>(*w);
             *w &= ~((bad >> 15) * 0xFFFFu);
@@ -1186,8 +1190,9 @@ static int short_launch(Context* ctx, const Call& c, CUDAStatus* status) {
     const uint32_t group = c.heads / c.kvHeads, D = c.dim > 64 ? 128 : 64;
     ShortParams p{(const uint16_t*)c.q, (const uint16_t*)c.k, (const uint16_t*)c.v, (uint16_t*)c.out, c.seqs, c.cosT, c.sinT, (int)c.heads, (int)c.kvHeads,
                   (int)c.dim, (int)c.causal, (int)c.ropeMode, (c.seqs.maxLen + 31) & ~31, (float)(1.4426950408889634 / sqrt((double)c.dim))};
-    // several blocks per (sequence, KV head) while there are too few to fill the GPU twice; each has four blocks of 16 rows at least
-    const size_t pairs = (size_t)c.seqs.batch * c.kvHeads, most = ((size_t)c.seqs.maxLen * group + 16 * kShortWarps - 1) / (16 * kShortWarps);
+    const size_t warps = D == 128 ? kShortWarps<128> : kShortWarps<64>;
+    // several blocks per (sequence, KV head) while there are too few to fill the GPU twice; each has 16 rows per warp at least
+    const size_t pairs = (size_t)c.seqs.batch * c.kvHeads, most = ((size_t)c.seqs.maxLen * group + 16 * warps - 1) / (16 * warps);
     size_t split = (2 * (size_t)ctx->smCount + pairs - 1) / pairs;
     if (split > most) split = most;
     if (split > 65535) split = 65535;
@@ -1196,7 +1201,7 @@ static int short_launch(Context* ctx, const Call& c, CUDAStatus* status) {
 #define SHORT(D)                                                                                                                        \
     do {                                                                                                                                \
         allow_smem<short_kernel<BF16, D>>(ctx->device, kShortMax * D * 4);                                                              \
-        short_kernel<BF16, D><<<grid, kShortWarps * 32, smem, ctx->stream>>>(p);                                                        \
+        short_kernel<BF16, D><<<grid, kShortWarps<D> * 32, smem, ctx->stream>>>(p);                                                        \
     } while (0)
     if (D == 128) SHORT(128);
     else SHORT(64);
