@@ -1176,13 +1176,24 @@ static bool tiles_take(const Call& c) {
     return (all & 15u) == 0 && encode_fn() != nullptr;
 }
 
-// By rows per (sequence, KV head), measured on both sides (us, short against tiles): 200 sequences of up to 96 rows 22 : 72, 64 of 128 rows 26 : 36,
-// of 256 rows (64 tokens, group 4) 50 : 42; and where all blocks of 64 rows fit the SMs at once the short latency decides: one sequence of
-// 33 tokens 7.7 : 13.8, of 128 12.5 : 14.9, of 256 20.9 : 16.6.
-static bool short_takes(Context* ctx, const Call& c) {
+// heads of a group that share a tile: the largest power of two in the group
+static int pack_log(uint32_t group) {
+    int log = 0;
+    while (log < 7 && group % (2u << log) == 0) log++;
+    return log;
+}
+
+// Measured on both sides (us, short against tiles).  64 dimensions, up to 160 tokens: short wins throughout (64 sequences of 160, 4 heads per KV
+// head 33 : 42; 300 of 64, 12 KV heads 50 : 130; 64 of 160, 16 heads on one KV head 38 : 37).  128 dimensions, by rows (tokens x heads of a group) per sequence
+// and KV head: 160 7.9 : 15.2 and 23 : 42, 192 28 : 43, 36 : 46 and 20 : 23, 256 54 : 43 and 163 : 134, 384 59 : 56, so up to 192; more where a
+// group that is no power of two fills the tiles to a third at most (7 heads, 252 rows 18 : 77), or where few blocks let the shorter latency
+// decide: one sequence of 128 tokens (8 x 512 rows) 12.4 : 13.2, of 160 13.8 : 13.6.
+static bool short_takes(const Call& c) {
     if (!tiles_take(c) || c.seqs.maxLen > kShortMax || c.kvHeads > 65535 || (c.ropeMode != 2 && c.dim != 64 && c.dim != 128)) return false;
     const size_t rows = (size_t)c.seqs.maxLen * (c.heads / c.kvHeads), pairs = (size_t)c.seqs.batch * c.kvHeads;
-    return rows <= 160 || (c.seqs.maxLen <= 128 && pairs * rows <= 64 * (size_t)ctx->smCount);
+    const int pack = pack_log(c.heads / c.kvHeads), span = 2 * (kRows >> pack);
+    const size_t tileRows = ((size_t)c.seqs.maxLen + span - 1) / span * (c.heads / c.kvHeads >> pack) * 2 * kRows;
+    return c.dim <= 64 || rows <= 192 || 3 * rows <= tileRows || pairs * rows <= 4096;
 }
 
 template <bool BF16>
@@ -1213,9 +1224,7 @@ template <bool BF16>
 static int tiles_launch(Context* ctx, const Call& c, CUDAStatus* status) {
     constexpr int DT = BF16 ? DT_BF16 : DT_F16;
     const uint32_t group = c.heads / c.kvHeads;
-    int packLog = 0;
-    while (packLog < 7 && group % (2u << packLog) == 0) packLog++;
-    const int span = 2 * (kRows >> packLog);
+    const int packLog = pack_log(group), span = 2 * (kRows >> packLog);
     const uint32_t total = (uint32_t)c.seqs.total;
     const size_t levels = ((size_t)c.seqs.maxLen + span - 1) / span, most = (size_t)total / span + c.seqs.batch;  // entries at most
     const bool fused = c.ropeMode != 2 && (c.dim == 64 || c.dim == 128);  // q is rotated in its tile: a pass over q would cost as much as reading it all
@@ -1335,7 +1344,7 @@ extern "C" int cuda_dispatch_rope_packed_attention_prefill(CUDADeviceRef context
         if (!table) return status ? status->code : -7;
     }
     const pk::Call c{elementDType, q, k, v, out, seqs, numHeads, kvHeads, headDim, causal ? 1u : 0u, ropeMode, table, sinT};
-    if (pk::short_takes(ctx, c)) return elementDType == DT_BF16 ? pk::short_launch<true>(ctx, c, status) : pk::short_launch<false>(ctx, c, status);
+    if (pk::short_takes(c)) return elementDType == DT_BF16 ? pk::short_launch<true>(ctx, c, status) : pk::short_launch<false>(ctx, c, status);
     if (pk::tiles_take(c)) return elementDType == DT_BF16 ? pk::tiles_launch<true>(ctx, c, status) : pk::tiles_launch<false>(ctx, c, status);
     const int cap = ctx->smCount * 8;
     if (ropeMode != 2) {
