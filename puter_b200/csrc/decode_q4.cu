@@ -744,8 +744,9 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
                 exponentials();
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) most += J == 2 ? eSum[nt][0] + eSum[nt][J - 1] : eSum[nt][0];
-                // (sums in the place of maxima: they run on another pipe than the logic instructions and cover the maxima)
-                if (__any_sync(0xffffffffu, most > limit || vSum > 2 * MT * veUp)) {
+                // (sums in the place of maxima: they run on another pipe than the logic instructions and cover the maxima.  A sum over the heads of a
+                // lane that is NaN says nothing of the others: it counts as too large)
+                if (__any_sync(0xffffffffu, !(most <= limit) || vSum > 2 * MT * veUp)) {
                     float vTop = 0.f;
 #pragma unroll
                     for (int i = 0; i < 2 * MT; i++) vTop = fmaxf(vTop, vs[i]);
