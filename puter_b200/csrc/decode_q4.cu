@@ -21,9 +21,12 @@
 //     words of two tokens, then the same masks.
 //   * Up to four query heads per KV head (QUAD): the scores are integer products.  As bytes the codes need no conversion at all: F is the word
 //     as it lies in memory and L one mask per word (16 logic instructions per step and lane where the f16 form needs 80), and
-//     the four unused columns take the lower bytes of the queries' integers, so that a lane has whole scores of one head.  The integers
-//     hold a query to 2^-16 of its largest element.  More heads take the f16 form: queries as f16, scaled by a power of two per
-//     (sequence, head) so that a bf16 query of any size fits.
+//     the four unused columns take the lower bytes of the queries' integers, so that a lane has whole scores of one head.  Two bytes hold a
+//     query to 2^-16 of its largest element, three to 2^-24.  What two leave shows where one channel is far larger than the others (norm of
+//     the output's error, channel 50 / 200 / 1000 times as large): bf16 1.8 / 2.5 / 3.5e-3 with two and 1.6 / 1.7 / 1.6e-3 with three, both below the
+//     half step of its rounding (2^-8); f16 9 / 23 / 26e-4 with two, 2e-4 with three, its half step being 4.9e-4.  The third byte costs a product per
+//     tile and 16 bytes of queries (64 sequences of 512 to 32768 tokens: bf16 110 -> 117 us, f16 132 -> 135).  So f16 takes three bytes, bf16
+//     two.  More heads take the f16 form: queries as f16, scaled by a power of two per (sequence, head) so that a bf16 query of any size fits.
 //   * The weights p_t * step_t enter as f16, relative to a running power of two about the largest step, which joins the running maximum of
 //     the softmax in rescaling the accumulator.  Their rounding (half a step of 2^-11) multiplies codes of 0 .. 15, more than the
 //     values themselves amount to: 2^-10 of the output, measured, unseen in a bf16 output and five times the rounding of an f16 one.  For
@@ -260,6 +263,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
     constexpr int ROW = S::ROW;
     constexpr bool QUAD = S::QUAD;
     constexpr bool SPLIT = DT == DT_F16;  // weights in two parts
+    constexpr bool FINE = QUAD && DT == DT_F16;  // queries as integers of three bytes
     constexpr int J = QUAD ? 1 : 2;  // heads of a lane: t, or 8nt + 2t and 8nt + 2t + 1
     constexpr int kPart = S::HEADS * D * 4 + S::HEADS * 8;  // a partial in shared memory: accumulators, then (maximum, sum)
     static_assert(kPart <= S::STAGES * S::STAGE, "a warp's partial takes the place of its stages");
@@ -270,6 +274,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
     __shared__ int sB[32], sUnit[32], sWhere[32];  // of an entry: sequence, unit; pair inside the CTA's range (2) or begun before it (0) or going on behind it (1)
     __shared__ int sShared[2], sFirst[2], sOwners[2], sGo[2];  // pairs shared with other CTAs: entry, first owner, owners, whether to join
     __shared__ __align__(8) uint64_t sBar[S::WARPS * S::STAGES];
+    __shared__ uint4 sTop[FINE ? S::WARPS * 32 : 1];
     const int* ts = p.tileStart;
     if (!ts) {
         block_prefix(p, kStart, sStart, sCtx);
@@ -489,11 +494,13 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
             const int head0 = kvh * p.group + block * S::HEADS, heads = min(p.group - block * S::HEADS, S::HEADS);
 
             // ---- queries, and their sums for the least terms.
-            // QUAD: integers Q = q 32600 / max |q| (an error of 2^-16 of the largest element), in signed bytes.  With L and F as above,
-            // 16 q . n = sum (16 Q_even - Q_odd) L + Q_odd F: three and two bytes.  Column 2h takes the middle byte of head h and column 2h + 1 the
-            // lowest, so a lane finds both in its two accumulators; the top byte has products of its own.
+            // QUAD: integers Q = q kUnits / max |q|, in signed bytes.  With L and F as above, 16 q . n = sum (16 Q_even - Q_odd) L + Q_odd F:
+            // three and two bytes, FINE four and three.  Column 2h takes byte 1 of head h and column 2h + 1 byte 0, so a lane finds both in its two
+            // accumulators; bytes 2 and 3 have products of their own.
             // Otherwise: f16 fragments in the order of the masks, scaled by 2^-qe (and by 1/16 where the codes come 16-fold). ----
-            uint32_t qb[WK][NT][4];  // f16: [word][block of heads][dims (0,4), (2,6), (1,5), (3,7)]; QUAD: [word][0][bytes for L, top for L, for F]
+            constexpr float kUnits = FINE ? 8300000.f : 32600.f;  // three signed bytes hold 127 * 65793, two 127 * 257
+            uint32_t qb[WK][NT][4];  // f16: [word][block of heads][dims (0,4), (2,6), (1,5), (3,7)]; QUAD: [word][0][bytes 1, 0 for L, bytes 2, 3 for L, bytes 1, 0 for F]
+            uint32_t* const topF = (uint32_t*)(sTop + (FINE ? threadIdx.x : 0));  // FINE: byte 2 for F, this thread's words (there is no register for them)
             float qScale[NT][J], qSum[NT][J];
             if (QUAD) {
                 float x[WK][8], big = 0.f, sum = 0.f;
@@ -518,21 +525,24 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
                 big = fminf(fmaxf(big, 1e-30f), 1e36f);
-                const float toInt = 32600.f / big;
+                const float toInt = kUnits / big;
 #pragma unroll
                 for (int w = 0; w < WK; w++) {
+                    uint32_t last = 0;
                     qb[w][0][0] = qb[w][0][1] = qb[w][0][2] = 0;
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int even = __float2int_rn(x[w][2 * i] * toInt);
                         int odd = __float2int_rn(x[w][2 * i + 1] * toInt), mix = 16 * even - odd;
-                        const uint32_t m0 = limb(mix), m1 = limb(mix), o0 = limb(odd);
+                        const uint32_t m0 = limb(mix), m1 = limb(mix), m2 = FINE ? limb(mix) : (uint32_t)mix & 255u, o0 = limb(odd), o1 = FINE ? limb(odd) : (uint32_t)odd & 255u;
                         qb[w][0][0] |= ((g & 1) ? m0 : m1) << (8 * i);
-                        qb[w][0][1] |= ((g & 1) ? 0u : (uint32_t)mix & 255u) << (8 * i);
-                        qb[w][0][2] |= ((g & 1) ? o0 : (uint32_t)odd & 255u) << (8 * i);
+                        qb[w][0][1] |= ((g & 1) ? (FINE ? (uint32_t)mix & 255u : 0u) : m2) << (8 * i);
+                        qb[w][0][2] |= ((g & 1) ? o0 : o1) << (8 * i);
+                        last |= ((g & 1) ? 0u : (uint32_t)odd & 255u) << (8 * i);
                     }
+                    if (FINE) topF[w] = last;
                 }
-                qScale[0][0] = __shfl_sync(0xffffffffu, big * (p.scaleLog2 / (16.f * 32600.f * 4096.f)), 8 * t);
+                qScale[0][0] = __shfl_sync(0xffffffffu, big * (p.scaleLog2 / (16.f * kUnits * 4096.f)), 8 * t);
                 qSum[0][0] = __shfl_sync(0xffffffffu, sum * p.scaleLog2, 8 * t);
             } else {
 #pragma unroll
@@ -644,7 +654,10 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
                     }
                     // (tiles innermost: the products of a tile wait for one another)
                     if (QUAD) {
-                        int mid[MT][4], top[MT][4];  // 256 and 1 times a sum; 65536 times a sum
+                        int mid[MT][4], top[MT][4];  // 256 and 1 times a sum; 65536 and (FINE) 65536 * 256 times a sum
+                        uint32_t qt[4] = {};
+                        if (FINE && WK == 4) *(uint4*)qt = *(const uint4*)topF;
+                        else if (FINE) *(uint2*)qt = *(const uint2*)topF;
 #pragma unroll
                         for (int w = 0; w < WK; w += 2) {
 #pragma unroll
@@ -660,12 +673,16 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
                                     imma(top[mt], x0, y0, x1, y1, qb[w][0][1], qb[w + 1][0][1]);
                                 }
                                 imma(mid[mt], x[0], y[0], x[1], y[1], qb[w][0][2], qb[w + 1][0][2]);
+                                if (FINE) imma(top[mt], x[0], y[0], x[1], y[1], qt[w], qt[w + 1]);
                             }
                         }
 #pragma unroll
-                        for (int mt = 0; mt < MT; mt++) {  // at most 16 * 32600 * 15 * 128 < 2^30
-                            se[mt][0][0] = (float)(top[mt][0] * 65536 + mid[mt][0] * 256 + mid[mt][1]);
-                            se[mt][0][2] = (float)(top[mt][2] * 65536 + mid[mt][2] * 256 + mid[mt][3]);
+                        for (int mt = 0; mt < MT; mt++) {
+#pragma unroll
+                            for (int i = 0; i < 4; i += 2)
+                                // FINE: at most 64 * 128 * 270 * 257 < 2^30 in the lower half, 2^22 in the upper; otherwise 16 * 32600 * 15 * 128 < 2^30 in all
+                                se[mt][0][i] = FINE ? fmaf((float)(top[mt][i + 1] * 256 + top[mt][i]), 65536.f, (float)(mid[mt][i] * 256 + mid[mt][i + 1]))
+                                                    : (float)(top[mt][i] * 65536 + mid[mt][i] * 256 + mid[mt][i + 1]);
                         }
                     } else
 #pragma unroll

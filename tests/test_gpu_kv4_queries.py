@@ -3,7 +3,7 @@ the values and the scores."""
 import pytest
 import torch
 
-from test_gpu_kv4 import check_decode, decode, make
+from test_gpu_kv4 import check_decode, decode, make, values64
 
 pytestmark = pytest.mark.gpu
 
@@ -44,4 +44,24 @@ def test_a_query_that_is_not_finite_spoils_its_own_head_only(d, fmt, bad, kv, gr
     assert bool(got[:, :, first].isnan().all())
     got[:, :, first] = clean.view(-1, kv, group, dim)[:, :, first]
     check_decode(got.view(q.shape), t, kv, dim, page, group, fmt)
+    assert d.take_error() == 0
+
+
+@pytest.mark.parametrize("fmt", [2, 1])
+@pytest.mark.parametrize("kv,group,dim", [(8, 4, 128), (4, 1, 64), (2, 8, 128)])
+@pytest.mark.parametrize("strong", [1, 50, 200, 1000])
+def test_a_strong_channel_in_the_query(d, fmt, kv, group, dim, strong):
+    """One channel far larger than the others leaves the output as near as its rounding, half a step of the type (2^-11, 2^-8), in the norm over a
+    sequence's heads; float32 scores of magnitude S and their exponentials: 2^-22 S of the values."""
+    t = make(fmt, [3000, 700, 40, 1], kv, dim, 16, group, 3)
+    q, kc, kp, vc, vp, table, ctx = t
+    q.view(4, -1, dim)[:, :, 7] *= strong
+    got = decode(d, t, kv, dim, 16, group, fmt)
+    u = float(torch.finfo(q.dtype).eps) / 2
+    for b, n in enumerate(ctx.tolist()):
+        pages = table[b, :-(-n // 16)].long()
+        k, v = values64(kc, kp, pages, n), values64(vc, vp, pages, n)
+        s = torch.einsum("hgd,nhd->hgn", q[b].double().view(kv, group, dim), k) / dim ** 0.5
+        want = torch.einsum("hgn,nhd->hgd", torch.softmax(s, -1), v).reshape(-1)
+        assert float((got[b].double() - want).norm()) <= u * float(want.norm()) + 2.0 ** -22 * float(s.abs().max()) * float(v.abs().max()) * want.numel() ** 0.5
     assert d.take_error() == 0
