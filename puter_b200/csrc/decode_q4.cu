@@ -524,7 +524,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
                 big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                big = fminf(fmaxf(big, 1e-30f), 1e36f);
+                big = fminf(fmaxf(big, 1e-34f), 3.38e38f);  // kUnits / big stays finite; smaller queries than that lose their lower bits
                 const float toInt = kUnits / big;
 #pragma unroll
                 for (int w = 0; w < WK; w++) {
@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
                     }
                     if (FINE) topF[w] = last;
                 }
-                qScale[0][0] = __shfl_sync(0xffffffffu, big * (p.scaleLog2 / (16.f * kUnits * 4096.f)), 8 * t);
+                qScale[0][0] = __shfl_sync(0xffffffffu, big * (p.scaleLog2 / (16.f * kUnits)), 8 * t);
                 qSum[0][0] = __shfl_sync(0xffffffffu, sum * p.scaleLog2, 8 * t);
             } else {
 #pragma unroll
@@ -723,10 +723,11 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
                     const uint32_t at = params + (8 * i + tokG) * 4;
                     unpack16_arith<DT>(lds32(at), ks[i], kl[i]);
                     unpack16_arith<DT>(lds32(at + kStep * 4), vs[i], vl[i]);
-                    ks[i] *= 4096.f;
+                    if (!QUAD) ks[i] *= 4096.f;  // (the other half of 2^24: see `up`)
                     vSum += vs[i];
                 }
-                // ---- scores in the log2 domain, relative to the reference, and their exponentials ----
+                // ---- scores in the log2 domain, relative to the reference, and their exponentials (sums times the query's scale first: that is
+                // the size of q . n, while either factor alone may be far from 1) ----
                 float x[NT][J][2 * MT], e[NT][J][2 * MT], eSum[NT][J], most = 0.f;
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
@@ -734,7 +735,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
                     for (int j = 0; j < J; j++) {
 #pragma unroll
                         for (int i = 0; i < 2 * MT; i++)
-                            x[nt][j][i] = fmaf(se[i >> 1][nt][2 * (i & 1) + j] * ks[i], qScale[nt][j], fmaf(kl[i], qSum[nt][j], -from[nt][j]));
+                            x[nt][j][i] = fmaf(se[i >> 1][nt][2 * (i & 1) + j] * qScale[nt][j], ks[i], fmaf(kl[i], qSum[nt][j], -from[nt][j]));
                     }
                 }
                 if (tail) {

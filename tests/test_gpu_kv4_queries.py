@@ -65,3 +65,17 @@ def test_a_strong_channel_in_the_query(d, fmt, kv, group, dim, strong):
         want = torch.einsum("hgn,nhd->hgd", torch.softmax(s, -1), v).reshape(-1)
         assert float((got[b].double() - want).norm()) <= u * float(want.norm()) + 2.0 ** -22 * float(s.abs().max()) * float(v.abs().max()) * want.numel() ** 0.5
     assert d.take_error() == 0
+
+
+@pytest.mark.parametrize("kv,group,dim", [(2, 4, 128), (3, 1, 64), (2, 8, 128), (1, 16, 64)])
+@pytest.mark.parametrize("power", [121, 60, -60, -110])
+def test_queries_keys_and_values_of_any_size_in_bf16(d, power, kv, group, dim):
+    """Queries times 2^power, keys times 2^-power: the scores are those of ordinary numbers.  Values times 2^power then."""
+    t = make(2, [300, 20, 1], kv, dim, 16, group, 6)
+    t[0].mul_(2.0 ** power)
+    t[2].mul_(2.0 ** -power)
+    check_decode(decode(d, t, kv, dim, 16, group, 2), t, kv, dim, 16, group, 2)
+    if power > -100:  # (a value of 2^-110 takes part as a subnormal weight: not this format's business)
+        t[4].mul_(2.0 ** min(power, 100))
+        check_decode(decode(d, t, kv, dim, 16, group, 2), t, kv, dim, 16, group, 2)
+    assert d.take_error() == 0
