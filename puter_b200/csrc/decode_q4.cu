@@ -63,6 +63,7 @@ constexpr int kTile = 16;             // tokens per tile
 constexpr int kPrefixSmem = 1024;     // sequences whose tile prefix sums fit shared memory
 constexpr int kStageBytes = 209 * 1024;  // of shared memory for the copies in flight: three steps of 16 warps or of 8 with twice the tokens
 constexpr int kWarpTiles = 2;         // tiles that a warp gets at least before another CTA takes part
+constexpr int kMostTokens = INT_MAX - 255;  // of a context: places two steps behind its last token still fit 31 bits
 
 struct Params {
     const uint16_t* q;
@@ -1137,6 +1138,7 @@ __global__ void __launch_bounds__(S::WARPS * 32, 1) decode_kernel(Params p) {
 
 template <int DT, typename S>
 static int launch(Context* ctx, Params& p, CUDAStatus* status) {
+    static_assert(2 * S::STEP <= INT_MAX - kMostTokens, "places behind the context are counted in 31 bits");
     const char* what = "paged decode attention (4 bits)";
     const unsigned grid = (unsigned)ctx->smCount;
     p.blocks = (p.group + S::HEADS - 1) / S::HEADS;
@@ -1200,7 +1202,7 @@ extern "C" int cuda_dispatch_paged_decode_attention_q4(CUDADeviceRef contextRef,
     if (pageSize == 0 || pageCount == 0 || maxPagesPerSeq == 0) return fail(status, -2, "%s: empty page geometry", what);
     if ((size_t)batch * numHeads > 0x7FFFFFFFull) return fail(status, -2, "%s: %u sequences of %u heads exceed 31 bits", what, batch, numHeads);
     const size_t slots = pool_vectors(pageCount, pageSize, kvHeads);
-    if (slots > 0xFFFFFFFFull || (size_t)maxPagesPerSeq * pageSize > 0x7FFFFFE0ull || batch > 0x7FFFFFFEu)
+    if (slots > 0xFFFFFFFFull || (size_t)maxPagesPerSeq * pageSize > (size_t)q4d::kMostTokens || batch > 0x7FFFFFFEu)
         return fail(status, -2, "%s: a pool of %zu vectors or a context of %zu tokens exceeds the index range", what, slots,
                     (size_t)maxPagesPerSeq * pageSize);
     if ((size_t)batch * ((size_t)maxPagesPerSeq * pageSize / q4d::kTile + 16) > 0x7FFFFFFFull)  // tiles are counted in 31 bits
