@@ -1191,6 +1191,7 @@ static int pack_log(uint32_t group) {
 static bool short_takes(const Call& c) {
     if (!tiles_take(c) || c.seqs.maxLen > kShortMax || c.kvHeads > 65535 || (c.ropeMode != 2 && c.dim != 64 && c.dim != 128)) return false;
     const size_t rows = (size_t)c.seqs.maxLen * (c.heads / c.kvHeads), pairs = (size_t)c.seqs.batch * c.kvHeads;
+    if (rows > 1u << 30) return false;  // a block counts its rows in 31 bits
     const int pack = pack_log(c.heads / c.kvHeads), span = 2 * (kRows >> pack);
     const size_t tileRows = ((size_t)c.seqs.maxLen + span - 1) / span * (c.heads / c.kvHeads >> pack) * 2 * kRows;
     return c.dim <= 64 || rows <= 192 || 3 * rows <= tileRows || pairs * rows <= 4096;
@@ -1320,6 +1321,8 @@ extern "C" int cuda_dispatch_rope_packed_attention_prefill(CUDADeviceRef context
         if (headDim % 2 != 0) return fail(status, -2, "rope: head dimension must be even");
     }
     if (maxSeqLen > totalTokens) maxSeqLen = totalTokens;
+    if ((size_t)numHeads * headDim > 0x7FFFFFFFull)  // the kernels count within a row in 31 bits
+        return fail(status, -2, "%s: rows of %u heads of %u exceed 31 bits", what, numHeads, headDim);
     if ((size_t)totalTokens * numHeads > (size_t)1 << 48) return fail(status, -2, "%s: %u tokens of %u heads", what, totalTokens, numHeads);
     const size_t es = dtype_size(elementDType), qBytes = (size_t)totalTokens * numHeads * headDim * es,
                  kvBytes = (size_t)totalTokens * kvHeads * headDim * es;
