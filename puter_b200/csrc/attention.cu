@@ -22,7 +22,7 @@ bool decode_supported(int dt, int kvDT, uint32_t numHeads, uint32_t kvHeads, uin
 bool prefill_supported(int dt, uint32_t seqQ, uint32_t seqK, uint32_t numHeads, uint32_t kvHeads, uint32_t headDim, uint32_t causal);
 int launch_prefill(Context* ctx, int dt, const void* q, const void* k, const void* v, void* out, uint32_t batch, uint32_t seqLen,
                    uint32_t numHeads, uint32_t kvHeads, uint32_t headDim, uint32_t causal, int ropeMode, const float* ropeTable,
-                   CUDAStatus* status);
+                   void* kRotated, CUDAStatus* status);
 int validate_rope(CUDAStatus* status, double base, uint32_t halfMode, uint32_t scaling, double factor, double low, double high,
                   uint32_t origCtx);
 const float* cached_rope_table(Context* ctx, size_t seqLen, int headDim, double base, long long startPos, int scaling, double factor,
@@ -60,7 +60,7 @@ extern "C" int cuda_dispatch_multi_head_attention(CUDADeviceRef contextRef, int 
                                        0, (seqK + 15) / 16, 16, numHeads, kvHeads, 0, (long long)((seqK + 15) / 16), nullptr, status);
         }
         if (prefill_supported(elementDType, seqQ, seqK, numHeads, kvHeads, headDim, causal))
-            return launch_prefill(ctx, elementDType, q, k, v, o, 1, seqQ, numHeads, kvHeads, headDim, causal, 2, nullptr, status);
+            return launch_prefill(ctx, elementDType, q, k, v, o, 1, seqQ, numHeads, kvHeads, headDim, causal, 2, nullptr, nullptr, status);
     }
     return launch_mha_exact(ctx, elementDType, q, k, v, o, seqQ, seqK, numHeads, kvHeads, headDim, causal, windowSize, status);
 }
@@ -103,14 +103,17 @@ extern "C" int cuda_dispatch_rope_attention_prefill(CUDADeviceRef contextRef, in
 
     if (!ctx->exact && aligned && prefill_supported(elementDType, seqLen, seqLen, numHeads, kvHeads, headDim, causal)) {
         const float* table = nullptr;
+        Scratch kRotated{};
         if (ropeMode != 2) {
             // scratch for the rotated K; the cos/sin table comes from the context's cache
-            if (!ensure_workspace(ctx, batch * kvElems * es + 1024, status)) return status ? status->code : -7;
+            int rc = call_scratch(ctx, batch * kvElems * es, 0, &kRotated, status);
+            if (rc != 0) return rc;
             table = cached_rope_table(ctx, seqLen, (int)headDim, baseFreq, (long long)startPosition, (int)scaling, scalingFactor,
                                       lowFreqFactor, highFreqFactor, (int)originalContext, status);
             if (!table) return status ? status->code : -7;
         }
-        return launch_prefill(ctx, elementDType, q, k, v, o, batch, seqLen, numHeads, kvHeads, headDim, causal, (int)ropeMode, table, status);
+        return launch_prefill(ctx, elementDType, q, k, v, o, batch, seqLen, numHeads, kvHeads, headDim, causal, (int)ropeMode, table, kRotated.base,
+                              status);
     }
 
     // general path: rotate into scratch with the standalone RoPE kernels, then attend one batch item at a time

@@ -1201,7 +1201,7 @@ size_t decode_scratch_bytes(uint32_t batch, uint32_t numHeads, int workers) {
 // Host launcher shared by both paged entry points and the seqQ == 1 fast path of MultiHeadAttention.
 // pageTable == nullptr selects contiguous K/V ([ctx, kvHeads*128] per sequence, sequences seqStrideKV apart);
 // ctxLens == nullptr gives every sequence uniformCtx tokens.  `fixed` != nullptr supplies the scratch (nothing is
-// allocated); otherwise it comes from the context's grow-only workspace and counter block.
+// allocated); otherwise it comes from the context, or belongs to the graph that the call is captured into (call_scratch).
 int launch_paged_decode(Context* ctx, int dt, int kvDT, const void* q, const void* kPages, const void* vPages, const int32_t* pageTable,
                         const int32_t* ctxLens, int uniformCtx, const float* kScale, const float* vScale, void* out, int* errorFlag,
                         uint32_t batch, uint32_t maxPages, uint32_t pageCount, uint32_t pageSize, uint32_t numHeads, uint32_t kvHeads,
@@ -1241,17 +1241,13 @@ int launch_paged_decode(Context* ctx, int dt, int kvDT, const void* q, const voi
         ws = fixed->base;
         p.counters = fixed->counters;
         clear = fixed->clearCounters;
-    } else if (counterBytes <= ctx->decodeCounterBytes) {
-        ws = (char*)ensure_workspace(ctx, need + 512, status);
-        if (!ws) return status ? status->code : -7;
-        p.counters = ctx->decodeCounters;  // zero since the context was opened; every launch leaves them zero
-        clear = false;
     } else {
-        const size_t cOff = (need + 255) & ~(size_t)255;
-        ws = (char*)ensure_workspace(ctx, cOff + counterBytes + 512, status);
-        if (!ws) return status ? status->code : -7;
-        p.counters = (int*)(ws + cOff);  // the workspace is shared with other ops: not known to be zero
-        clear = true;
+        Scratch own;
+        const int rc = call_scratch(ctx, need, counterBytes, &own, status);
+        if (rc != 0) return rc;
+        ws = own.base;
+        p.counters = own.counters;
+        clear = own.clearCounters;
     }
     p.partAcc = (float*)ws;
     p.partML = (float2*)(ws + accBytes);

@@ -686,17 +686,15 @@ __global__ void __launch_bounds__(256) rope_k_prepass_kernel(const uint16_t* __r
 
 int launch_prefill(Context* ctx, int dt, const void* q, const void* k, const void* v, void* out, uint32_t batch, uint32_t seqLen,
                    uint32_t numHeads, uint32_t kvHeads, uint32_t headDim, uint32_t causal, int ropeMode, const float* ropeTable,
-                   CUDAStatus* status) {
+                   void* kRotated, CUDAStatus* status) {
     if (!prefill_supported(dt, seqLen, seqLen, numHeads, kvHeads, headDim, causal))
         return fail(status, -6, "prefill attention: tensor-core kernel not available for this shape");
     const bool bf16 = dt == DT_BF16;
     const void* kUse = k;
     if (ropeMode != 2) {
         if (!ropeTable) return fail(status, -2, "prefill attention: missing rope table");
-        // rotated K lives in the workspace (the caller sized it)
-        const size_t kBytes = (size_t)batch * seqLen * kvHeads * 128 * 2;
-        if (ctx->workspaceBytes < kBytes) return fail(status, -7, "prefill attention: workspace not prepared");
-        uint16_t* kRot = (uint16_t*)ctx->workspace;
+        // rotated K lives in the caller's scratch, as large as K
+        uint16_t* kRot = (uint16_t*)kRotated;
         const size_t items = (size_t)batch * seqLen * kvHeads * (ropeMode == 1 ? 8 : 16);
         size_t blocks = (items + 255) / 256, cap = (size_t)ctx->smCount * 16;
         if (blocks > cap) blocks = cap;
