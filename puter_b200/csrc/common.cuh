@@ -26,11 +26,12 @@ struct Buffer {
 };
 
 // One cached cos/sin table.  `pinned`: a captured launch reads it, so it is neither overwritten nor freed before the context closes.
+// `finished`: known to be built (until then `built` tells).
 struct RopeTable {
     float* data;
     size_t bytes;
     double key[10];
-    int valid, pinned;
+    int valid, pinned, finished;
     cudaEvent_t built;
     unsigned long long used;
     RopeTable* next;
@@ -70,7 +71,27 @@ struct Context {
     unsigned long long ropeClock;
     // scratch of captured calls: one list entry per graph (see call_scratch)
     struct GraphScratch* graphScratch;
-    cudaEvent_t streamSwitchEvent;  // orders work of a newly adopted stream after what the previous stream still has queued
+    // Change of stream (adopt_stream, settle_stream): whatever the adopted stream launches comes after what the streams before it have queued.
+    cudaEvent_t streamSwitchEvent;  // behind the work of the streams before
+    cudaEvent_t captureEvent;       // (the edges within a capture have an event of their own)
+    int switchWaits;                // the next eager launch has to wait for it
+    int switchLost;                 // eager work in front of a capture that was still open when its stream was left: no event can stand behind it
+    cudaStream_t lostStream;        // that stream
+    int scratchUsed;                // an eager call on `stream` has used the shared scratch or a table since the stream was adopted
+    struct SetAside* setAside;      // scratch that such work may still use
+};
+
+struct SetAside {
+    void* workspace;
+    int* counters;
+    SetAside* next;
+};
+
+// Allocations and waits that are no part of any capture, allowed while one is open.
+struct RelaxedCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
 };
 
 int fail(CUDAStatus* status, int code, const char* fmt, ...);
@@ -83,6 +104,8 @@ int check_launch(Context* ctx, CUDAStatus* status, const char* what);
 void* ensure_workspace(Context* ctx, size_t bytes, CUDAStatus* status);
 // capture state of the context's stream; *id (may be null) names the capture
 bool stream_capturing(Context* ctx, unsigned long long* id);
+// makes the context's stream wait for the streams before it; called by every entry point while one is outstanding
+int settle_stream(Context* ctx, CUDAStatus* status);
 
 // Scratch of one call.  Eager calls share the context's grow-only workspace and its arrival counters: the context's launches are
 // stream-ordered, also across a change of stream.  A captured call gets scratch that belongs to its graph alone, so that a workspace
@@ -129,7 +152,11 @@ inline bool overlap(const void* a, size_t aBytes, const void* b, size_t bBytes) 
     cuda_status_clear(status);                       \
     puter::Context* ctxVar = puter::ctx_of(contextRef, status); \
     if (!ctxVar) return status ? status->code : -1;  \
-    cudaSetDevice(ctxVar->device);
+    cudaSetDevice(ctxVar->device);                   \
+    if (ctxVar->switchWaits | ctxVar->switchLost) {  \
+        int _rc = puter::settle_stream(ctxVar, status); \
+        if (_rc != 0) return _rc;                    \
+    }
 
 #define PUTER_REQUIRE(ref, name, bytes)                                   \
     do {                                                                  \

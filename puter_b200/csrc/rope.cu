@@ -444,17 +444,11 @@ static constexpr int kRopeTables = 4;  // tables that no captured launch reads, 
 
 // Work that is not to be recorded while the context's stream is being captured.
 struct OutsideCapture {
+    RelaxedCapture relaxed;
     Context* ctx;
     cudaStream_t stream;
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    explicit OutsideCapture(Context* c) : ctx(c), stream(c->stream) {
-        cudaThreadExchangeStreamCaptureMode(&mode);
-        ctx->stream = ctx->uploadStream;
-    }
-    ~OutsideCapture() {
-        ctx->stream = stream;
-        cudaThreadExchangeStreamCaptureMode(&mode);
-    }
+    explicit OutsideCapture(Context* c) : ctx(c), stream(c->stream) { ctx->stream = ctx->uploadStream; }
+    ~OutsideCapture() { ctx->stream = stream; }
 };
 
 // exact: the table must have seqLen positions, its sines lying behind them; otherwise a longer one serves too
@@ -463,19 +457,21 @@ static const RopeTable* rope_table(Context* ctx, size_t seqLen, bool exact, int 
     double key[10] = {(double)seqLen, (double)headDim, base, (double)startPos, (double)scaling, scaling ? factor : 0.0,
                       scaling ? low : 0.0, scaling ? high : 0.0, scaling ? (double)origCtx : 0.0, 0.0};
     const bool capturing = stream_capturing(ctx, nullptr);
+    if (!capturing) ctx->scratchUsed = 1;
     RopeTable* oldest = nullptr;
     int unpinned = 0;
     for (RopeTable* t = ctx->ropeTables; t; t = t->next) {
         if (t->valid && memcmp(key + 1, t->key + 1, sizeof(key) - sizeof(key[0])) == 0 && (exact ? t->key[0] == key[0] : t->key[0] >= key[0])) {
             t->used = ++ctx->ropeClock;
-            if (capturing && !t->pinned) {
+            if (capturing && !t->finished) {
                 OutsideCapture now(ctx);
                 if (cudaEventSynchronize(t->built) != cudaSuccess) {
                     fail(status, -7, "rope: waiting for the table failed: %s", cudaGetErrorString(cudaGetLastError()));
                     return nullptr;
                 }
-                t->pinned = 1;
+                t->finished = 1;
             }
+            if (capturing) t->pinned = 1;
             return t;
         }
         if (!t->pinned) {
@@ -501,7 +497,8 @@ static const RopeTable* rope_table(Context* ctx, size_t seqLen, bool exact, int 
         t->next = ctx->ropeTables;
         ctx->ropeTables = t;
     }
-    t->valid = 0;
+    t->valid = t->finished = 0;
+    RelaxedCapture relaxed;  // (another stream may be under capture)
     if (t->bytes < need && t->data) {
         cudaStreamSynchronize(ctx->stream);  // earlier launches may still read the old table
         cudaFree(t->data);
@@ -531,7 +528,7 @@ static const RopeTable* rope_table(Context* ctx, size_t seqLen, bool exact, int 
     if (capturing) {
         OutsideCapture now(ctx);
         if (!fill()) return nullptr;
-        t->pinned = 1;
+        t->pinned = t->finished = 1;
     } else if (!fill()) {
         return nullptr;
     }

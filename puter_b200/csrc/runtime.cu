@@ -53,6 +53,8 @@ int check_launch(Context* ctx, CUDAStatus* status, const char* what) {
 }
 
 void* ensure_workspace(Context* ctx, size_t bytes, CUDAStatus* status) {
+    ctx->scratchUsed = 1;
+    RelaxedCapture relaxed;  // (another stream may be under capture)
     if (bytes <= ctx->workspaceBytes) return ctx->workspace;
     // grow-only; the old block may still be in use by work queued on the stream
     if (ctx->workspace) {
@@ -71,15 +73,79 @@ void* ensure_workspace(Context* ctx, size_t bytes, CUDAStatus* status) {
     return ctx->workspace;
 }
 
-bool stream_capturing(Context* ctx, unsigned long long* id) {
+enum Capture { kNotCaptured, kCaptured, kUntouchable };  // kUntouchable: the legacy stream while a blocking stream is under capture
+
+static Capture capture_of(cudaStream_t stream, unsigned long long* id) {
     cudaStreamCaptureStatus state = cudaStreamCaptureStatusNone;
     unsigned long long name = 0;
-    if (cudaStreamGetCaptureInfo(ctx->stream, &state, &name) != cudaSuccess) {
-        cudaGetLastError();  // the legacy stream while another stream is being captured: this call is not part of that capture
-        return false;
+    if (cudaStreamGetCaptureInfo(stream, &state, &name) != cudaSuccess) {
+        cudaGetLastError();
+        return kUntouchable;
     }
     if (id) *id = name;
-    return state == cudaStreamCaptureStatusActive;
+    return state == cudaStreamCaptureStatusActive ? kCaptured : state == cudaStreamCaptureStatusNone ? kNotCaptured : kUntouchable;
+}
+
+bool stream_capturing(Context* ctx, unsigned long long* id) { return capture_of(ctx->stream, id) == kCaptured; }
+
+// Goes over to another stream.  Two eager streams are ordered by an event, two streams of one capture by an edge of its graph (they share its
+// scratch).  An event may not tie a stream under capture to work outside the capture, and such a stream runs nothing now: the wait stays
+// outstanding until the context launches eagerly again, on whichever stream that is.
+static void adopt_stream(Context* ctx, cudaStream_t next) {
+    cudaSetDevice(ctx->device);
+    cudaStream_t last = ctx->stream;
+    unsigned long long idFrom = 0, idTo = 0;
+    const Capture from = capture_of(last, &idFrom), to = capture_of(next, &idTo);
+    bool covered = false;  // an event stands behind the eager work of `last`
+    if (from == kNotCaptured) {
+        if (ctx->switchWaits) cudaStreamWaitEvent(last, ctx->streamSwitchEvent, 0);  // the event moves on, and what it stood for with it
+        covered = cudaEventRecord(ctx->streamSwitchEvent, last) == cudaSuccess;
+        if (covered) ctx->switchWaits = 1;
+    } else if (from == kCaptured && to == kCaptured && idFrom == idTo) {
+        if (cudaEventRecord(ctx->captureEvent, last) == cudaSuccess) cudaStreamWaitEvent(next, ctx->captureEvent, 0);
+    }
+    if (ctx->scratchUsed && !covered) {
+        ctx->switchLost = 1;
+        ctx->lostStream = last;
+    } else if (covered && ctx->switchLost && ctx->lostStream == last) {
+        ctx->switchLost = 0;
+    }
+    ctx->stream = next;
+    ctx->scratchUsed = 0;
+    if (ctx->switchWaits && to == kNotCaptured && cudaStreamWaitEvent(next, ctx->streamSwitchEvent, 0) == cudaSuccess) ctx->switchWaits = 0;
+    cudaGetLastError();
+}
+
+int settle_stream(Context* ctx, CUDAStatus* status) {
+    if (capture_of(ctx->stream, nullptr) != kNotCaptured) return 0;
+    if (ctx->switchWaits) {
+        cudaError_t err = cudaStreamWaitEvent(ctx->stream, ctx->streamSwitchEvent, 0);
+        if (err != cudaSuccess) return fail(status, -7, "cuda: ordering two streams failed: %s", cudaGetErrorString(cudaGetLastError()));
+        ctx->switchWaits = 0;
+    }
+    if (ctx->lostStream == ctx->stream) ctx->switchLost = 0;  // back on the stream itself
+    if (!ctx->switchLost) return 0;
+    // nothing can wait for that work: it keeps the scratch and the tables, and this stream gets others
+    RelaxedCapture relaxed;
+    int* counters = nullptr;
+    cudaError_t err = cudaMalloc((void**)&counters, ctx->decodeCounterBytes);
+    if (err == cudaSuccess) err = cudaMemsetAsync(counters, 0, ctx->decodeCounterBytes, ctx->uploadStream);
+    if (err == cudaSuccess) err = cudaStreamSynchronize(ctx->uploadStream);
+    if (err != cudaSuccess) {
+        cudaGetLastError();
+        if (counters) cudaFree(counters);
+        return fail(status, -7, "cuda: scratch for another stream failed: %s", cudaGetErrorString(err));
+    }
+    ctx->setAside = new SetAside{ctx->workspace, ctx->decodeCounters, ctx->setAside};
+    ctx->workspace = nullptr;
+    ctx->workspaceBytes = 0;
+    ctx->decodeCounters = counters;
+    for (RopeTable* t = ctx->ropeTables; t; t = t->next) {
+        if (t->valid && !t->finished) cudaStreamWaitEvent(ctx->stream, t->built, 0);
+        t->pinned = 1;
+    }
+    ctx->switchLost = 0;
+    return 0;
 }
 
 int call_scratch(Context* ctx, size_t bytes, size_t counterBytes, Scratch* out, CUDAStatus* status) {
@@ -98,15 +164,13 @@ int call_scratch(Context* ctx, size_t bytes, size_t counterBytes, Scratch* out, 
     GraphScratch* g = ctx->graphScratch;
     while (g && (g->id != id || g->bytes < need)) g = g->next;
     if (!g) {
-        // allocating is not part of the captured work: done in relaxed mode, cleared on a stream of the context's own
-        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-        cudaThreadExchangeStreamCaptureMode(&mode);
+        // allocating is not part of the captured work, and neither is clearing, on a stream of the context's own
+        RelaxedCapture relaxed;
         void* p = nullptr;
         const size_t total = ctx->decodeCounterBytes + need;
         cudaError_t err = cudaMalloc(&p, total);
         if (err == cudaSuccess) err = cudaMemsetAsync(p, 0, ctx->decodeCounterBytes, ctx->uploadStream);
         if (err == cudaSuccess) err = cudaStreamSynchronize(ctx->uploadStream);
-        cudaThreadExchangeStreamCaptureMode(&mode);
         if (err != cudaSuccess) {
             cudaGetLastError();
             if (p) cudaFree(p);
@@ -171,6 +235,7 @@ int cuda_open_device_index(int ordinal, CUDADeviceRef* outDevice, CUDAStatus* st
     ctx->stream = ctx->ownStream;
     for (int i = 0; i < 4; i++) cudaEventCreateWithFlags(&ctx->stageEvents[i], cudaEventDisableTiming);
     cudaEventCreateWithFlags(&ctx->streamSwitchEvent, cudaEventDisableTiming);
+    cudaEventCreateWithFlags(&ctx->captureEvent, cudaEventDisableTiming);
     if (cudaMalloc((void**)&ctx->errorFlag, 256) != cudaSuccess) {
         delete ctx;
         return fail(status, -7, "cuda: context allocation failed");
@@ -215,9 +280,17 @@ void cuda_close_device(CUDADeviceRef device) {
         delete g;
         g = next;
     }
+    for (SetAside* a = ctx->setAside; a;) {
+        SetAside* next = a->next;
+        cudaFree(a->workspace);
+        cudaFree(a->counters);
+        delete a;
+        a = next;
+    }
     for (int i = 0; i < 4; i++)
         if (ctx->stageEvents[i]) cudaEventDestroy(ctx->stageEvents[i]);
     if (ctx->streamSwitchEvent) cudaEventDestroy(ctx->streamSwitchEvent);
+    if (ctx->captureEvent) cudaEventDestroy(ctx->captureEvent);
     cudaStreamDestroy(ctx->ownStream);
     cudaStreamDestroy(ctx->uploadStream);
     {
@@ -354,21 +427,7 @@ int cuda_context_set_stream(CUDADeviceRef device, void* cudaStream, CUDAStatus* 
     Context* ctx = ctx_of(device, status);
     if (!ctx) return -1;
     cudaStream_t next = (cudaStream_t)cudaStream;  // NULL = the legacy default stream
-    if (next != ctx->stream) {
-        // the context's scratch (workspace, RoPE table, decode counters) may still be read by kernels queued on the old stream:
-        // whatever the new stream launches is ordered after them
-        cudaSetDevice(ctx->device);
-        // (a stream under capture runs nothing now, and an event may not tie it to work outside its capture: two streams of one capture
-        // are ordered in the graph, since they share its scratch)
-        unsigned long long idFrom = 0, idTo = 0;
-        const bool from = stream_capturing(ctx, &idFrom);
-        cudaStream_t last = ctx->stream;
-        ctx->stream = next;
-        const bool to = stream_capturing(ctx, &idTo);
-        if (from == to && (!from || idFrom == idTo) && cudaEventRecord(ctx->streamSwitchEvent, last) == cudaSuccess)
-            cudaStreamWaitEvent(next, ctx->streamSwitchEvent, 0);
-        cudaGetLastError();
-    }
+    if (next != ctx->stream) adopt_stream(ctx, next);
     return ok(status);
 }
 
@@ -376,12 +435,7 @@ int cuda_context_reset_stream(CUDADeviceRef device, CUDAStatus* status) {
     cuda_status_clear(status);
     Context* ctx = ctx_of(device, status);
     if (!ctx) return -1;
-    if (ctx->stream != ctx->ownStream) {
-        cudaSetDevice(ctx->device);
-        if (cudaEventRecord(ctx->streamSwitchEvent, ctx->stream) == cudaSuccess) cudaStreamWaitEvent(ctx->ownStream, ctx->streamSwitchEvent, 0);
-        cudaGetLastError();
-        ctx->stream = ctx->ownStream;
-    }
+    if (ctx->stream != ctx->ownStream) adopt_stream(ctx, ctx->ownStream);
     return ok(status);
 }
 
@@ -399,6 +453,10 @@ int cuda_context_take_error(CUDADeviceRef device, int* outFlag, CUDAStatus* stat
     if (!ctx) return -1;
     if (!outFlag) return fail(status, -2, "cuda: nil outFlag");
     cudaSetDevice(ctx->device);
+    if (ctx->switchWaits | ctx->switchLost) {  // calls on the streams before may still raise it
+        int rc = settle_stream(ctx, status);
+        if (rc != 0) return rc;
+    }
     int flag = 0;
     cudaError_t err = cudaMemcpyAsync(&flag, ctx->errorFlag, sizeof(int), cudaMemcpyDeviceToHost, ctx->stream);
     if (err == cudaSuccess) err = cudaMemsetAsync(ctx->errorFlag, 0, sizeof(int), ctx->stream);

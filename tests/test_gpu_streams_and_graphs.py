@@ -96,3 +96,168 @@ def test_graphs_of_the_16_bit_steps_keep_their_scratch(d, kind):
         out.fill_(7)
         torch.cuda.synchronize()
     assert d.take_error() == 0
+
+
+def busy(ms):
+    torch.cuda._sleep(int(ms * 1.8e6))
+
+
+def raw_capture(graph, stream, fn):
+    """What torch.cuda.graph does, without its synchronisation of the device."""
+    with torch.cuda.stream(stream):
+        graph.capture_begin(capture_error_mode="thread_local")
+        try:
+            fn()
+        finally:
+            graph.capture_end()
+
+
+def warm(d, run, outs):
+    """Scratch of its final size and the tables: growing frees memory, which waits for the device."""
+    for i in range(len(outs)):
+        run(d, i)
+    torch.cuda.synchronize()
+    for o in outs:
+        o.fill_(7)
+    torch.cuda.synchronize()
+
+
+ROPE = dict(Mode=1, BaseFreq=500000.0)
+
+
+def prompts(number, d=None):
+    """Inputs, outputs and what each call gives alone: different sizes, so that scratch grows and tables differ."""
+    import puter_b200
+
+    rope = puter_b200.RoPEConfig(**ROPE)
+    ts = [make_prompt(2, [300 + 200 * i, 150], 8, 2, 128, i) for i in range(number)]
+    outs = [torch.full_like(t[0], 7.0) for t in ts]
+    wants = [prompt(puter_b200.Device(), *t, 8, 2, 128, 2, rope=rope) for t in ts]
+    run = lambda dev, i: prompt(dev, *ts[i], 8, 2, 128, 2, rope=rope, out=outs[i])  # noqa: E731
+    torch.cuda.synchronize()
+    return run, outs, wants
+
+
+@pytest.mark.parametrize("after", ["the captured stream", "a third stream", "the default stream", "by way of a capture more"])
+def test_eager_calls_after_a_capture_follow_those_before_it(d, after):
+    """Eager on A, a capture on B that waits for nothing, eager again: the last call uses the scratch of the first, so it comes behind it."""
+    run, outs, wants = prompts(4)
+    a, b, c = (torch.cuda.Stream() for _ in range(3))
+    graph, other = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    done = [torch.cuda.Event() for _ in range(2)]
+    with torch.cuda.stream(a):
+        warm(d, run, outs)
+        busy(60)
+        run(d, 0)
+        done[0].record()
+    raw_capture(graph, b, lambda: run(d, 1))
+    if after == "by way of a capture more":
+        raw_capture(other, c, lambda: run(d, 3))
+    last = {"the captured stream": b, "a third stream": c, "the default stream": torch.cuda.default_stream(), "by way of a capture more": b}[after]
+    with torch.cuda.stream(last):
+        run(d, 2)
+        done[1].record()
+    assert not done[0].query()  # (the first stream is still busy)
+    done[1].synchronize()
+    assert done[0].query()
+    graph.replay()
+    if after == "by way of a capture more":
+        other.replay()
+    else:
+        run(d, 3)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, wants)) and d.take_error() == 0
+
+
+def test_the_error_flag_of_calls_before_a_capture_is_seen(d):
+    """take_error waits for the calls on the streams before, too."""
+    run, outs, wants = prompts(2)
+    t = make4(2, [40], 2, 64, 16, 2, 1)
+    t[5][0, 0] = t[1].shape[0]
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    graph, out = torch.cuda.CUDAGraph(), torch.full_like(t[0], 7.0)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(a):
+        busy(30)
+        decode4(d, t, 2, 64, 16, 2, 2, out=out)
+    raw_capture(graph, b, lambda: run(d, 1))
+    with torch.cuda.stream(b):
+        assert d.take_error() == 1
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[1], wants[1])
+
+
+@pytest.mark.parametrize("way", ["plain", "through a fork of the capture"])
+def test_eager_calls_beside_a_capture_whose_stream_has_work_queued(d, way):
+    """Work queued on B in front of its capture cannot be waited for while the capture is open: a call on C gets scratch of its own."""
+    run, outs, wants = prompts(5)
+    steps = make4(2, [3000, 17, 900], 8, 128, 16, 4, 1)
+    step = [torch.full_like(steps[0], 7.0) for _ in range(2)]
+    b, c, side = (torch.cuda.Stream() for _ in range(3))
+    want = decode4(d, steps, 8, 128, 16, 4, 2)
+    graph = torch.cuda.CUDAGraph()
+    fork, join = torch.cuda.Event(), torch.cuda.Event()
+    with torch.cuda.stream(b):
+        warm(d, run, outs)
+        busy(60)
+        run(d, 0)
+        decode4(d, steps, 8, 128, 16, 4, 2, out=step[0])
+        graph.capture_begin(capture_error_mode="relaxed")
+        run(d, 1)
+        if way != "plain":
+            fork.record()
+            with torch.cuda.stream(side):
+                side.wait_event(fork)
+                run(d, 4)
+                join.record()
+        with torch.cuda.stream(c):
+            for _ in range(3):
+                run(d, 2)
+                decode4(d, steps, 8, 128, 16, 4, 2, out=step[1])
+        if way != "plain":
+            b.wait_event(join)
+        run(d, 3)
+        graph.capture_end()
+    graph.replay()
+    torch.cuda.synchronize()
+    if way == "plain":
+        run(d, 4)
+        torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, wants))
+    assert torch.equal(step[0], want) and torch.equal(step[1], want) and d.take_error() == 0
+
+
+def test_back_to_the_own_stream_in_the_middle_of_a_capture():
+    """cuda_context_reset_stream neither joins its stream to the capture nor forgets the stream before."""
+    import ctypes
+
+    import puter_b200
+
+    d = puter_b200.Device(follow_torch_stream=False)
+    run, outs, wants = prompts(3)
+    adopt = lambda s: d._check(d.lib.cuda_context_set_stream(d.ref, ctypes.c_void_p(s.cuda_stream), ctypes.byref(d._status)))  # noqa: E731
+    back = lambda: d._check(d.lib.cuda_context_reset_stream(d.ref, ctypes.byref(d._status)))  # noqa: E731
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    done = torch.cuda.Event()
+    graph = torch.cuda.CUDAGraph()
+    adopt(a)
+    warm(d, run, outs)
+    with torch.cuda.stream(a):
+        busy(60)
+    run(d, 0)
+    done.record(a)
+
+    def middle():
+        adopt(b)
+        run(d, 1)
+        back()
+        run(d, 2)
+
+    raw_capture(graph, b, middle)
+    assert not done.query()
+    assert d.take_error() == 0  # (synchronises the own stream, which waits for a)
+    assert done.query()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, wants))
