@@ -137,7 +137,8 @@ int cuda_context_set_stream(CUDADeviceRef device, void* cudaStream, CUDAStatus* 
 /* NEW: go back to the context's own non-blocking stream */
 int cuda_context_reset_stream(CUDADeviceRef device, CUDAStatus* status);
 /* NEW: 1 = always use the kernels that reproduce device/cpu operation order exactly
-   (sequential sums); 0 (default) = use the tensor-core / split-KV kernels where they apply */
+   (sequential sums) in multi-head attention, prefill and packed prefill (paged decode has one form, with either cache);
+   0 (default) = use the tensor-core / split-KV kernels where they apply */
 int cuda_context_set_exact(CUDADeviceRef device, int exact, CUDAStatus* status);
 /* NEW: synchronises the context's stream, returns the device-side error flag in *outFlag and clears it:
    1 = some call since the last read met an out-of-range page id / offset or an over-long context and skipped it;
@@ -412,7 +413,8 @@ int cuda_dispatch_paged_decode_attention_q4(CUDADeviceRef contextRef, int elemen
 /* NEW: attention over whole prompts of different lengths, packed one behind the other: q/out [totalTokens, numHeads*headDim], k/v
    [totalTokens, kvHeads*headDim]; sequence i holds rows seqStarts[i] .. seqStarts[i+1]-1 (device int32 [batch + 1], non-decreasing).
    Per sequence as cuda_dispatch_rope_attention_prefill: positions startPosition .. restart with every sequence, causal or not,
-   ropeMode 2 = inputs already rotated.  float32, f16, bf16; headDim <= 256.  Rows of no sequence are left as they were.  A pair of starts
+   ropeMode 2 = inputs already rotated.  float32, f16, bf16; headDim <= 256; with cuda_context_set_exact(1) the operations of the CPU in its
+   order, for sequences that its kernel holds a row of scores of (about 57000 keys).  Rows of no sequence are left as they were.  A pair of starts
    that is no range of the packed rows, or is longer than maxSeqLen, is skipped and raises the error flag (1); where the starts are
    not non-decreasing the other rows of the call are not valid either.  out may not overlap an input. */
 int cuda_dispatch_rope_packed_attention_prefill(CUDADeviceRef contextRef, int elementDType, CUDABufferRef queryRef, CUDABufferRef keyRef,

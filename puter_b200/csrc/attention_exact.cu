@@ -15,6 +15,7 @@
 // do not cover; they favour exactness over speed: one block per (query row, head), the scores of the row live
 // in shared memory, sums over keys are sequential per thread.
 #include "common.cuh"
+#include "packed.cuh"
 
 namespace puter {
 
@@ -50,21 +51,29 @@ __device__ __forceinline__ float block_max(float v, float* red) {
     return t;
 }
 
-template <int DT>
+// PACKED: row blockIdx.x of packed sequences attends to the keys of its own; otherwise query blockIdx.x of seqQ to seqK keys.
+template <int DT, bool PACKED>
 __global__ void __launch_bounds__(256) mha_exact_kernel(const void* __restrict__ q, const void* __restrict__ k, const void* __restrict__ v,
                                                        void* __restrict__ out, int seqQ, int seqK, int numHeads, int kvHeads, int headDim,
-                                                       int causal, int window, float scale) {
+                                                       int causal, int window, float scale, pk::Seqs seqs) {
     extern __shared__ float smem[];
-    float* scores = smem;               // [seqK]
-    float* qs = smem + seqK;            // [headDim]
     __shared__ float red[32];
     __shared__ float sumShared;
     __shared__ int infCount;
-    const int qi = blockIdx.x, head = blockIdx.y;
+    int qi = blockIdx.x, first = 0;
+    if (PACKED) {
+        int end;
+        if (!pk::seq_rows(seqs, pk::seq_of(seqs, qi), first, end) || qi < first || qi >= end) return;
+        seqQ = seqK = end - first;
+        qi -= first;
+    }
+    const int head = blockIdx.y;
+    float* scores = smem;               // [seqK]
+    float* qs = smem + seqK;            // [headDim]
     const int kvHead = head / (numHeads / kvHeads);
     const size_t qStride = (size_t)numHeads * headDim, kvStride = (size_t)kvHeads * headDim;
-    const size_t qOff = (size_t)qi * qStride + (size_t)head * headDim;
-    const size_t kvOff = (size_t)kvHead * headDim;
+    const size_t qOff = (size_t)(first + qi) * qStride + (size_t)head * headDim;
+    const size_t kvOff = (size_t)first * kvStride + (size_t)kvHead * headDim;
     for (int d = threadIdx.x; d < headDim; d += blockDim.x) qs[d] = load_el<DT>(q, qOff + d);
     if (threadIdx.x == 0) infCount = 0;
     __syncthreads();
@@ -161,9 +170,9 @@ int launch_mha_exact(Context* ctx, int dt, const void* q, const void* k, const v
     dim3 grid(seqQ, numHeads);
 #define MHA_LAUNCH(DT)                                                                                                   \
     do {                                                                                                                 \
-        cudaFuncSetAttribute(mha_exact_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxDynSmem);       \
-        mha_exact_kernel<DT><<<grid, 256, smem, ctx->stream>>>(q, k, v, out, (int)seqQ, (int)seqK, (int)numHeads, (int)kvHeads, \
-                                                               (int)headDim, (int)causal, (int)window, scale);           \
+        cudaFuncSetAttribute(mha_exact_kernel<DT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxDynSmem); \
+        mha_exact_kernel<DT, false><<<grid, 256, smem, ctx->stream>>>(q, k, v, out, (int)seqQ, (int)seqK, (int)numHeads, (int)kvHeads, \
+                                                                      (int)headDim, (int)causal, (int)window, scale, pk::Seqs{}); \
     } while (0)
     if (dt == DT_F32) MHA_LAUNCH(DT_F32);
     else if (dt == DT_BF16) MHA_LAUNCH(DT_BF16);
@@ -171,6 +180,33 @@ int launch_mha_exact(Context* ctx, int dt, const void* q, const void* k, const v
     else return fail(status, -6, "attention: MultiHeadAttention unsupported dtype");
 #undef MHA_LAUNCH
     return check_launch(ctx, status, "multi-head attention (exact)");
+}
+
+int check_mha_exact_packed(CUDAStatus* status, int maxLen, uint32_t numHeads, uint32_t headDim) {
+    if (((size_t)maxLen + headDim) * sizeof(float) > kMaxDynSmem)
+        return fail(status, -6, "attention: exact kernel holds one score row in shared memory; maxSeqLen=%d exceeds its limit of %zu keys", maxLen,
+                    kMaxDynSmem / 4 - headDim);
+    if (numHeads > 65535) return fail(status, -6, "attention: exact kernel takes up to 65535 heads, got %u", numHeads);
+    return 0;
+}
+
+// The same over packed sequences, q / out [total, numHeads, headDim], k / v [total, kvHeads, headDim]; check_mha_exact_packed has passed.
+int launch_mha_exact_packed(Context* ctx, int dt, const void* q, const void* k, const void* v, void* out, const pk::Seqs& seqs, uint32_t numHeads,
+                            uint32_t kvHeads, uint32_t headDim, uint32_t causal, CUDAStatus* status) {
+    const size_t smem = ((size_t)seqs.maxLen + headDim) * sizeof(float);
+    const float scale = (float)(1.0 / sqrt((double)headDim));
+    const dim3 grid((unsigned)seqs.total, numHeads);
+#define MHA_PACKED(DT)                                                                                                              \
+    do {                                                                                                                            \
+        cudaFuncSetAttribute(mha_exact_kernel<DT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxDynSmem);            \
+        mha_exact_kernel<DT, true><<<grid, 256, smem, ctx->stream>>>(q, k, v, out, 0, 0, (int)numHeads, (int)kvHeads, (int)headDim, \
+                                                                     (int)causal, 0, scale, seqs);                                 \
+    } while (0)
+    if (dt == DT_F32) MHA_PACKED(DT_F32);
+    else if (dt == DT_BF16) MHA_PACKED(DT_BF16);
+    else MHA_PACKED(DT_F16);
+#undef MHA_PACKED
+    return check_launch(ctx, status, "packed prefill attention (exact)");
 }
 
 }  // namespace puter

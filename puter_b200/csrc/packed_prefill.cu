@@ -7,7 +7,9 @@
 // Rows that belong to no sequence (before the first start, behind the last) are neither read into a result nor written.
 // A pair of starts that is not 0 <= start <= end <= totalTokens with at most maxSeqLen rows is skipped and raises the error flag.
 //
-// Three kernels.  rows_kernel is a warp per (row, head) for any type and head dimension.  short_kernel is for calls without long sequences: a
+// cuda_context_set_exact(1) rotates into scratch and attends with the kernel that keeps the CPU's order of operations (attention_exact.cu).
+//
+// Three kernels otherwise.  rows_kernel is a warp per (row, head) for any type and head dimension.  short_kernel is for calls without long sequences: a
 // block per (sequence, KV head), see there.  tiles_kernel is the tensor-core form (bf16 / f16,
 // head dimensions up to 128 that are multiples of 8), built like the prefill kernel for equal lengths: two tiles of 128 rows that take turns
 // on the tensor core, softmax in registers with one row a thread, P handed back through TMEM, K and V through a TMA ring.  What the
@@ -27,6 +29,7 @@
 #include <math.h>
 
 #include "common.cuh"
+#include "packed.cuh"
 #include "tcgen05.cuh"
 
 namespace puter {
@@ -36,36 +39,11 @@ int validate_rope(CUDAStatus* status, double base, uint32_t halfMode, uint32_t s
 const float* cached_rope_table_at_least(Context* ctx, size_t positions, int headDim, double base, long long startPos, int scaling,
                                         double factor, double low, double high, int origCtx, const float** sinT, CUDAStatus* status);
 
+int check_mha_exact_packed(CUDAStatus* status, int maxLen, uint32_t numHeads, uint32_t headDim);
+int launch_mha_exact_packed(Context* ctx, int dt, const void* q, const void* k, const void* v, void* out, const pk::Seqs& seqs, uint32_t numHeads,
+                            uint32_t kvHeads, uint32_t headDim, uint32_t causal, CUDAStatus* status);
+
 namespace pk {
-
-struct Seqs {
-    const int32_t* starts;
-    int batch, total, maxLen;
-    int* errorFlag;
-};
-
-// rows [s0, s1) of sequence b; false (and the flag) where the starts make none
-__device__ __forceinline__ bool seq_rows(const Seqs& s, int b, int& s0, int& s1) {
-    s0 = s.starts[b];
-    s1 = s.starts[b + 1];
-    if (s0 < 0 || s1 < s0 || s1 > s.total || s1 - s0 > s.maxLen) {
-        atomicExch(s.errorFlag, 1);
-        s1 = s0;
-        return false;
-    }
-    return s1 > s0;
-}
-
-// the sequence that holds `row`: the last one that starts at or before it
-__device__ __forceinline__ int seq_of(const Seqs& s, int row) {
-    int a = 0, z = s.batch;
-    while (z - a > 1) {
-        const int m = (a + z) >> 1;
-        if (s.starts[m] <= row) a = m;
-        else z = m;
-    }
-    return a;
-}
 
 // x [total, heads, D] rotated at the positions of its rows within their sequences, any even D
 template <int DT>
@@ -1339,6 +1317,10 @@ extern "C" int cuda_dispatch_rope_packed_attention_prefill(CUDADeviceRef context
         return fail(status, -2, "%s: out may not overlap an input", what);
     if ((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & (es - 1)) != 0 || ((uintptr_t)dev_ptr(seqStartsRef) & 3u) != 0)
         return fail(status, -2, "%s: a buffer is not aligned to its elements", what);
+    if (ctx->exact) {
+        int rc = check_mha_exact_packed(status, (int)maxSeqLen, numHeads, headDim);
+        if (rc != 0) return rc;
+    }
     const pk::Seqs seqs{(const int32_t*)dev_ptr(seqStartsRef), (int)batch, (int)totalTokens, (int)maxSeqLen, ctx->errorFlag};
     const float *table = nullptr, *sinT = nullptr;
     if (ropeMode != 2) {
@@ -1347,8 +1329,8 @@ extern "C" int cuda_dispatch_rope_packed_attention_prefill(CUDADeviceRef context
         if (!table) return status ? status->code : -7;
     }
     const pk::Call c{elementDType, q, k, v, out, seqs, numHeads, kvHeads, headDim, causal ? 1u : 0u, ropeMode, table, sinT};
-    if (pk::short_takes(c)) return elementDType == DT_BF16 ? pk::short_launch<true>(ctx, c, status) : pk::short_launch<false>(ctx, c, status);
-    if (pk::tiles_take(c)) return elementDType == DT_BF16 ? pk::tiles_launch<true>(ctx, c, status) : pk::tiles_launch<false>(ctx, c, status);
+    if (!ctx->exact && pk::short_takes(c)) return elementDType == DT_BF16 ? pk::short_launch<true>(ctx, c, status) : pk::short_launch<false>(ctx, c, status);
+    if (!ctx->exact && pk::tiles_take(c)) return elementDType == DT_BF16 ? pk::tiles_launch<true>(ctx, c, status) : pk::tiles_launch<false>(ctx, c, status);
     const int cap = ctx->smCount * 8;
     if (ropeMode != 2) {
         const size_t qAt = 0, kAt = (qBytes + 255) & ~(size_t)255;
@@ -1374,6 +1356,7 @@ extern "C" int cuda_dispatch_rope_packed_attention_prefill(CUDADeviceRef context
         q = ws.base + qAt;
         k = ws.base + kAt;
     }
+    if (ctx->exact) return launch_mha_exact_packed(ctx, elementDType, q, k, v, out, seqs, numHeads, kvHeads, headDim, causal ? 1u : 0u, status);
     const size_t blocks = ((size_t)totalTokens * numHeads + 7) / 8;
     const int grid = blocks < (size_t)cap ? (int)blocks : cap;
     const float scaleLog2 = (float)(1.4426950408889634 / sqrt((double)headDim));
