@@ -87,6 +87,7 @@ class SharedBuffer:
 
 
 _NO_TOKEN = ctypes.c_uint64(0)  # completionToken
+_PLAIN = frozenset({int, ctypes.c_double, ctypes.c_int64})  # what passes as it is where no argument types are declared
 
 
 class Device:
@@ -155,10 +156,9 @@ class Device:
             for old in self._refs.values():
                 self.lib.cuda_buffer_release(old)
             self._refs.clear()
-        # a handle that is there was made of CUDA memory; whether this view of it is contiguous is asked every time
         known = self._refs
         try:
-            return [None if t is None else known[t.data_ptr(), t.nbytes] if t.is_contiguous() else self._ref(t) for t in tensors]
+            return [None if t is None else known[t.data_ptr(), t.nbytes] if t.is_cuda and t.is_contiguous() else self._ref(t) for t in tensors]
         except KeyError:  # a handle to be made
             return [self._ref(t) for t in tensors]
 
@@ -169,9 +169,11 @@ class Device:
         self._check(rc)
 
     def _call_plain(self, name, format, tensors, rest):
-        """_call of an entry point (context, format, buffers, rest, token, status): `rest` in the declared types, integers of 32 bits as they are."""
+        """_call of an entry point (context, format, buffers, rest, token, status): `rest` in the declared types, integers of 32 bits as they are.
+        Anything else (numpy's integers, what has to be refused) is converted by declaration."""
         self._enter()
-        fn = getattr(self.lib.__dict__.get("plain", self.lib), name)
+        plain = type(format) is int and _PLAIN.issuperset(map(type, rest))
+        fn = getattr(self.lib.__dict__.get("plain", self.lib) if plain else self.lib, name)
         rc = fn(self.ref, format, *self._handles(tensors), *rest, _NO_TOKEN, ctypes.byref(self._status))
         if rc != 0:
             self._check(rc)
