@@ -477,12 +477,17 @@ static const RopeTable* rope_table(Context* ctx, size_t seqLen, bool exact, int 
                                    double factor, double low, double high, int origCtx, CUDAStatus* status) {
     double key[10] = {(double)seqLen, (double)headDim, base, (double)startPos, (double)scaling, scaling ? factor : 0.0,
                       scaling ? low : 0.0, scaling ? high : 0.0, scaling ? (double)origCtx : 0.0, 0.0};
+    // rounded up so that calls of all lengths share a few tables: to a power of two up to 4096 positions, to a multiple of 4096 up to 65536, then by
+    // an eighth at most
     size_t made = seqLen;
-    if (!exact) {  // to the next power of two, so that calls of all lengths share a few
-        made = 64;
-        while (made < seqLen) made *= 2;
+    if (!exact) {
+        size_t step = 64;
+        while (step < seqLen && step < 4096) step *= 2;
+        while (step * 16 <= seqLen) step *= 2;
+        made = (seqLen + step - 1) / step * step;
     }
-    const size_t need = made * (size_t)(headDim / 2) * 2 * sizeof(float);
+    const size_t perPosition = (size_t)(headDim / 2) * 2 * sizeof(float);
+    size_t need = made * perPosition;
     const bool capturing = stream_capturing(ctx, nullptr);
     if (!capturing) ctx->scratchUsed = 1;
     RopeTable *oldest = nullptr, *unread = nullptr;  // the table used longest ago, and a large enough one that launches of graphs alone have read
@@ -507,8 +512,6 @@ static const RopeTable* rope_table(Context* ctx, size_t seqLen, bool exact, int 
             if (!t->eager && t->bytes >= need) unread = t;
         }
     }
-    seqLen = made;
-    key[0] = (double)made;
     RelaxedCapture relaxed;  // (another stream may be under capture)
     if (!capturing && loose > kRopeTables) {  // graphs that are gone have left more
         cudaStreamSynchronize(ctx->stream);
@@ -546,7 +549,14 @@ static const RopeTable* rope_table(Context* ctx, size_t seqLen, bool exact, int 
     }
     auto fill = [&]() {
         if (!t->data) {
-            if (cudaMalloc((void**)&t->data, need) != cudaSuccess) {
+            cudaError_t err = cudaMalloc((void**)&t->data, need);
+            if (err != cudaSuccess && made > seqLen) {  // what the call needs may still fit
+                cudaGetLastError();
+                made = seqLen;
+                need = made * perPosition;
+                err = cudaMalloc((void**)&t->data, need);
+            }
+            if (err != cudaSuccess) {
                 cudaGetLastError();
                 t->data = nullptr;
                 fail(status, -7, "rope: table allocation of %zu bytes failed", need);
@@ -554,7 +564,8 @@ static const RopeTable* rope_table(Context* ctx, size_t seqLen, bool exact, int 
             }
             t->bytes = need;
         }
-        if (build_rope_table(ctx, t->data, seqLen, headDim, base, startPos, scaling, factor, low, high, origCtx, status) != 0) return false;
+        if (build_rope_table(ctx, t->data, made, headDim, base, startPos, scaling, factor, low, high, origCtx, status) != 0) return false;
+        key[0] = (double)made;
         cudaError_t err = cudaEventRecord(t->built, ctx->stream);
         if (err == cudaSuccess && capturing) err = cudaEventSynchronize(t->built);
         if (err != cudaSuccess) {

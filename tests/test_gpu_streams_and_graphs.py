@@ -336,3 +336,22 @@ def test_scratch_of_a_graph_that_still_runs_is_not_handed_on(d):
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs) and d.take_error() == 0
     print("still running:", taken >> 20, "MB more")
+
+
+@pytest.mark.parametrize("positions", [(1 << 20) + 1, 1 << 20, 1500001])
+def test_tables_are_little_larger_than_asked_for(d, positions):
+    """maxPositions is a bound that a program may set generously: 512 bytes a position with 128 dimensions, an eighth more at most."""
+    import puter_b200
+
+    x = torch.randn(3, 256, device="cuda").bfloat16()
+    codes, params = torch.zeros(1, 2, 16, 64, dtype=torch.uint8, device="cuda"), torch.zeros(1, 2, 16, 2, dtype=torch.bfloat16, device="cuda")
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+    pos, ids, off = i32([0, 5, positions - 1]), i32([0, 0, 0]), i32([0, 1, 2])
+    free = free_memory()
+    d.RoPEKVPageWriteQ4(puter_b200.RoPEConfig(Mode=1), x, x, pos, ids, off, codes, params, codes.clone(), params.clone(), 3, 2, 128, 1, 16, positions, 2)
+    torch.cuda.synchronize()
+    assert 0 <= free - torch.cuda.mem_get_info()[0] <= positions * 512 * 9 // 8 + (16 << 20)
+    assert d.take_error() == 0
+    pos[2] = positions
+    d.RoPEKVPageWriteQ4(puter_b200.RoPEConfig(Mode=1), x, x, pos, ids, off, codes, params, codes.clone(), params.clone(), 3, 2, 128, 1, 16, positions, 2)
+    assert d.take_error() == 1
