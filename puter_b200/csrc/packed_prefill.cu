@@ -1161,18 +1161,22 @@ static int pack_log(uint32_t group) {
     return log;
 }
 
-// Measured on both sides (us, short against tiles).  64 dimensions, up to 160 tokens: short wins throughout (64 sequences of 160, 4 heads per KV
-// head 33 : 42; 300 of 64, 12 KV heads 50 : 130; 64 of 160, 16 heads on one KV head 38 : 37).  128 dimensions, by rows (tokens x heads of a group) per sequence
-// and KV head: 160 7.9 : 15.2 and 23 : 42, 192 28 : 43, 36 : 46 and 20 : 23, 256 54 : 43 and 163 : 134, 384 59 : 56, so up to 192; more where a
-// group that is no power of two fills the tiles to a third at most (7 heads, 252 rows 18 : 77), or where few blocks let the shorter latency
-// decide: one sequence of 128 tokens (8 x 512 rows) 12.4 : 13.2, of 160 13.8 : 13.6.
+// Measured on both sides (us, short against tiles), calls of up to 160 tokens per sequence.
+// 64 dimensions: short wins (64 sequences of 160, 4 heads per KV head 33 : 42, 28 heads on 4 46 : 77; 300 of 64, 12 KV heads 50 : 130, 8 heads per KV
+// head 35 : 53; 64 of 128, 16 heads per KV head 23 : 26, of 160 33 : 30) except where the group fills the tiles to four fifths, the keys most of a key
+// tile, and there are more than 2^18 rows in all: 300 of 96 with 8 heads per KV head 67 : 69, 32 134 : 120; 300 of 112 with 8 83 : 83, 16 87 : 78; 300 of
+// 128 with 8 98 : 85, 12 80 : 69, 32 203 : 158; 300 of 160 with 12 112 : 95, 16 147 : 107; 64 of 128 with 32 40 : 39, of 160 63 : 50.
+// 128 dimensions, by rows (tokens x heads of a group) per sequence and KV head: 160 7.9 : 15.2 and 23 : 42, 192 28 : 43, 36 : 46 and 20 : 23, 256 54 : 43 and
+// 163 : 134, 384 59 : 56, so up to 192; more where a group that is no power of two fills the tiles to a third at most (7 heads, 252 rows 18 : 77), or
+// where few blocks let the shorter latency decide: one sequence of 128 tokens (8 x 512 rows) 12.4 : 13.2, of 160 13.8 : 13.6.
 static bool short_takes(const Call& c) {
     if (!tiles_take(c) || c.seqs.maxLen > kShortMax || c.kvHeads > 65535 || (c.ropeMode != 2 && c.dim != 64 && c.dim != 128)) return false;
     const size_t rows = (size_t)c.seqs.maxLen * (c.heads / c.kvHeads), pairs = (size_t)c.seqs.batch * c.kvHeads;
     if (rows > 1u << 30) return false;  // a block counts its rows in 31 bits
     const int pack = pack_log(c.heads / c.kvHeads), span = 2 * (kRows >> pack);
     const size_t tileRows = ((size_t)c.seqs.maxLen + span - 1) / span * (c.heads / c.kvHeads >> pack) * 2 * kRows;
-    return c.dim <= 64 || rows <= 192 || 3 * rows <= tileRows || pairs * rows <= 4096;
+    if (c.dim <= 64) return c.seqs.maxLen < 96 || 5 * rows <= 4 * tileRows || pairs * rows <= 1u << 18;
+    return rows <= 192 || 3 * rows <= tileRows || pairs * rows <= 4096;
 }
 
 template <bool BF16>
