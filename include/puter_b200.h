@@ -136,6 +136,9 @@ CUDABufferRef cuda_buffer_ipc_import(CUDADeviceRef device, const void* handle64,
 int cuda_context_set_stream(CUDADeviceRef device, void* cudaStream, CUDAStatus* status);
 /* NEW: go back to the context's own non-blocking stream */
 int cuda_context_reset_stream(CUDADeviceRef device, CUDAStatus* status);
+/* NEW: frees the scratch and the RoPE tables that captured calls of this context use.  None of the graphs captured so far may be launched
+   afterwards.  Waits for the device; not while a stream is under capture. */
+int cuda_context_release_captures(CUDADeviceRef device, CUDAStatus* status);
 /* NEW: 1 = always use the kernels that reproduce device/cpu operation order exactly
    (sequential sums) in multi-head attention, prefill and packed prefill (paged decode has one form, with either cache);
    0 (default) = use the tensor-core / split-KV kernels where they apply */

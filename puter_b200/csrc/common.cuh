@@ -10,8 +10,6 @@
 #include <string.h>
 #include <stdio.h>
 #include <atomic>
-#include <memory>
-#include <vector>
 
 #include "../../include/puter_b200.h"
 
@@ -27,29 +25,22 @@ struct Buffer {
     int device;
 };
 
-// What a captured call needs for as long as its graph may run: `alive` until CUDA has released the graph, every executable made of it and
-// every launch of those (a user object of the graph says so).
-struct GraphLease {
-    unsigned long long id;  // of the capture
-    std::atomic<int> alive{1};
-};
-
-// One cached cos/sin table.  Captured launches that read it hold it by their leases, work that nothing can wait for by `kept`: a held table
-// is neither overwritten nor freed.  `finished`: known to be built (until then `built` tells); `eager`: eager launches have read it.
+// One cached cos/sin table.  `held`: a captured launch reads it, or work that nothing can wait for, so it is neither overwritten nor freed
+// before cuda_context_release_captures.  `finished`: known to be built (until then `built` tells).
 struct RopeTable {
     float* data;
     size_t bytes;
     double key[10];
-    int valid, kept, finished, eager;
-    std::vector<std::shared_ptr<GraphLease>> leases;
+    int valid, held, finished;
     cudaEvent_t built;
     unsigned long long used;
     RopeTable* next;
 };
 
-// Scratch of the launches captured under one capture; another capture may have it once that graph is gone.
+// Scratch of the launches captured under one capture.  (A user object of the graph could tell when it is gone; with one every replay takes 2.2 to
+// 3 us longer, a decode step of one sequence 13.5 -> 16.5.)
 struct GraphScratch {
-    std::shared_ptr<GraphLease> lease;
+    unsigned long long id;
     char* base;
     size_t bytes;
     int* counters;
@@ -79,10 +70,8 @@ struct Context {
     // cos/sin tables of the last RoPE configurations (positions x headDim/2, cos then sin), reused while a config repeats
     struct RopeTable* ropeTables;
     unsigned long long ropeClock;
-    // scratch of captured calls (see call_scratch), and the lease of the last capture
+    // scratch of captured calls: one list entry per graph (see call_scratch)
     struct GraphScratch* graphScratch;
-    int graphScratchTooSmall;  // a capture found nothing large enough among what earlier ones have left: that is freed
-    std::shared_ptr<GraphLease>* lease;
     // Change of stream (adopt_stream, settle_stream): whatever the adopted stream launches comes after what the streams before it have queued.
     cudaEvent_t streamSwitchEvent;  // behind the work of the streams before
     cudaEvent_t captureEvent;       // (the edges within a capture have an event of their own)
@@ -116,8 +105,6 @@ int check_launch(Context* ctx, CUDAStatus* status, const char* what);
 void* ensure_workspace(Context* ctx, size_t bytes, CUDAStatus* status);
 // capture state of the context's stream; *id (may be null) names the capture
 bool stream_capturing(Context* ctx, unsigned long long* id);
-// the lease of the capture that the context's stream is part of; null (and status) on failure
-std::shared_ptr<GraphLease> capture_lease(Context* ctx, CUDAStatus* status);
 // makes the context's stream wait for the streams before it; called by every entry point while one is outstanding
 int settle_stream(Context* ctx, CUDAStatus* status);
 

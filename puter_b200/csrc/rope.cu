@@ -439,29 +439,8 @@ int build_rope_table(Context* ctx, float* table, size_t seqLen, int headDim, dou
 // float64 angle evaluation runs once per configuration instead of once per call; several tables are kept because a layer may
 // alternate between two (prefill over its own length, cache writes over the whole range of positions).
 // A captured launch keeps the pointer: its table is finished before the capture goes on (a replay may run on a stream that knows
-// nothing of the one it was built on), and neither overwritten nor freed while the graph is there.
+// nothing of the one it was built on), and neither overwritten nor freed before cuda_context_release_captures.
 static constexpr int kRopeTables = 4;  // tables that no captured launch reads, kept at a time
-
-static bool held(RopeTable* t) {
-    for (size_t i = 0; i < t->leases.size();) {
-        if (t->leases[i]->alive.load(std::memory_order_acquire)) {
-            i++;
-            continue;
-        }
-        t->leases[i] = t->leases.back();
-        t->leases.pop_back();
-    }
-    return t->kept || !t->leases.empty();
-}
-
-static bool hold(Context* ctx, RopeTable* t, CUDAStatus* status) {
-    std::shared_ptr<GraphLease> lease = capture_lease(ctx, status);
-    if (!lease) return false;
-    for (auto& have : t->leases)
-        if (have == lease) return true;
-    t->leases.push_back(lease);
-    return true;
-}
 
 // Work that is not to be recorded while the context's stream is being captured.
 struct OutsideCapture {
@@ -490,7 +469,7 @@ static const RopeTable* rope_table(Context* ctx, size_t seqLen, bool exact, int 
     size_t need = made * perPosition;
     const bool capturing = stream_capturing(ctx, nullptr);
     if (!capturing) ctx->scratchUsed = 1;
-    RopeTable *oldest = nullptr, *unread = nullptr;  // the table used longest ago, and a large enough one that launches of graphs alone have read
+    RopeTable* oldest = nullptr;
     int loose = 0;
     for (RopeTable* t = ctx->ropeTables; t; t = t->next) {
         if (t->valid && memcmp(key + 1, t->key + 1, sizeof(key) - sizeof(key[0])) == 0 && (exact ? t->key[0] == key[0] : t->key[0] >= key[0])) {
@@ -503,32 +482,16 @@ static const RopeTable* rope_table(Context* ctx, size_t seqLen, bool exact, int 
                 }
                 t->finished = 1;
             }
-            if (!capturing) t->eager = 1;
-            return !capturing || hold(ctx, t, status) ? t : nullptr;
+            if (capturing) t->held = 1;
+            return t;
         }
-        if (!held(t)) {
+        if (!t->held) {
             loose++;
             if (!oldest || t->used < oldest->used) oldest = t;
-            if (!t->eager && t->bytes >= need) unread = t;
         }
     }
     RelaxedCapture relaxed;  // (another stream may be under capture)
-    if (!capturing && loose > kRopeTables) {  // graphs that are gone have left more
-        cudaStreamSynchronize(ctx->stream);
-        for (; loose > kRopeTables; loose--) {
-            RopeTable** at = &ctx->ropeTables;
-            while (*at != oldest) at = &(*at)->next;
-            *at = oldest->next;
-            cudaFree(oldest->data);
-            cudaEventDestroy(oldest->built);
-            delete oldest;
-            oldest = nullptr;
-            for (RopeTable* t = ctx->ropeTables; t; t = t->next)
-                if (!held(t) && (!oldest || t->used < oldest->used)) oldest = t;
-        }
-    }
-    // (a captured call overwrites nothing that eager launches may still read)
-    RopeTable* t = loose < kRopeTables ? nullptr : capturing ? unread : oldest;
+    RopeTable* t = loose >= kRopeTables && !capturing ? oldest : nullptr;
     if (!t) {
         t = new RopeTable();
         if (cudaEventCreateWithFlags(&t->built, cudaEventDisableTiming) != cudaSuccess) {
@@ -540,7 +503,6 @@ static const RopeTable* rope_table(Context* ctx, size_t seqLen, bool exact, int 
         ctx->ropeTables = t;
     }
     t->valid = t->finished = 0;
-    t->eager = !capturing;
     if (t->bytes < need && t->data) {
         cudaStreamSynchronize(ctx->stream);  // earlier launches may still read the old table
         cudaFree(t->data);
@@ -578,11 +540,10 @@ static const RopeTable* rope_table(Context* ctx, size_t seqLen, bool exact, int 
     if (capturing) {
         OutsideCapture now(ctx);
         if (!fill()) return nullptr;
-        t->finished = 1;
+        t->held = t->finished = 1;
     } else if (!fill()) {
         return nullptr;
     }
-    if (capturing && !hold(ctx, t, status)) return nullptr;  // (outside the guard: the lease is that of the captured stream)
     memcpy(t->key, key, sizeof(key));
     t->valid = 1;
     t->used = ++ctx->ropeClock;

@@ -142,69 +142,18 @@ int settle_stream(Context* ctx, CUDAStatus* status) {
     ctx->decodeCounters = counters;
     for (RopeTable* t = ctx->ropeTables; t; t = t->next) {
         if (t->valid && !t->finished) cudaStreamWaitEvent(ctx->stream, t->built, 0);
-        t->kept = 1;
+        t->held = 1;
     }
     ctx->switchLost = 0;
     return 0;
-}
-
-// A user object's destructor: may run on a thread of CUDA's, calls nothing of it, and may come after the context has closed.
-static void lease_over(void* p) {
-    auto* held = (std::shared_ptr<GraphLease>*)p;
-    (*held)->alive.store(0, std::memory_order_release);
-    delete held;
-}
-
-std::shared_ptr<GraphLease> capture_lease(Context* ctx, CUDAStatus* status) {
-    cudaStreamCaptureStatus state = cudaStreamCaptureStatusNone;
-    unsigned long long id = 0;
-    cudaGraph_t graph = nullptr;
-    cudaError_t err = cudaStreamGetCaptureInfo(ctx->stream, &state, &id, &graph);
-    if (err == cudaSuccess && *ctx->lease && (*ctx->lease)->id == id) return *ctx->lease;
-    auto lease = std::make_shared<GraphLease>();
-    lease->id = id;
-    auto* held = new std::shared_ptr<GraphLease>(lease);
-    cudaUserObject_t object = nullptr;
-    if (err == cudaSuccess) err = cudaUserObjectCreate(&object, held, lease_over, 1, cudaUserObjectNoDestructorSync);
-    if (err != cudaSuccess) {
-        cudaGetLastError();
-        delete held;
-        fail(status, -7, "cuda: holding scratch for a graph failed: %s", cudaGetErrorString(err));
-        return nullptr;
-    }
-    err = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
-    if (err != cudaSuccess) {
-        cudaGetLastError();
-        cudaUserObjectRelease(object, 1);
-        fail(status, -7, "cuda: holding scratch for a graph failed: %s", cudaGetErrorString(err));
-        return nullptr;
-    }
-    *ctx->lease = lease;
-    return lease;
-}
-
-// Frees the scratch of graphs that are gone (which waits for the device: only where a capture could not use it).
-static void free_left_scratch(Context* ctx) {
-    RelaxedCapture relaxed;
-    for (GraphScratch** at = &ctx->graphScratch; *at;) {
-        GraphScratch* g = *at;
-        if (g->lease->alive.load(std::memory_order_acquire)) {
-            at = &g->next;
-            continue;
-        }
-        *at = g->next;
-        cudaFree(g->counters);
-        delete g;
-    }
-    ctx->graphScratchTooSmall = 0;
 }
 
 int call_scratch(Context* ctx, size_t bytes, size_t counterBytes, Scratch* out, CUDAStatus* status) {
     const bool own = counterBytes <= ctx->decodeCounterBytes;  // the kept, always-zero counters hold this call's
     const size_t body = (bytes + 255) & ~(size_t)255;
     const size_t need = body + (own ? 0 : counterBytes) + 512;
-    if (!stream_capturing(ctx, nullptr)) {
-        if (ctx->graphScratchTooSmall) free_left_scratch(ctx);
+    unsigned long long id = 0;
+    if (!stream_capturing(ctx, &id)) {
         char* ws = (char*)ensure_workspace(ctx, need, status);
         if (!ws) return status ? status->code : -7;
         out->base = ws;
@@ -212,41 +161,43 @@ int call_scratch(Context* ctx, size_t bytes, size_t counterBytes, Scratch* out, 
         out->clearCounters = !own;
         return 0;
     }
-    std::shared_ptr<GraphLease> lease = capture_lease(ctx, status);
-    if (!lease) return status ? status->code : -7;
-    GraphScratch *g = ctx->graphScratch, *left = nullptr;
-    bool small = false;
-    for (; g && (g->lease != lease || g->bytes < need); g = g->next) {
-        if (g->lease->alive.load(std::memory_order_acquire)) continue;
-        if (g->bytes < need) small = true;
-        else if (!left || g->bytes < left->bytes) left = g;
-    }
+    GraphScratch* g = ctx->graphScratch;
+    while (g && (g->id != id || g->bytes < need)) g = g->next;
     if (!g) {
         // allocating is not part of the captured work, and neither is clearing, on a stream of the context's own
         RelaxedCapture relaxed;
-        void* p = left ? left->counters : nullptr;
+        void* p = nullptr;
         const size_t total = ctx->decodeCounterBytes + need;
-        cudaError_t err = left ? cudaSuccess : cudaMalloc(&p, total);
+        cudaError_t err = cudaMalloc(&p, total);
         if (err == cudaSuccess) err = cudaMemsetAsync(p, 0, ctx->decodeCounterBytes, ctx->uploadStream);
         if (err == cudaSuccess) err = cudaStreamSynchronize(ctx->uploadStream);
         if (err != cudaSuccess) {
             cudaGetLastError();
-            if (p && !left) cudaFree(p);
+            if (p) cudaFree(p);
             return fail(status, -7, "cuda: scratch of %zu bytes for a captured call failed: %s", total, cudaGetErrorString(err));
         }
-        if (left) {
-            g = left;
-            g->lease = lease;
-        } else {
-            if (small) ctx->graphScratchTooSmall = 1;
-            g = new GraphScratch{lease, (char*)p + ctx->decodeCounterBytes, need, (int*)p, ctx->graphScratch};
-            ctx->graphScratch = g;
-        }
+        g = new GraphScratch{id, (char*)p + ctx->decodeCounterBytes, need, (int*)p, ctx->graphScratch};
+        ctx->graphScratch = g;
     }
     out->base = g->base;
     out->counters = own ? g->counters : (int*)(g->base + body);
     out->clearCounters = !own;
     return 0;
+}
+
+// Frees what captured calls and work set aside have used; none of it is in use any more.
+static void free_held_scratch(Context* ctx) {
+    while (GraphScratch* g = ctx->graphScratch) {
+        ctx->graphScratch = g->next;
+        cudaFree(g->counters);
+        delete g;
+    }
+    while (SetAside* a = ctx->setAside) {
+        ctx->setAside = a->next;
+        cudaFree(a->workspace);
+        cudaFree(a->counters);
+        delete a;
+    }
 }
 
 static std::mutex g_mu;
@@ -288,7 +239,6 @@ int cuda_open_device_index(int ordinal, CUDADeviceRef* outDevice, CUDAStatus* st
     Context* ctx = new Context();
     memset(ctx, 0, sizeof(*ctx));
     ctx->device = ordinal;
-    ctx->lease = new std::shared_ptr<GraphLease>();
     ctx->ccMajor = prop.major;
     ctx->smCount = prop.multiProcessorCount;
     ctx->totalMem = (long long)prop.totalGlobalMem;
@@ -339,24 +289,11 @@ void cuda_close_device(CUDADeviceRef device) {
         delete t;
         t = next;
     }
-    for (GraphScratch* g = ctx->graphScratch; g;) {
-        GraphScratch* next = g->next;
-        cudaFree(g->counters);
-        delete g;
-        g = next;
-    }
-    for (SetAside* a = ctx->setAside; a;) {
-        SetAside* next = a->next;
-        cudaFree(a->workspace);
-        cudaFree(a->counters);
-        delete a;
-        a = next;
-    }
+    free_held_scratch(ctx);
     for (int i = 0; i < 4; i++)
         if (ctx->stageEvents[i]) cudaEventDestroy(ctx->stageEvents[i]);
     if (ctx->streamSwitchEvent) cudaEventDestroy(ctx->streamSwitchEvent);
     if (ctx->captureEvent) cudaEventDestroy(ctx->captureEvent);
-    delete ctx->lease;
     cudaStreamDestroy(ctx->ownStream);
     cudaStreamDestroy(ctx->uploadStream);
     {
@@ -502,6 +439,29 @@ int cuda_context_reset_stream(CUDADeviceRef device, CUDAStatus* status) {
     Context* ctx = ctx_of(device, status);
     if (!ctx) return -1;
     if (ctx->stream != ctx->ownStream) adopt_stream(ctx, ctx->ownStream);
+    return ok(status);
+}
+
+int cuda_context_release_captures(CUDADeviceRef device, CUDAStatus* status) {
+    cuda_status_clear(status);
+    Context* ctx = ctx_of(device, status);
+    if (!ctx) return -1;
+    cudaSetDevice(ctx->device);
+    if (capture_of(ctx->stream, nullptr) != kNotCaptured) return fail(status, -2, "cuda: captures cannot be released while the context's stream is part of one");
+    cudaError_t err = cudaDeviceSynchronize();  // replays may be in flight on any stream
+    if (err != cudaSuccess) return fail(status, -7, "cuda: waiting for the device failed: %s", cudaGetErrorString(err));
+    free_held_scratch(ctx);
+    for (RopeTable** at = &ctx->ropeTables; *at;) {
+        RopeTable* t = *at;
+        if (!t->held) {
+            at = &t->next;
+            continue;
+        }
+        *at = t->next;
+        cudaFree(t->data);
+        cudaEventDestroy(t->built);
+        delete t;
+    }
     return ok(status);
 }
 

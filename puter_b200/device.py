@@ -201,6 +201,11 @@ class Device:
         refs = [self._ref_any(t) for t in items]
         return (ctypes.c_void_p * len(refs))(*[r.value for r in refs])
 
+    def release_captures(self):
+        """Frees the scratch and tables of captured calls.  None of the CUDA graphs captured so far may be replayed afterwards."""
+        self._enter()
+        self._check(self.lib.cuda_context_release_captures(self.ref, ctypes.byref(self._status)))
+
     def set_exact(self, exact: bool):
         self._check(self.lib.cuda_context_set_exact(self.ref, int(exact), ctypes.byref(self._status)))
 

@@ -272,8 +272,8 @@ def free_memory():
 
 
 @pytest.mark.parametrize("eager", [False, True])
-def test_what_a_graph_held_is_free_once_it_is_gone(d, eager):
-    """A program that captures again and again: 4- and 16-bit steps and prompts, each time with another RoPE setting, other lengths."""
+def test_what_captured_calls_hold_is_freed_on_request(d, eager):
+    """A program that captures again and again: 4- and 16-bit steps and prompts, each time with another RoPE setting."""
     import puter_b200
 
     steps = make4(2, [3000, 17, 900], 8, 128, 16, 4, 1)
@@ -299,43 +299,40 @@ def test_what_a_graph_held_is_free_once_it_is_gone(d, eager):
         assert torch.equal(outs[0], wants[0]) and torch.equal(outs[1], wants[1])
         if i in (0, 23):
             assert torch.equal(outs[2], prompt(puter_b200.Device(), *big, 8, 2, 128, 2, rope=rope))
-        if eager:  # (also the table that the next graph would have taken)
-            prompt(d, *big, 8, 2, 128, 2, rope=puter_b200.RoPEConfig(Mode=1, BaseFreq=20000.0 + i // 2), out=outs[2])
+        if eager:
+            other = puter_b200.RoPEConfig(Mode=1, BaseFreq=20000.0 + i // 2)
+            prompt(d, *big, 8, 2, 128, 2, rope=other, out=outs[2])
         graph.reset()
         del graph
+        d.release_captures()
         free.append(free_memory())
     assert free[8] - free[23] < 4 << 20, free  # a graph's scratch and table are 25 MB
     assert d.take_error() == 0
 
 
-def test_scratch_of_a_graph_that_still_runs_is_not_handed_on(d):
-    """A graph is destroyed while its launches wait behind other work: what it holds stays with them, the next capture allocates."""
+def test_release_waits_for_replays_and_is_refused_in_a_capture(d):
     import puter_b200
 
-    rope = puter_b200.RoPEConfig(Mode=1, BaseFreq=500000.0)
-    x = make_prompt(2, [20000, 300], 8, 2, 128, 1)  # 10 MB of rotated K
-    outs = [torch.full_like(x[0], 7.0) for _ in range(2)]
-    run = lambda i: prompt(d, *x, 8, 2, 128, 2, rope=rope, out=outs[i])  # noqa: E731
-    want = run(0).clone()
-    outs[0].fill_(7)
-    graph = torch.cuda.CUDAGraph()
-    first = capture(lambda: run(0))
-    a, b = torch.cuda.Stream(), torch.cuda.Stream()
-    done = torch.cuda.Event()
+    run, outs, wants = prompts(2)
+    graph, a = capture(lambda: run(d, 0)), torch.cuda.Stream()
     with torch.cuda.stream(a):
-        busy(300)
-        first.replay()
-        done.record()
-    first.reset()
-    free = torch.cuda.mem_get_info()[0]
-    raw_capture(graph, b, lambda: run(1))
-    taken = free - torch.cuda.mem_get_info()[0]
-    assert done.query() or taken >= 10 << 20
-    with torch.cuda.stream(b):
+        busy(100)
         graph.replay()
+    d.release_captures()
+    assert torch.equal(outs[0], wants[0])
+    graph.reset()
+
+    def refused():
+        with pytest.raises(puter_b200.DeviceError) as e:
+            d.release_captures()
+        assert e.value.code == -2
+        run(d, 1)
+
+    again = capture(refused)
+    run(d, 0)
+    again.replay()
     torch.cuda.synchronize()
-    assert all(torch.equal(o, want) for o in outs) and d.take_error() == 0
-    print("still running:", taken >> 20, "MB more")
+    assert all(torch.equal(o, w) for o, w in zip(outs, wants)) and d.take_error() == 0
 
 
 @pytest.mark.parametrize("positions", [(1 << 20) + 1, 1 << 20, 1500001])
