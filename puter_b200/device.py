@@ -87,7 +87,6 @@ class SharedBuffer:
 
 
 _NO_TOKEN = ctypes.c_uint64(0)  # completionToken
-_PLAIN = frozenset({int, ctypes.c_double, ctypes.c_int64})  # what passes as it is where no argument types are declared
 
 
 class Device:
@@ -168,13 +167,13 @@ class Device:
         rc = getattr(self.lib, name)(self.ref, *args, ctypes.byref(self._status))
         self._check(rc)
 
-    def _call_plain(self, name, format, tensors, rest):
-        """_call of an entry point (context, format, buffers, rest, token, status): `rest` in the declared types, integers of 32 bits as they are.
-        Anything else (numpy's integers, what has to be refused) is converted by declaration."""
+    def _call_plain(self, name, format, tensors, sizes, rest=()):
+        """_call of an entry point (context, format, buffers, sizes, rest, token, status), sizes of 32 bits, `rest` in the declared types or plain
+        integers.  Sizes that are not Python's integers (then neither is their sum) are converted, or refused, by declaration."""
         self._enter()
-        plain = type(format) is int and _PLAIN.issuperset(map(type, rest))
+        plain = type(sum(sizes, format)) is int
         fn = getattr(self.lib.__dict__.get("plain", self.lib) if plain else self.lib, name)
-        rc = fn(self.ref, format, *self._handles(tensors), *rest, _NO_TOKEN, ctypes.byref(self._status))
+        rc = fn(self.ref, format, *self._handles(tensors), *sizes, *rest, _NO_TOKEN, ctypes.byref(self._status))
         if rc != 0:
             self._check(rc)
 
@@ -443,7 +442,7 @@ class Device:
         rc = rope or RoPEConfig()
         f64 = ctypes.c_double
         self._call_plain("cuda_dispatch_rope_kv_page_write_q4", format, (k, v, positions, pageIDs, offsets, kCodes, kParams, vCodes, vParams),
-                         (rows, kvHeads, headDim, pageCount, pageSize, maxPositions, 2 if rope is None else int(rc.Mode), f64(rc.BaseFreq),
+                         (rows, kvHeads, headDim, pageCount, pageSize, maxPositions), (2 if rope is None else int(rc.Mode), f64(rc.BaseFreq),
                           int(rc.Scaling), f64(rc.ScalingFactor), f64(rc.LowFreqFactor), f64(rc.HighFreqFactor), int(rc.OriginalContext)))
 
     def KVPageGatherQ4(self, codes, params, pageTable, output, pageCount, pageSize, kvHeads, headDim, outRows, format):
@@ -488,7 +487,7 @@ class Device:
         rc = rope or RoPEConfig()
         f64 = ctypes.c_double
         self._call_plain("cuda_dispatch_rope_packed_attention_prefill", format, (query, key, value, seqStarts, output),
-                         (batch, totalTokens, maxSeqLen, attn.NumHeads, kv, attn.HeadDim, int(attn.Causal), 2 if rope is None else int(rc.Mode),
+                         (batch, totalTokens, maxSeqLen, attn.NumHeads, kv, attn.HeadDim), (int(attn.Causal), 2 if rope is None else int(rc.Mode),
                           f64(rc.BaseFreq), ctypes.c_int64(rc.StartPosition), int(rc.Scaling), f64(rc.ScalingFactor), f64(rc.LowFreqFactor),
                           f64(rc.HighFreqFactor), int(rc.OriginalContext)))
 
