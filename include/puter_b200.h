@@ -321,7 +321,7 @@ int cuda_dispatch_rope_kv_page_write(CUDADeviceRef contextRef, int elementDType,
 /* ---- paged KV in 4 bits (no counterpart in the reference) ----
    A vector x of one (token, KV head) is held as 16 levels between its extremes:
      least = round(min x), step = round((max x - min x) * (1 / 15)), code = clamp(rint((x - least) / step), 0, 15), value = least + step * code,
-   round = to elementDType (f16 / bf16).  A vector with a NaN or an infinity reads back as NaN.
+   round = to elementDType (f16 / bf16).  A vector with a NaN or an infinity reads back as NaN, and so does one whose max x - min x leaves float32.
      codes  [pageCount, kvHeads, pageSize, headDim / 2] bytes: byte j = element 2j (low four bits) and 2j + 1 (high)
      params [pageCount, kvHeads, pageSize, 2] elementDType: (step, least)
    headDim is 64 or 128; pools are 16-byte aligned; any page size. */

@@ -35,7 +35,7 @@
 //     sum(p_t least_t) joins them, and the matrix unit cuts its sums off (100001 tokens, 16 heads: error 1.2e-3 of the output with
 //     n, 2.1e-4, the rounding of the output, with n - 8; 46 -> 48 us).
 // Sums, maxima and accumulators are float32.
-// Measured (bf16, 32 heads of 128, page size 16): 64 sequences of 512 to 32768 tokens on 8 KV heads 110 us, 5.1 TB/s (86 us at the copy rate;
+// Measured (bf16, 32 heads of 128, page size 16): 64 sequences of 512 to 32768 tokens on 8 KV heads 109 us, 5.2 TB/s (86 us at the copy rate;
 // the steps between the first and the last stream 6.1 TB/s, the rest is the start and the joins); two of 131072 tokens on 4 KV heads 44 us,
 // on 2 KV heads 40; one of 1024 tokens 12 us, of which 2 are the launch, 2 the prefix, 3 the first copies, 3 the step itself, 2 the joins.
 //

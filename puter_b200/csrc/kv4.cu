@@ -5,8 +5,11 @@
 //     least = rn16(min x),  step = rn16((max x - min x) * (1 / 15)),  code_d = clamp(rint((x_d - least) / step), 0, 15),
 //     value_d = least + step * code_d,
 // rn16 = rounding to the 16-bit type of the tensors (their range: a bf16 vector may hold 1e30).  The codes are chosen against the
-// rounded step and least, so that rounding costs no accuracy but the cover of the extremes (at most 15 / 512 of a step in bf16).
-// A vector that holds a NaN or an infinity gets a NaN step: it reads back as NaN, never as finite numbers.
+// rounded step and least, so that rounding costs no accuracy but the cover of the extremes: in bf16 up to 15 / 256 of a step for the step's and
+// 2^-8 of least for its own (0.4 of a step where least is a hundred steps), in f16 an eighth of both.
+// A vector that holds a NaN or an infinity gets a step that is one of them: it reads back as NaN, never as finite numbers.  So does a finite one
+// whose extremes lie further apart than float32 reaches (3.4e38, bf16).  K is rotated in float32 and not rounded before: a rotation that leaves f16
+// (by a factor of 1.41 at most) gives an infinite least, as it gives an infinite element where K is kept in 16 bits.
 //
 // Layout: codes [page, kvHead, token, D / 2] bytes, byte j = element 2j in the low and 2j + 1 in the high four bits; params
 // [page, kvHead, token, 2] = (step, least).  The head comes before the token so that the 16 tokens that a warp of the decode kernel
@@ -97,8 +100,8 @@ __device__ __forceinline__ void quantise(const float* x, uint32_t& c0, uint32_t&
     float step = __fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f), least = lo;
     params = round_pair_arith<DT>(step, least);
     const float inv = 1.0f / step;
-    // no element falls below level -0.2 or above 15.25 while the rounding of least (2^-9 of it at most) stays below 0.2 of a step and the
-    // step is a normal number of its type: then rounding alone keeps 0 .. 15
+    // no element falls below level -0.4 or above 15.46 while the rounding of least (2^-8 of it at most) stays below 0.4 of a step and the
+    // step is a normal number of its type (2^-8 off at most): then rounding alone keeps 0 .. 15
     const bool plain = fabsf(least) <= 100.f * step && step >= (DT == DT_F16 ? 6.103515625e-5f : 1e-30f) && step < INFINITY;
     if (__all_sync(0xffffffffu, plain)) {
         c0 = levels8(x, step, least, inv);
@@ -119,10 +122,10 @@ template <int DT> __device__ __forceinline__ void widen8(const Vec16& v, float* 
 }
 
 // MODE 0: neighbouring pairs, 1: halves, 2: K comes rotated.
-// Bound: instructions, ~10 per element against the 14 that the memory system leaves time for; every lane has 64 bytes of K and V in flight before it
-// looks at its indices.  59748 rows of 8 KV heads of 128 in bf16, rotated: 70 us for 310 MB, 4.5 TB/s (47 us at the copy rate; issue slots 60 %,
-// logic pipe 49 %); 64 rows 2.7 us.  The next vectors fetched a round ahead made it slower (78 us in
-// registers, 74 through shared memory).
+// Bound: no pipe is full (~10 instructions per element against the 14 that the memory system leaves time for; issue slots 65 %, logic pipe 49 %): a
+// warp waits for its loads, and 60 registers leave four blocks on an SM.  Every lane has 64 bytes of K and V in flight before it looks at its
+// indices.  59748 rows of 8 KV heads of 128 in bf16, rotated: 70 us for 310 MB, 4.5 TB/s (47 us at the copy rate); 64 rows 2.7 us.  The next
+// vectors fetched a round ahead made it slower (78 us in registers, 74 through shared memory).
 template <int DT, int D, int MODE>
 __global__ void __launch_bounds__(256) append_kernel(const uint16_t* __restrict__ k, const uint16_t* __restrict__ v,
                                                      const int32_t* __restrict__ positions, const int32_t* __restrict__ pageIDs,
@@ -254,7 +257,8 @@ __global__ void __launch_bounds__(256) gather_kernel(const uint8_t* __restrict__
 }
 
 static int grid_of(Context* ctx, size_t warps) {
-    const size_t blocks = (warps + 8) / 8, cap = (size_t)ctx->smCount * 8;  // 8 blocks of 256 threads fill an SM
+    // 8 blocks of 256 threads fill an SM in the gather; the producer's registers leave room for 4, and 4, 8 and 16 times the SMs take it equally long
+    const size_t blocks = (warps + 8) / 8, cap = (size_t)ctx->smCount * 8;
     return (int)(blocks < cap ? (blocks ? blocks : 1) : cap);
 }
 

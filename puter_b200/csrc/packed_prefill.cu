@@ -23,9 +23,14 @@
 //     that is not finite would still reach every row of the tile through 0 * NaN, so a warp looks through the value tiles that are not
 //     seen by all rows, clears what is not finite, and the rows that do see it add it back at the end.
 //   * The last rows of a sequence share their TMA box with the next sequence, so that box is written row by row.
-// Bound: the softmax of a tile between its two products (one row a thread, 128 exponentials) and, in long calls, the power limit.  bf16, 32 heads
-// on 8 KV heads of 128, RoPE included: eight prompts of 150 to 4096 tokens 305 us, 1.06 PFLOP/s counting what the mask leaves (193 us at the
-// dense rate; 12 us are the list and K's rotation, a pass over K in memory), one of 16384 tokens 1.63 to 1.8 ms, 1.2 to 1.35 PFLOP/s.
+// Roundings to 16 bits: rotated q and k, as the framework's RoPE stores them and its other prefill uses them; the weights before P V, because one
+// tcgen05 product takes one type for both operands and V comes in 16 bits (the sum of the weights stays in float32 and is not rounded).  In
+// bf16 the weights leave an error of 1.8 to 2.0e-3 of the output's norm and RoPE 2.1 to 2.8e-3 (33 to 1500 tokens), where rounding the output alone
+// leaves 1.6e-3; in f16 2.2 to 2.6e-4 and 2.7 to 3.5e-4 of 2.0e-4.  Maxima, sums and accumulators are float32.
+// Bound: the softmax of a tile between its two products (one row a thread, 128 exponentials; counters: tensor pipe 52 % of the cycles, exponentials
+// 53 %, issue slots 38 %) and, in long calls, the power limit.  bf16, 32 heads on 8 KV heads of 128, RoPE included: eight prompts of 150 to 4096
+// tokens 301 to 309 us, 1.04 to 1.07 PFLOP/s counting what the mask leaves (193 us at the dense rate; 12 us are the list and K's rotation, a pass over K in
+// memory), one of 16384 tokens 1.65 to 1.8 ms, 1.2 to 1.35 PFLOP/s, and 1.87 ms when called again and again.
 #include <math.h>
 
 #include "common.cuh"
