@@ -54,8 +54,8 @@ int check_launch(Context* ctx, CUDAStatus* status, const char* what) {
 
 void* ensure_workspace(Context* ctx, size_t bytes, CUDAStatus* status) {
     ctx->scratchUsed = 1;
-    RelaxedCapture relaxed;  // (another stream may be under capture)
     if (bytes <= ctx->workspaceBytes) return ctx->workspace;
+    RelaxedCapture relaxed;  // (another stream may be under capture)
     // grow-only; the old block may still be in use by work queued on the stream
     if (ctx->workspace) {
         cudaStreamSynchronize(ctx->stream);
