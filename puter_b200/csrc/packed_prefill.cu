@@ -874,12 +874,6 @@ __device__ __forceinline__ void ldmatrix_trans(uint32_t at, uint32_t* r) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-
 // sum + 0 * v for two elements: 0 while all are finite, NaN from the first that is not
 template <bool BF16> __device__ __forceinline__ uint32_t times0(uint32_t v, uint32_t sum) {
     uint32_t d;
@@ -1049,8 +1043,8 @@ __global__ void __launch_bounds__(kShortWarps<D> * 32) short_kernel(ShortParams 
             float topA = fmaxf(s[0][0], s[0][1]), topB = fmaxf(s[0][2], s[0][3]);
 #pragma unroll
             for (int n = 1; n < 4; n++) {
-                topA = max3(topA, s[n][0], s[n][1]);
-                topB = max3(topB, s[n][2], s[n][3]);
+                topA = fmax3(topA, s[n][0], s[n][1]);
+                topB = fmax3(topB, s[n][2], s[n][3]);
             }
             topA = fmaxf(topA, __shfl_xor_sync(0xffffffffu, topA, 1));
             topB = fmaxf(topB, __shfl_xor_sync(0xffffffffu, topB, 1));
